@@ -16,7 +16,9 @@ DTYPE_BF16, DTYPE_FP32 = 0, 1
 EXPORTED = ("geoattn_version", "geoattn_error_string", "geoattn_prior_bytes", "geoattn_prior_from_dense",
             "geoattn_prior_from_coords", "geoattn_stats_bytes", "geoattn_fwd_workspace_bytes",
             "geoattn_bwd_workspace_bytes", "geoattn_fwd", "geoattn_bwd", "geoattn_bwd_noalloc",
-            "geoattn_read_status", "geoattn_wait_selftest")
+            "geoattn_read_status", "geoattn_wait_selftest", "geoattn_xattn_fwd_workspace_bytes",
+            "geoattn_xattn_bwd_workspace_bytes", "geoattn_xattn_fwd", "geoattn_xattn_bwd",
+            "geoattn_distance_buckets", "geoattn_dropout", "geoattn_rng_take")
 
 c_ll4 = ctypes.c_longlong * 4
 
@@ -42,6 +44,30 @@ class BwdArgs(ctypes.Structure):
                 ("dq", ctypes.c_void_p), ("dq_stride", c_ll4), ("dk", ctypes.c_void_p), ("dk_stride", c_ll4),
                 ("dv", ctypes.c_void_p), ("dv_stride", c_ll4), ("dabg", ctypes.c_void_p),
                 ("workspace", ctypes.c_void_p), ("events", ctypes.c_void_p)]
+
+
+class XattnShape(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("batch", "heads", "kv_heads", "nq", "nk", "head_dim", "dtype", "buckets",
+                                            "table_dtype")]
+
+
+class XattnInputs(ctypes.Structure):
+    _fields_ = [("shape", XattnShape), ("q", Tensor), ("k", Tensor), ("v", Tensor), ("ids", ctypes.c_void_p),
+                ("ids_ld", ctypes.c_longlong), ("table", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p),
+                ("key_mask", ctypes.c_void_p), ("key_mask_ld", ctypes.c_longlong), ("rng", ctypes.c_void_p),
+                ("drop_threshold", ctypes.c_int), ("scale", ctypes.c_float)]
+
+
+class XattnFwdArgs(ctypes.Structure):
+    _fields_ = [("inputs", XattnInputs), ("o", ctypes.c_void_p), ("o_stride", c_ll4), ("stats", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p)]
+
+
+class XattnBwdArgs(ctypes.Structure):
+    _fields_ = [("inputs", XattnInputs), ("o", Tensor), ("dout", Tensor), ("stats", ctypes.c_void_p),
+                ("dq", ctypes.c_void_p), ("dq_stride", c_ll4), ("dk", ctypes.c_void_p), ("dk_stride", c_ll4),
+                ("dv", ctypes.c_void_p), ("dv_stride", c_ll4), ("dtable", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p)]
 
 
 class GeoAttnError(RuntimeError):
@@ -86,6 +112,20 @@ def lib():
         L.geoattn_read_status.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_int), ctypes.c_void_p]
         L.geoattn_wait_selftest.restype = ctypes.c_int
         L.geoattn_wait_selftest.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+        xp, vp, ci = ctypes.POINTER(XattnShape), ctypes.c_void_p, ctypes.c_int
+        for fn in ("geoattn_xattn_fwd_workspace_bytes", "geoattn_xattn_bwd_workspace_bytes"):
+            getattr(L, fn).restype = ctypes.c_size_t
+            getattr(L, fn).argtypes = [xp]
+        L.geoattn_xattn_fwd.restype = ci
+        L.geoattn_xattn_fwd.argtypes = [ctypes.POINTER(XattnFwdArgs), vp]
+        L.geoattn_xattn_bwd.restype = ci
+        L.geoattn_xattn_bwd.argtypes = [ctypes.POINTER(XattnBwdArgs), vp]
+        L.geoattn_distance_buckets.restype = ci
+        L.geoattn_distance_buckets.argtypes = [ci, vp, vp, ci, vp, vp, vp, ci, ctypes.c_double, vp, vp]
+        L.geoattn_dropout.restype = ci
+        L.geoattn_dropout.argtypes = [ci, ctypes.c_longlong, vp, vp, vp, vp, ci, vp]
+        L.geoattn_rng_take.restype = ci
+        L.geoattn_rng_take.argtypes = [vp, vp, vp]
         if L.geoattn_version() != ABI_VERSION:  # argument structs of another layout: refuse before any call
             raise RuntimeError("%s has ABI version %d, this binding expects %d; rebuild it"
                                % (LIB_PATH, L.geoattn_version(), ABI_VERSION))

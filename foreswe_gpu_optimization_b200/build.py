@@ -5,10 +5,11 @@ import subprocess
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libgeoattn.so")
-SOURCES = ("geoattn.cu",)
-HEADERS = ("geoattn_kernels.cuh", "sm100.cuh", "tma_host.h")
-NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo", "-shared",
-              "-Xcompiler", "-fPIC"]
+OBJ = os.path.join(HERE, "_build")
+SOURCES = ("geoattn.cu", "xattn.cu")
+HEADERS = {"geoattn.cu": ("geoattn_kernels.cuh", "sm100.cuh", "tma_host.h", "host_util.h"),
+           "xattn.cu": ("xattn_common.cuh", "xattn_simt.cuh", "xattn_aux.cuh", "philox.cuh", "host_util.h")}
+NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC"]
 
 
 def nvcc():
@@ -16,24 +17,42 @@ def nvcc():
     return cand if os.path.exists(cand) else "nvcc"
 
 
-def _stale():
-    if not os.path.exists(OUT):
-        return True
-    t = os.path.getmtime(OUT)
-    deps = [os.path.join(CSRC, f) for f in SOURCES + HEADERS]
-    deps.append(os.path.join(HERE, "..", "include", "geoattn.h"))
-    return any(os.path.getmtime(f) > t for f in deps)
+def _deps(src):
+    return [os.path.join(CSRC, f) for f in (src,) + HEADERS[src]] + [os.path.join(HERE, "..", "include", "geoattn.h")]
+
+
+def _newer(target, deps):
+    if not os.path.exists(target):
+        return False
+    t = os.path.getmtime(target)
+    return all(os.path.getmtime(f) <= t for f in deps)
 
 
 def build(force=False, verbose=False):
-    """Compile csrc/geoattn.cu into libgeoattn.so next to this file; returns the path."""
-    if not force and not _stale():
+    """Compile csrc/*.cu (in parallel, those that changed) and link libgeoattn.so next to this file; returns the path."""
+    if not force and _newer(OUT, [d for s in SOURCES for d in _deps(s)]):
         return OUT
-    cmd = [nvcc(), *NVCC_FLAGS, "-o", OUT + ".tmp", os.path.join(CSRC, "geoattn.cu")]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-    subprocess.run(cmd, check=True, capture_output=not verbose)
-    os.replace(OUT + ".tmp", OUT)
+    os.makedirs(OBJ, exist_ok=True)
+    objs, jobs = [], []
+    for src in SOURCES:
+        obj = os.path.join(OBJ, src[:-3] + ".o")
+        objs.append(obj)
+        if not force and _newer(obj, _deps(src)):
+            continue
+        tmp = "%s.%d" % (obj, os.getpid())
+        cmd = [nvcc(), *NVCC_FLAGS, "-c", "-o", tmp, os.path.join(CSRC, src)]
+        if verbose:
+            cmd.insert(1, "-Xptxas=-v")
+        jobs.append((cmd, tmp, obj, subprocess.Popen(cmd, stdout=None if verbose else subprocess.PIPE,
+                                                     stderr=None if verbose else subprocess.STDOUT)))
+    done = [(cmd, tmp, obj, p, p.communicate()[0]) for cmd, tmp, obj, p in jobs]
+    for cmd, tmp, obj, p, out in done:
+        if p.returncode:
+            raise subprocess.CalledProcessError(p.returncode, cmd, output=out)
+        os.replace(tmp, obj)
+    tmp = "%s.%d" % (OUT, os.getpid())
+    subprocess.run([nvcc(), *NVCC_FLAGS, "-shared", "-o", tmp, *objs], check=True, capture_output=not verbose)
+    os.replace(tmp, OUT)
     return OUT
 
 

@@ -10,6 +10,7 @@
 
 #include "../../include/geoattn.h"
 #include "geoattn_kernels.cuh"
+#include "host_util.h"
 #include "tma_host.h"
 
 namespace geoattn {
@@ -231,9 +232,6 @@ __global__ void wait_selftest_kernel(int* status) {
 // ---------------------------------------------------------------------------------------------------------------
 namespace {
 
-constexpr size_t kAlign = 256;
-inline size_t align_up(size_t x) { return (x + kAlign - 1) / kAlign * kAlign; }
-
 struct Dims {
   int B, H, N, D, DP, nrb, np;
   bool bf16;
@@ -247,21 +245,6 @@ inline bool uses_ds(const Dims&) { return true; }
 
 // Row records per query row (m1, c2, delta1, delta2; fp32 above head dim 64 also b, for the key pass's d(alpha)).
 inline int nrec(const Dims& d) { return (!d.bf16 && d.DP > 64) ? 5 : 4; }
-
-// Every data pointer handed to a kernel must be memory of the current device (or managed memory): the kernels run
-// on the current device, which would dereference a host pointer or another device's memory. Checked on the host
-// before any launch.
-bool dev_ptr(const void* p) {
-  if (!p) return false;
-  cudaPointerAttributes a;
-  if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
-    cudaGetLastError();  // clear the sticky-free error of an unregistered host pointer
-    return false;
-  }
-  if (a.type == cudaMemoryTypeManaged) return true;
-  int cur = -1;
-  return a.type == cudaMemoryTypeDevice && cudaGetDevice(&cur) == cudaSuccess && a.device == cur;
-}
 
 int check_shape(const GeoAttnShape* s, Dims& d) {
   if (!s || s->batch <= 0 || s->heads <= 0 || s->n <= 0 || s->head_dim <= 0) return GEOATTN_ERR_INVALID;

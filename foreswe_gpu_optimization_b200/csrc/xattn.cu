@@ -1,0 +1,319 @@
+// Host launchers of the cross attention, its bucketed bias and dropout, behind the C ABI in include/geoattn.h.
+#include <cmath>
+#include <cstdint>
+#include <cstring>
+
+#include "../../include/geoattn.h"
+#include "host_util.h"
+#include "xattn_aux.cuh"
+#include "xattn_simt.cuh"
+
+namespace geoattn {
+namespace {
+
+constexpr int kSMs = 148;  // B200
+
+// Most dS^T scratch of one backward launch. Larger problems run in several launches over (batch, key head) units, so
+// that the scratch stays bounded; below this size a launch already fills the GPU.
+constexpr size_t kDsCap = (size_t)4 << 30;
+
+struct XDims {
+  int B, H, Hkv, G, Nq, Nk, D, DP, T, nqp, nkp;
+  bool bf16;
+  int splits;           // forward key splits
+  int units_per_launch; // backward
+  int launches, chunks;
+  size_t ds_unit;       // dS^T bytes of one (batch, key head) unit
+};
+
+int forward_splits(const XDims& d) {
+  // enough key ranges to give every SM a tile when the rows alone do not; each range keeps at least 4 key tiles
+  const long long tiles = (long long)((d.Nq + 127) / 128) * d.B * d.H;
+  const int ktiles = (d.Nk + 63) / 64;
+  if (tiles >= kSMs || ktiles < 8) return 1;
+  const long long want = (2 * kSMs + tiles - 1) / tiles;
+  const long long most = ktiles / 4;
+  return (int)(want < most ? want : most);
+}
+
+int check_xshape(const GeoXattnShape* s, XDims& d) {
+  if (!s || s->batch <= 0 || s->heads <= 0 || s->kv_heads <= 0 || s->nq <= 0 || s->nk <= 0 || s->head_dim <= 0 ||
+      s->heads % s->kv_heads || s->buckets < 0)
+    return GEOATTN_ERR_INVALID;
+  if (s->dtype != GEOATTN_DTYPE_BF16 && s->dtype != GEOATTN_DTYPE_FP32) return GEOATTN_ERR_INVALID;
+  if (s->table_dtype != GEOATTN_DTYPE_BF16 && s->table_dtype != GEOATTN_DTYPE_FP32) return GEOATTN_ERR_INVALID;
+  if (s->head_dim > 192 || s->buckets > kMaxBuckets) return GEOATTN_ERR_UNSUPPORTED;
+  d.B = s->batch, d.H = s->heads, d.Hkv = s->kv_heads, d.G = d.H / d.Hkv;
+  d.Nq = s->nq, d.Nk = s->nk, d.D = s->head_dim, d.T = s->buckets;
+  d.DP = d.D <= 64 ? 64 : d.D <= 128 ? 128 : 192;
+  d.bf16 = s->dtype == GEOATTN_DTYPE_BF16;
+  // rows and keys fit an int after padding, and so do a launch's CTAs
+  if (d.Nq > (1 << 30) || d.Nk > (1 << 30) || (long long)d.B * d.H > (1 << 30)) return GEOATTN_ERR_UNSUPPORTED;
+  d.nqp = (d.Nq + 63) / 64 * 64;
+  d.nkp = (d.Nk + 127) / 128 * 128;
+  d.splits = forward_splits(d);
+  const long long qt = (d.Nq + 63) / 64, kt = (d.Nk + 31) / 32;
+  if (qt * d.B * d.H * d.splits > (1ll << 30) || kt * d.B * d.Hkv > (1ll << 30)) return GEOATTN_ERR_UNSUPPORTED;
+  d.ds_unit = (size_t)d.G * d.nkp * d.nqp * 4;
+  const long long units = (long long)d.B * d.Hkv;
+  long long per = (long long)(kDsCap / d.ds_unit);
+  per = per < 1 ? 1 : per > units ? units : per;
+  d.units_per_launch = (int)per;
+  d.launches = (int)((units + per - 1) / per);
+  const long long want = (8ll * kSMs + d.H - 1) / d.H, most = ((long long)d.Nk * d.nqp / 4 + 255) / 256;
+  d.chunks = (int)(want < most ? want : most);
+  return GEOATTN_OK;
+}
+
+struct XFwdWs {
+  int* status;
+  float *part_o, *part_ml;
+};
+size_t xfwd_ws(const XDims& d, uint8_t* base, XFwdWs* w) {
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    uint8_t* p = base ? base + off : nullptr;
+    off += align_up(bytes);
+    return p;
+  };
+  XFwdWs t{};
+  t.status = reinterpret_cast<int*>(take(sizeof(int)));
+  if (d.splits > 1) {
+    const size_t rows = (size_t)d.splits * d.B * d.H * d.Nq;
+    t.part_o = reinterpret_cast<float*>(take(rows * d.D * 4));
+    t.part_ml = reinterpret_cast<float*>(take(rows * 2 * 4));
+  }
+  if (w) *w = t;
+  return off;
+}
+
+struct XBwdWs {
+  int* status;
+  float* delta;
+  void* ds;
+  uint8_t* idsT;
+  float* part;
+};
+size_t xbwd_ws(const XDims& d, uint8_t* base, XBwdWs* w) {
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    uint8_t* p = base ? base + off : nullptr;
+    off += align_up(bytes);
+    return p;
+  };
+  XBwdWs t{};
+  t.status = reinterpret_cast<int*>(take(sizeof(int)));
+  t.delta = reinterpret_cast<float*>(take((size_t)d.B * d.H * d.Nq * 4));
+  t.ds = take(d.ds_unit * d.units_per_launch);
+  if (d.T) {
+    t.idsT = take((size_t)d.nkp * d.nqp);
+    t.part = reinterpret_cast<float*>(take((size_t)d.launches * d.H * d.chunks * d.T * 4));
+  }
+  if (w) *w = t;
+  return off;
+}
+
+int status_of(cudaError_t e) { return e == cudaSuccess ? GEOATTN_OK : GEOATTN_ERR_LAUNCH; }
+
+XTensor xt(const void* p, const long long* s) {
+  XTensor t;
+  t.p = const_cast<void*>(p);
+  for (int i = 0; i < 3; ++i) t.s[i] = s[i];
+  return t;
+}
+
+int check_inputs(const GeoXattnInputs& a, const XDims& d) {
+  if (!dev_ptr(a.q.data) || !dev_ptr(a.k.data) || !dev_ptr(a.v.data)) return GEOATTN_ERR_INVALID;
+  if (d.T && (!dev_ptr(a.ids) || !dev_ptr(a.table) || a.ids_ld < d.Nk)) return GEOATTN_ERR_INVALID;
+  if (a.kv_lens && !dev_ptr(a.kv_lens)) return GEOATTN_ERR_INVALID;
+  if (a.key_mask && (!dev_ptr(a.key_mask) || a.key_mask_ld < d.Nk)) return GEOATTN_ERR_INVALID;
+  if (a.drop_threshold < 0 || a.drop_threshold > 65536 || (a.drop_threshold > 0 && !dev_ptr(a.rng)))
+    return GEOATTN_ERR_INVALID;
+  for (const GeoAttnTensor* t : {&a.q, &a.k, &a.v})
+    if (t->stride[3] != 1) return GEOATTN_ERR_ALIGNMENT;
+  return GEOATTN_OK;
+}
+
+XParams xparams(const GeoXattnInputs& a, const XDims& d) {
+  XParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.B = d.B, p.H = d.H, p.Hkv = d.Hkv, p.G = d.G, p.Nq = d.Nq, p.Nk = d.Nk, p.D = d.D, p.T = d.T;
+  p.q = xt(a.q.data, a.q.stride), p.k = xt(a.k.data, a.k.stride), p.v = xt(a.v.data, a.v.stride);
+  if (d.T) {
+    p.ids = a.ids, p.ids_ld = a.ids_ld, p.table = a.table;
+    p.table_bf16 = a.shape.table_dtype == GEOATTN_DTYPE_BF16;
+  }
+  p.lens = a.kv_lens, p.kmask = a.key_mask, p.kmask_ld = a.key_mask_ld;
+  p.rng = a.rng, p.drop_thr = a.drop_threshold;
+  p.drop_scale = a.drop_threshold >= 65536 ? 0.f : (float)(65536.0 / (65536 - a.drop_threshold));
+  p.scale = a.scale, p.scale_log2 = (float)((double)a.scale * 1.4426950408889634);
+  p.nqp = d.nqp, p.nkp = d.nkp, p.splits = 1;
+  return p;
+}
+
+template <class K>
+int xlaunch(K kernel, long long grid, int threads, int smem, cudaStream_t st, const XParams& p) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return GEOATTN_ERR_LAUNCH;
+  kernel<<<(unsigned)grid, threads, smem, st>>>(p);
+  return status_of(cudaGetLastError());
+}
+
+template <class E, int DP>
+int simt_fwd(const XParams& p, cudaStream_t st) {
+  return xlaunch(xattn_simt_fwd_kernel<E, DP>, (long long)((p.Nq + 127) / 128) * p.B * p.H * p.splits, kSimtThreads,
+                 SimtFwd<DP>::SMEM, st, p);
+}
+template <class E>
+int simt_fwd_any(const XParams& p, const XDims& d, cudaStream_t st) {
+  return d.DP == 64 ? simt_fwd<E, 64>(p, st) : d.DP == 128 ? simt_fwd<E, 128>(p, st) : simt_fwd<E, 192>(p, st);
+}
+template <class E, int DP>
+int simt_bwd(const XParams& p, int units, cudaStream_t st) {
+  using C = SimtBwd<DP>;
+  int rc = xlaunch(xattn_simt_bwd_keys_kernel<E, DP>, (long long)((p.Nk + C::TK - 1) / C::TK) * units, kSimtThreads,
+                   C::SMEM, st, p);
+  if (rc) return rc;
+  return xlaunch(xattn_simt_bwd_dq_kernel<E, DP>, (long long)((p.Nq + 63) / 64) * units * p.G, kSimtThreads,
+                 SimtDq<DP>::SMEM, st, p);
+}
+template <class E>
+int simt_bwd_any(const XParams& p, const XDims& d, int units, cudaStream_t st) {
+  return d.DP == 64 ? simt_bwd<E, 64>(p, units, st)
+                    : d.DP == 128 ? simt_bwd<E, 128>(p, units, st) : simt_bwd<E, 192>(p, units, st);
+}
+
+}  // namespace
+}  // namespace geoattn
+
+using namespace geoattn;
+
+extern "C" {
+
+size_t geoattn_xattn_fwd_workspace_bytes(const GeoXattnShape* shape) {
+  XDims d;
+  return check_xshape(shape, d) ? 0 : xfwd_ws(d, nullptr, nullptr);
+}
+
+size_t geoattn_xattn_bwd_workspace_bytes(const GeoXattnShape* shape) {
+  XDims d;
+  return check_xshape(shape, d) ? 0 : xbwd_ws(d, nullptr, nullptr);
+}
+
+int geoattn_xattn_fwd(const GeoXattnFwdArgs* a, void* stream) {
+  if (!a) return GEOATTN_ERR_INVALID;
+  XDims d;
+  if (int rc = check_xshape(&a->in.shape, d)) return rc;
+  if (int rc = check_inputs(a->in, d)) return rc;
+  if (!dev_ptr(a->o) || (a->stats && !dev_ptr(a->stats)) || !dev_ptr(a->workspace)) return GEOATTN_ERR_INVALID;
+  if (a->o_stride[3] != 1 || (reinterpret_cast<uintptr_t>(a->workspace) & (kAlign - 1))) return GEOATTN_ERR_ALIGNMENT;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  XFwdWs ws;
+  xfwd_ws(d, reinterpret_cast<uint8_t*>(a->workspace), &ws);
+  XParams p = xparams(a->in, d);
+  p.o = xt(a->o, a->o_stride), p.stats = reinterpret_cast<float2*>(a->stats);
+  p.splits = d.splits, p.part_o = ws.part_o, p.part_ml = ws.part_ml, p.status = ws.status;
+  int rc = d.bf16 ? simt_fwd_any<__nv_bfloat16>(p, d, st) : simt_fwd_any<float>(p, d, st);
+  if (rc || d.splits == 1) return rc;
+  const long long rows = (long long)d.B * d.H * d.Nq;
+  return d.bf16 ? xlaunch(xattn_combine_kernel<__nv_bfloat16>, (rows + 7) / 8, 256, 0, st, p)
+                : xlaunch(xattn_combine_kernel<float>, (rows + 7) / 8, 256, 0, st, p);
+}
+
+int geoattn_xattn_bwd(const GeoXattnBwdArgs* a, void* stream) {
+  if (!a) return GEOATTN_ERR_INVALID;
+  XDims d;
+  if (int rc = check_xshape(&a->in.shape, d)) return rc;
+  if (int rc = check_inputs(a->in, d)) return rc;
+  if (!dev_ptr(a->o.data) || !dev_ptr(a->dout.data) || !dev_ptr(a->stats) || !dev_ptr(a->dq) || !dev_ptr(a->dk) ||
+      !dev_ptr(a->dv) || (d.T && !dev_ptr(a->dtable)) || !dev_ptr(a->workspace))
+    return GEOATTN_ERR_INVALID;
+  if (a->o.stride[3] != 1 || a->dout.stride[3] != 1 || a->dq_stride[3] != 1 || a->dk_stride[3] != 1 ||
+      a->dv_stride[3] != 1 || (reinterpret_cast<uintptr_t>(a->workspace) & (kAlign - 1)))
+    return GEOATTN_ERR_ALIGNMENT;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  XBwdWs ws;
+  xbwd_ws(d, reinterpret_cast<uint8_t*>(a->workspace), &ws);
+  XParams p = xparams(a->in, d);
+  p.o = xt(a->o.data, a->o.stride), p.dout = xt(a->dout.data, a->dout.stride);
+  p.dq = xt(a->dq, a->dq_stride), p.dk = xt(a->dk, a->dk_stride), p.dv = xt(a->dv, a->dv_stride);
+  p.stats = reinterpret_cast<float2*>(const_cast<float*>(a->stats)), p.delta = ws.delta, p.ds = ws.ds, p.idsT = ws.idsT, p.status = ws.status;
+  const long long rows = (long long)d.B * d.H * d.Nq;
+  int rc = d.bf16 ? xlaunch(xattn_delta_kernel<__nv_bfloat16>, (rows + 7) / 8, 256, 0, st, p)
+                  : xlaunch(xattn_delta_kernel<float>, (rows + 7) / 8, 256, 0, st, p);
+  if (rc) return rc;
+  if (d.T) {
+    ids_transpose_kernel<<<dim3(d.nqp / 64, d.nkp / 64), 256, 0, st>>>(p.ids, p.ids_ld, d.Nq, d.Nk, d.nqp, ws.idsT);
+    if ((rc = status_of(cudaGetLastError()))) return rc;
+  }
+  const int units = d.B * d.Hkv;
+  for (int l = 0; l < d.launches; ++l) {
+    p.u0 = l * d.units_per_launch;
+    const int nu = units - p.u0 < d.units_per_launch ? units - p.u0 : d.units_per_launch;
+    rc = d.bf16 ? simt_bwd_any<__nv_bfloat16>(p, d, nu, st) : simt_bwd_any<float>(p, d, nu, st);
+    if (rc) return rc;
+    if (d.T) {
+      float* part = ws.part + (size_t)l * d.H * d.chunks * d.T;
+      if (cudaFuncSetAttribute(table_grad_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               kMaxBuckets * 1024) != cudaSuccess)
+        return GEOATTN_ERR_LAUNCH;
+      table_grad_kernel<float><<<dim3(d.chunks, d.H), 256, d.T * 1024, st>>>(p, nu, part);
+      if ((rc = status_of(cudaGetLastError()))) return rc;
+    }
+  }
+  if (d.T) {
+    table_grad_sum_kernel<<<d.H * d.T, 32, 0, st>>>(ws.part, d.launches, d.H, d.chunks, d.T, a->dtable,
+                                                    a->in.shape.table_dtype == GEOATTN_DTYPE_BF16);
+    rc = status_of(cudaGetLastError());
+  }
+  return rc;
+}
+
+int geoattn_distance_buckets(int nq, const double* lat_q, const double* lon_q, int nk, const double* lat_k,
+                             const double* lon_k, const double* edges, int nedges, double max_km, unsigned char* ids,
+                             void* stream) {
+  if (nq <= 0 || nk <= 0 || nedges < 0) return GEOATTN_ERR_INVALID;
+  if (nedges >= kMaxBuckets) return GEOATTN_ERR_UNSUPPORTED;
+  if (!dev_ptr(lat_q) || !dev_ptr(lon_q) || !dev_ptr(lat_k) || !dev_ptr(lon_k) || (nedges && !dev_ptr(edges)) ||
+      !dev_ptr(ids))
+    return GEOATTN_ERR_INVALID;
+  const long long blocks = ((long long)nq * nk + 255) / 256;
+  if (blocks > (1ll << 31) - 1) return GEOATTN_ERR_UNSUPPORTED;
+  distance_buckets_kernel<<<(unsigned)blocks, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+      nq, lat_q, lon_q, nk, lat_k, lon_k, edges, nedges, max_km, ids);
+  return status_of(cudaGetLastError());
+}
+
+int geoattn_dropout(int dtype, long long n, const void* x, const void* residual, void* y, const long long* rng,
+                    int threshold, void* stream) {
+  if (n <= 0 || threshold < 0 || threshold > 65536) return GEOATTN_ERR_INVALID;
+  if (dtype != GEOATTN_DTYPE_BF16 && dtype != GEOATTN_DTYPE_FP32) return GEOATTN_ERR_INVALID;
+  if (!dev_ptr(x) || !dev_ptr(y) || !dev_ptr(rng) || (residual && !dev_ptr(residual))) return GEOATTN_ERR_INVALID;
+  const long long blocks = (n + 2047) / 2048;
+  if (blocks > (1ll << 31) - 1) return GEOATTN_ERR_UNSUPPORTED;
+  const float scale = threshold >= 65536 ? 0.f : (float)(65536.0 / (65536 - threshold));
+  const int vec = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) |
+                    reinterpret_cast<uintptr_t>(residual)) & 15) == 0;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  auto go = [&](auto kernel, auto* e) {
+    using E = std::remove_pointer_t<decltype(e)>;
+    kernel<<<(unsigned)blocks, 256, 0, st>>>(reinterpret_cast<const E*>(x), reinterpret_cast<const E*>(residual),
+                                             reinterpret_cast<E*>(y), n, rng, threshold, scale, vec);
+  };
+  if (dtype == GEOATTN_DTYPE_BF16) {
+    if (residual) go(dropout_kernel<__nv_bfloat16, true>, (__nv_bfloat16*)nullptr);
+    else go(dropout_kernel<__nv_bfloat16, false>, (__nv_bfloat16*)nullptr);
+  } else {
+    if (residual) go(dropout_kernel<float, true>, (float*)nullptr);
+    else go(dropout_kernel<float, false>, (float*)nullptr);
+  }
+  return status_of(cudaGetLastError());
+}
+
+int geoattn_rng_take(long long* state, long long* out, void* stream) {
+  if (!dev_ptr(state) || !dev_ptr(out)) return GEOATTN_ERR_INVALID;
+  rng_take_kernel<<<1, 1, 0, reinterpret_cast<cudaStream_t>(stream)>>>(state, out);
+  return status_of(cudaGetLastError());
+}
+
+}  // extern "C"

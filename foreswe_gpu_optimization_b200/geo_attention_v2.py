@@ -26,6 +26,7 @@ import ctypes
 import torch
 
 from . import _lib
+from .counter_dropout import CounterRNG, dropout
 from .geometry import StationGeometry, prior_from_dense
 
 # Optional per-kernel timing hook: lists of torch.cuda.Event (already recorded once, so their handles exist) that
@@ -226,20 +227,46 @@ def geo_attention(q, k, v, geometry, alpha, beta, gamma, *, precision=None, mode
     return _run(q, k, v, geometry.prior, alpha, beta, gamma, precision, mode)
 
 
-def patch_model(model, preset="accurate_experimental", geometry=None, precision=None, mode="reference"):
+class _PatchedDropout:
+    """An nn.Dropout's forward on the counter-based generator."""
+
+    def __init__(self, module, rng):
+        self.module, self.rng = module, rng
+
+    def __call__(self, x):
+        return dropout(x, self.module.p, self.rng) if self.module.training else x
+
+
+def _patch_dropout(layer, rng):
+    """Point the nn.Dropout modules of one layer at `rng`; None takes an earlier patch away."""
+    for m in layer.modules() if isinstance(layer, torch.nn.Module) else ():
+        if not isinstance(m, torch.nn.Dropout):
+            continue
+        if isinstance(m.__dict__.get("forward"), _PatchedDropout):
+            del m.__dict__["forward"]
+        if rng is not None:
+            m.forward = _PatchedDropout(m, rng)
+
+
+def patch_model(model, preset="accurate_experimental", geometry=None, precision=None, mode="reference",
+                dropout_rng=None):
     """Swap every encoder layer's attention core for the B200 kernels (foreswe_bench/geo_attention_v2.py:468-478).
 
     With ``geometry`` (a StationGeometry) the layers ignore the dense (distances, angularities) arguments and use
     the coordinate prior; otherwise the prior is built from the dense arguments at each call. ``precision`` and
-    ``mode`` are passed to every call (module docstring). ``preset="eager"`` restores the production method
-    (foreswe_bench/geo_attention.py:326-328)."""
+    ``mode`` are passed to every call (module docstring). With ``dropout_rng`` (a CounterRNG) the nn.Dropout modules
+    of the layers draw from it in training: masks that are recomputed in the backward, and fresh ones at each replay
+    of a captured step. ``preset="eager"`` restores the production methods (foreswe_bench/geo_attention.py:326-328)."""
     if preset != "eager":
         if precision is not None and precision not in PRECISIONS:
             raise ValueError("precision must be one of %s, got %r" % (PRECISIONS, precision))
         if mode not in MODES:
             raise NotImplementedError("mode=%r: only the reference operator (mode='reference') is implemented" % (mode,))
+        if dropout_rng is not None and not isinstance(dropout_rng, CounterRNG):
+            raise TypeError("dropout_rng must be a CounterRNG")
     for layer in model.encoder_layers:
         att = layer.self_attn
+        _patch_dropout(layer, dropout_rng if preset != "eager" else None)
         if preset == "eager":
             att.__dict__.pop("scaled_dot_product_attention", None)
             continue

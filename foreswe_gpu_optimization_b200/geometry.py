@@ -10,6 +10,7 @@ kernels. The table is 2 x N_pad^2 pairs (fp16 pairs for bf16 inputs, fp32 pairs 
 resident in L2), built once per geometry and reused by every layer, head and step.
 """
 import ctypes
+import math
 
 import torch
 
@@ -93,3 +94,29 @@ class StationGeometry:
                 ctypes.c_void_p(self.elev_ft.data_ptr()), None, ctypes.c_void_p(dist.data_ptr()),
                 ctypes.c_void_p(ang.data_ptr()), _stream()))
         return dist, ang
+
+    def distance_buckets(self, edges_km, queries=None, max_km=math.inf):
+        """uint8 [Nq, N] bucket ids for cross_attention: the number of `edges_km` (ascending, at most 63) that are <=
+        the great-circle distance in km of query site i and station j; 255, which excludes the pair, beyond `max_km`.
+
+        queries: the StationGeometry of the query sites (default: these stations themselves)."""
+        queries = self if queries is None else queries
+        if not isinstance(queries, StationGeometry):
+            raise TypeError("queries must be a StationGeometry")
+        if queries.device != self.device:
+            raise ValueError("queries live on %s, the stations on %s" % (queries.device, self.device))
+        edges = torch.as_tensor(edges_km, dtype=torch.float64).reshape(-1)
+        host = edges.tolist()
+        if len(host) > 63 or any(not b >= a for a, b in zip(host, host[1:])) or any(e != e for e in host):
+            raise ValueError("edges_km must be ascending, at most 63 of them")
+        if not max_km >= 0:
+            raise ValueError("max_km must not be negative")
+        edges = edges.to(self.device)
+        ids = torch.empty(queries.n, self.n, dtype=torch.uint8, device=self.device)
+        if ids.numel():
+            with torch.cuda.device(self.device):
+                _lib.check(_lib.lib().geoattn_distance_buckets(
+                    queries.n, queries.lat.data_ptr(), queries.lon.data_ptr(), self.n, self.lat.data_ptr(),
+                    self.lon.data_ptr(), edges.data_ptr() if host else None, len(host), max_km, ids.data_ptr(),
+                    _stream()))
+        return ids

@@ -1,0 +1,171 @@
+"""Attention of sites to an encoder's states of another length, with a learned distance-bucket bias and dropout.
+
+    O = dropout(softmax(scale Q K^T + table[h, bucket(i, j)])) V
+
+next to geo_attention (stations against themselves with the fixed geo prior): queries and keys have their own lengths,
+key heads may be shared by groups of query heads, keys may be absent (ragged lengths, missing stations), pairs may be
+excluded (a distance cut-off), the bias per bucket is learned, and the keep mask of the dropout is recomputed in the
+backward instead of stored. No [Nq, Nk] tensor per head ever reaches memory in the forward.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from .counter_dropout import _dtype_code, _launch, _snapshot, _threshold
+from .geo_attention_v2 import _tma_ready
+
+MAX_BUCKETS = 64
+
+
+def _ready(t):
+    """Operand layout of the kernels: bf16 as TMA reads it; fp32 with the head dim contiguous."""
+    if t.dtype == torch.bfloat16:
+        return _tma_ready(t)
+    return t if t.stride(3) == 1 else t.contiguous()
+
+
+def _like(t):
+    """An output with t's layout where that keeps the head dim contiguous (split_heads views do), else contiguous."""
+    return torch.empty_like(t) if t.stride(3) == 1 else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _strides(t):
+    s = t.stride()  # of a head dim of size 1 any stride says the same
+    return _lib.c_ll4(s[0], s[1], s[2], 1 if t.shape[3] == 1 else s[3])
+
+
+def _tensor(t):
+    return _lib.Tensor(t.data_ptr(), _strides(t))
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _inputs(q, k, v, table, ids, lens, mask, rng, thr, scale):
+    B, H, Nq, D = q.shape
+    sh = _lib.XattnShape(B, H, k.shape[1], Nq, k.shape[2], D, _dtype_code(q, "q"), table.shape[1] if table is not None
+                         else 0, _dtype_code(table, "bias_table") if table is not None else _lib.DTYPE_FP32)
+    return _lib.XattnInputs(sh, _tensor(q), _tensor(k), _tensor(v), _ptr(ids),
+                            0 if ids is None else ids.stride(0), _ptr(table), _ptr(lens), _ptr(mask),
+                            0 if mask is None else mask.stride(0), _ptr(rng), thr, scale)
+
+
+def _forward(q, k, v, table, ids, lens, mask, rng, thr, scale, need_stats):
+    o = _like(q)
+    if k.shape[2] == 0:
+        return o.zero_(), None
+    q, k, v = _ready(q), _ready(k), _ready(v)
+    L = _lib.lib()
+    inp = _inputs(q, k, v, table, ids, lens, mask, rng, thr, scale)
+    ws = torch.empty(L.geoattn_xattn_fwd_workspace_bytes(ctypes.byref(inp.shape)), dtype=torch.uint8, device=q.device)
+    stats = torch.empty(*q.shape[:3], 2, dtype=torch.float32, device=q.device) if need_stats else None
+    args = _lib.XattnFwdArgs(inp, o.data_ptr(), _strides(o), _ptr(stats), ws.data_ptr())
+    _launch(q.device, lambda s: L.geoattn_xattn_fwd(ctypes.byref(args), s))
+    return o, stats
+
+
+def _backward(q, k, v, table, ids, lens, mask, rng, thr, scale, o, stats, do):
+    dq, dk, dv = _like(q), _like(k), _like(v)
+    dtable = torch.empty_like(table, memory_format=torch.contiguous_format) if table is not None else None
+    if k.shape[2] == 0:
+        return dq.zero_(), dk, dv, None if dtable is None else dtable.zero_()
+    q, k, v, do = _ready(q), _ready(k), _ready(v), _ready(do)
+    L = _lib.lib()
+    inp = _inputs(q, k, v, table, ids, lens, mask, rng, thr, scale)
+    ws = torch.empty(L.geoattn_xattn_bwd_workspace_bytes(ctypes.byref(inp.shape)), dtype=torch.uint8, device=q.device)
+    args = _lib.XattnBwdArgs(inp, _tensor(o), _tensor(do), stats.data_ptr(), dq.data_ptr(),
+                             _strides(dq), dk.data_ptr(), _strides(dk), dv.data_ptr(),
+                             _strides(dv), _ptr(dtable), ws.data_ptr())
+    _launch(q.device, lambda s: L.geoattn_xattn_bwd(ctypes.byref(args), s))
+    return dq, dk, dv, dtable
+
+
+class CrossAttention(torch.autograd.Function):
+    """O = dropout(softmax(scale Q K^T + table[h, ids])) V on libgeoattn (fwd + bwd)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, table, ids, lens, mask, rng, thr, scale):
+        o, stats = _forward(q, k, v, table, ids, lens, mask, rng, thr, scale, True)
+        ctx.save_for_backward(q, k, v, table, ids, lens, mask, rng, o, stats)
+        ctx.thr, ctx.scale = thr, scale
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        q, k, v, table, ids, lens, mask, rng, o, stats = ctx.saved_tensors
+        grads = _backward(q, k, v, table, ids, lens, mask, rng, ctx.thr, ctx.scale, o, stats, do)
+        return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), *([None] * 6))
+
+
+def cross_attention(q, k, v, *, buckets=None, bias_table=None, kv_lens=None, key_mask=None, dropout_p=0.0, rng=None,
+                    scale=None):
+    """Attention of q [B, H, Nq, D] to k, v [B, Hkv, Nk, D]; H is a multiple of Hkv (query head h reads key head
+    h // (H // Hkv)), D <= 192, bf16 or fp32, any strides. Returns [B, H, Nq, D] in q's dtype and layout.
+
+    buckets, bias_table: uint8 [Nq, Nk] bucket of each pair (StationGeometry.distance_buckets, or any ids) and the
+        learned [H, T] or [1, T] bias, T <= 64, bf16 or fp32. Ids >= T (255 by convention) exclude their pair.
+    kv_lens: int32 or int64 [B], keys of each batch entry (clamped to 0..Nk). key_mask: bool [B, Nk], True = present.
+        What absent keys hold is not used (NaN included) and their gradients are zero.
+    dropout_p, rng: dropout on the attention weights; rng as in `dropout`.
+    scale: of the scores, 1/sqrt(D) by default.
+    A row with no key left gives zeros. Differentiable (once) in q, k, v and bias_table; the results do not depend on
+    the order of any concurrent sums."""
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError("q must be [B, H, Nq, D] and k, v [B, Hkv, Nk, D], got %s, %s, %s"
+                         % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    B, H, Nq, D = q.shape
+    Hkv, Nk = k.shape[1], k.shape[2]
+    if (H % Hkv if Hkv else H):
+        raise ValueError("query heads (%d) must be a multiple of key heads (%d)" % (H, Hkv))
+    if D > 192:
+        raise ValueError("head dim must be at most 192, got %d" % D)
+    if q.dtype not in (torch.bfloat16, torch.float32) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("q, k, v must all be bf16 or all be fp32")
+    if (buckets is None) != (bias_table is None):
+        raise ValueError("buckets and bias_table come together")
+    if buckets is not None:
+        if buckets.dtype != torch.uint8 or buckets.shape != (Nq, Nk):
+            raise ValueError("buckets must be uint8 [%d, %d], got %s %s"
+                             % (Nq, Nk, buckets.dtype, tuple(buckets.shape)))
+        if bias_table.dim() != 2 or bias_table.shape[0] not in (1, H) or not 1 <= bias_table.shape[1] <= MAX_BUCKETS:
+            raise ValueError("bias_table must be [%d or 1, 1..%d], got %s" % (H, MAX_BUCKETS, tuple(bias_table.shape)))
+        _dtype_code(bias_table, "bias_table")
+    if kv_lens is not None and (kv_lens.dtype not in (torch.int32, torch.int64) or kv_lens.shape != (B,)):
+        raise ValueError("kv_lens must be int32 or int64 [%d]" % B)
+    if key_mask is not None and (key_mask.dtype != torch.bool or key_mask.shape != (B, Nk)):
+        raise ValueError("key_mask must be bool [%d, %d]" % (B, Nk))
+    thr = _threshold(dropout_p)
+    if thr and rng is None:
+        raise ValueError("dropout_p > 0 needs rng")
+    scale = 1.0 / math.sqrt(D) if scale is None and D else float(scale or 0.0)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    if not q.is_cuda:
+        raise RuntimeError("cross attention runs on CUDA tensors only (no CPU path)")
+    for name, t in (("k", k), ("v", v), ("buckets", buckets), ("bias_table", bias_table), ("kv_lens", kv_lens),
+                    ("key_mask", key_mask)):
+        if t is not None and t.device != q.device:
+            raise ValueError("%s lives on %s, q on %s" % (name, t.device, q.device))
+    key = _snapshot(rng, q.device) if thr else None
+    if q.numel() == 0:  # no batch, head, query or head dim: nothing to launch
+        return q * 1.0
+    if bias_table is not None:
+        if bias_table.shape[0] != H:
+            bias_table = bias_table.expand(H, -1)
+        bias_table = bias_table.contiguous()
+        if buckets.stride(1) != 1 or buckets.stride(0) < Nk:
+            buckets = buckets.contiguous()
+    if kv_lens is not None:
+        kv_lens = kv_lens.to(torch.int32).contiguous()
+    if key_mask is not None and (key_mask.stride(1) != 1 or key_mask.stride(0) < Nk):
+        key_mask = key_mask.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+                                    (bias_table is not None and bias_table.requires_grad)):
+        return CrossAttention.apply(q, k, v, bias_table, buckets, kv_lens, key_mask, key, thr, scale)
+    return _forward(q, k, v, bias_table, buckets, kv_lens, key_mask, key, thr, scale, False)[0]

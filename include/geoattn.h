@@ -139,6 +139,76 @@ int geoattn_bwd(const GeoAttnBwdArgs* args, void* stream);
  * It allocates nothing (no cudaMalloc/cudaFree, no allocating library call).                                  */
 int geoattn_bwd_noalloc(const GeoAttnBwdArgs* args, void* stream);
 
+/* ---- cross attention, learned distance-bucket bias, dropout (no counterpart in the reference's fused path) ------- */
+/* O = dropout(softmax(scale Q K^T + table[h, ids[i, j]])) V for queries and keys of different lengths. */
+typedef struct {
+  int batch, heads, kv_heads; /* heads is a multiple of kv_heads; query head h reads key head h / (heads / kv_heads) */
+  int nq, nk, head_dim;       /* head_dim 1..192 */
+  int dtype;                  /* q, k, v, o, dO, dQ, dK, dV: BF16 -> tensor cores; FP32 -> fp32 products on the FMA pipe */
+  int buckets;                /* 0 (no bias) .. 64 */
+  int table_dtype;            /* bias table and its gradient */
+} GeoXattnShape;
+
+typedef struct {
+  GeoXattnShape shape;
+  GeoAttnTensor q, k, v;        /* [B, H, Nq, D], [B, Hkv, Nk, D] twice. BF16: base and strides 16-byte aligned */
+  const unsigned char* ids;     /* bucket of each pair, [nq][ids_ld]; ids >= buckets exclude the pair (buckets > 0) */
+  long long ids_ld;
+  const void* table;            /* [heads][buckets] */
+  const int* kv_lens;           /* [batch] keys of each batch entry (clamped to 0..nk), or NULL */
+  const unsigned char* key_mask; /* [batch][key_mask_ld], 0 = absent, or NULL */
+  long long key_mask_ld;
+  const long long* rng;         /* device (seed, offset) of the dropout generator; read when drop_threshold > 0 */
+  int drop_threshold;           /* round(65536 p): 0 = no dropout, 65536 = nothing kept */
+  float scale;
+} GeoXattnInputs;
+
+size_t geoattn_xattn_fwd_workspace_bytes(const GeoXattnShape* shape);
+size_t geoattn_xattn_bwd_workspace_bytes(const GeoXattnShape* shape);
+
+typedef struct {
+  GeoXattnInputs in;
+  void* o;
+  long long o_stride[4];
+  float* stats;    /* [batch * heads * nq][2] fp32 for the backward (row maximum, 1 / row sum), or NULL */
+  void* workspace; /* geoattn_xattn_fwd_workspace_bytes, 256-byte aligned */
+} GeoXattnFwdArgs;
+
+/* Absent keys (kv_lens, key_mask) may hold anything, NaN included. A row with nothing to attend to gives 0. */
+int geoattn_xattn_fwd(const GeoXattnFwdArgs* args, void* stream);
+
+typedef struct {
+  GeoXattnInputs in;
+  GeoAttnTensor o, dout;
+  const float* stats; /* of the forward on the same inputs */
+  void* dq;
+  long long dq_stride[4];
+  void* dk;
+  long long dk_stride[4];
+  void* dv;
+  long long dv_stride[4];
+  void* dtable;      /* [heads][buckets], table_dtype (buckets > 0) */
+  void* workspace;   /* geoattn_xattn_bwd_workspace_bytes, 256-byte aligned */
+} GeoXattnBwdArgs;
+
+/* dQ, dK, dV (summed over the heads that share a key head) and the table's gradient. Deterministic: no atomics. Keys
+ * that are absent get zero gradients. */
+int geoattn_xattn_bwd(const GeoXattnBwdArgs* args, void* stream);
+
+/* ids[i * nk + j] = number of edges (ascending, km) <= the great-circle distance of site i and station j; 255 beyond
+ * max_km. Degrees, float64, all on the device; nedges <= 63. */
+int geoattn_distance_buckets(int nq, const double* lat_q, const double* lon_q, int nk, const double* lat_k,
+                             const double* lon_k, const double* edges, int nedges, double max_km, unsigned char* ids,
+                             void* stream);
+
+/* y = keep ? x * 65536 / (65536 - threshold) : 0, plus residual where given; n contiguous elements. Element e is kept
+ * where its 16 bits of Philox4x32-7(counter (e / 8, offset), key seed) are >= threshold; the backward is the same call
+ * on dy without the residual. */
+int geoattn_dropout(int dtype, long long n, const void* x, const void* residual, void* y, const long long* rng,
+                    int threshold, void* stream);
+/* out[0..1] = state[0..1] (seed, offset), then state[1] += 1, in stream order. */
+int geoattn_rng_take(long long* state, long long* out, void* stream);
+
 /* ---- diagnostics --------------------------------------------------------------------------------------- */
 /* Copies the device status word of a workspace (0 = ok, 1 = a bounded wait expired, 2 = a kernel found its shared
  * memory misaligned and did nothing) to *status. workspace = NULL reads the status word of the last
