@@ -6,7 +6,9 @@
 #include "../../include/geoattn.h"
 #include "host_util.h"
 #include "xattn_aux.cuh"
+#include "tma_host.h"
 #include "xattn_simt.cuh"
+#include "xattn_tc.cuh"
 
 namespace geoattn {
 namespace {
@@ -26,12 +28,14 @@ struct XDims {
   size_t ds_unit;       // dS^T bytes of one (batch, key head) unit
 };
 
+bool packs_rows(const XDims& d) { return d.bf16 && d.G > 1 && d.T == 0 && (long long)d.G * d.Nq <= 128; }
+
 int forward_splits(const XDims& d) {
   // enough key ranges to give every SM a tile when the rows alone do not; each range keeps at least 4 key tiles
-  const long long tiles = (long long)((d.Nq + 127) / 128) * d.B * d.H;
+  const long long tiles = packs_rows(d) ? (long long)d.B * d.Hkv : (long long)((d.Nq + 127) / 128) * d.B * d.H;
   const int ktiles = (d.Nk + 63) / 64;
   if (tiles >= kSMs || ktiles < 8) return 1;
-  const long long want = (2 * kSMs + tiles - 1) / tiles;
+  const long long want = (4 * kSMs + tiles - 1) / tiles;
   const long long most = ktiles / 4;
   return (int)(want < most ? want : most);
 }
@@ -68,6 +72,7 @@ int check_xshape(const GeoXattnShape* s, XDims& d) {
 struct XFwdWs {
   int* status;
   float *part_o, *part_ml;
+  uint8_t* ids;
 };
 size_t xfwd_ws(const XDims& d, uint8_t* base, XFwdWs* w) {
   size_t off = 0;
@@ -83,6 +88,7 @@ size_t xfwd_ws(const XDims& d, uint8_t* base, XFwdWs* w) {
     t.part_o = reinterpret_cast<float*>(take(rows * d.D * 4));
     t.part_ml = reinterpret_cast<float*>(take(rows * 2 * 4));
   }
+  if (d.T && d.bf16) t.ids = take((size_t)d.Nq * d.nkp);
   if (w) *w = t;
   return off;
 }
@@ -127,6 +133,7 @@ int check_inputs(const GeoXattnInputs& a, const XDims& d) {
   if (d.T && (!dev_ptr(a.ids) || !dev_ptr(a.table) || a.ids_ld < d.Nk)) return GEOATTN_ERR_INVALID;
   if (a.kv_lens && !dev_ptr(a.kv_lens)) return GEOATTN_ERR_INVALID;
   if (a.key_mask && (!dev_ptr(a.key_mask) || a.key_mask_ld < d.Nk)) return GEOATTN_ERR_INVALID;
+  if (!(a.scale > 0.f) || std::isinf(a.scale)) return GEOATTN_ERR_INVALID;
   if (a.drop_threshold < 0 || a.drop_threshold > 65536 || (a.drop_threshold > 0 && !dev_ptr(a.rng)))
     return GEOATTN_ERR_INVALID;
   for (const GeoAttnTensor* t : {&a.q, &a.k, &a.v})
@@ -183,6 +190,56 @@ int simt_bwd_any(const XParams& p, const XDims& d, int units, cudaStream_t st) {
                     : d.DP == 128 ? simt_bwd<E, 128>(p, units, st) : simt_bwd<E, 192>(p, units, st);
 }
 
+// TMA map over a bf16 tensor [batch, heads, rows, D] (box: 64 columns x `rows` rows x `heads` heads).
+int xmap(CUtensorMap* m, const XTensor& t, int D, int n, int heads, int batch, int box_rows, int box_heads) {
+  if (reinterpret_cast<uintptr_t>(t.p) & 15) return GEOATTN_ERR_ALIGNMENT;
+  for (int i = 0; i < 3; ++i)
+    if (t.s[i] <= 0 || ((t.s[i] * 2) & 15)) return GEOATTN_ERR_ALIGNMENT;
+  const uint64_t dims[4] = {(uint64_t)D, (uint64_t)n, (uint64_t)heads, (uint64_t)batch};
+  const uint64_t str[3] = {(uint64_t)t.s[2] * 2, (uint64_t)t.s[1] * 2, (uint64_t)t.s[0] * 2};
+  const uint32_t box[4] = {64, (uint32_t)box_rows, (uint32_t)box_heads, 1};
+  return make_tmap(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, t.p, dims, str, box) ? GEOATTN_OK : GEOATTN_ERR_TMA;
+}
+
+template <class K>
+int tc_launch(K kernel, long long grid, int threads, int smem, cudaStream_t st, const xa::XMaps& maps,
+              const XParams& p) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return GEOATTN_ERR_LAUNCH;
+  kernel<<<(unsigned)grid, threads, smem, st>>>(maps, p);
+  return status_of(cudaGetLastError());
+}
+
+template <int DP>
+int tc_fwd(const xa::XMaps& maps, const XParams& p, long long grid, cudaStream_t st) {
+  using C = xa::FwdCfg<DP>;
+  return p.ids ? tc_launch(xa::xattn_fwd_kernel<DP, true>, grid, C::THREADS, C::SMEM, st, maps, p)
+               : tc_launch(xa::xattn_fwd_kernel<DP, false>, grid, C::THREADS, C::SMEM, st, maps, p);
+}
+
+// 16-byte loads of ids rows: the caller's own where they allow it, else a padded copy.
+int aligned_ids(XParams& p, const XDims& d, uint8_t* copy, cudaStream_t st) {
+  if (!p.ids || ((p.ids_ld | d.Nk | (long long)reinterpret_cast<uintptr_t>(p.ids)) & 15) == 0) return GEOATTN_OK;
+  const long long blocks = ((long long)d.Nq * d.nkp / 4 + 255) / 256;
+  ids_pad_kernel<<<(unsigned)blocks, 256, 0, st>>>(p.ids, p.ids_ld, d.Nq, d.Nk, d.nkp, copy);
+  p.ids = copy, p.ids_ld = d.nkp;
+  return status_of(cudaGetLastError());
+}
+
+int forward_tc(XParams& p, const XDims& d, uint8_t* ids, cudaStream_t st) {
+  xa::XMaps maps;
+  std::memset(&maps, 0, sizeof(maps));
+  p.pack = packs_rows(d);
+  int rc;
+  if ((rc = p.pack ? xmap(&maps.q, p.q, d.D, d.Nq, d.H, d.B, d.Nq, d.G) : xmap(&maps.q, p.q, d.D, d.Nq, d.H, d.B, 128, 1)) ||
+      (rc = xmap(&maps.k, p.k, d.D, d.Nk, d.Hkv, d.B, 64, 1)) || (rc = xmap(&maps.v, p.v, d.D, d.Nk, d.Hkv, d.B, 64, 1)) ||
+      (rc = aligned_ids(p, d, ids, st)))
+    return rc;
+  const long long grid = (long long)d.splits * d.B * (p.pack ? d.Hkv : (long long)((d.Nq + 127) / 128) * d.H);
+  return d.DP == 64 ? tc_fwd<64>(maps, p, grid, st)
+                    : d.DP == 128 ? tc_fwd<128>(maps, p, grid, st) : tc_fwd<192>(maps, p, grid, st);
+}
+
 }  // namespace
 }  // namespace geoattn
 
@@ -213,7 +270,7 @@ int geoattn_xattn_fwd(const GeoXattnFwdArgs* a, void* stream) {
   XParams p = xparams(a->in, d);
   p.o = xt(a->o, a->o_stride), p.stats = reinterpret_cast<float2*>(a->stats);
   p.splits = d.splits, p.part_o = ws.part_o, p.part_ml = ws.part_ml, p.status = ws.status;
-  int rc = d.bf16 ? simt_fwd_any<__nv_bfloat16>(p, d, st) : simt_fwd_any<float>(p, d, st);
+  int rc = d.bf16 ? forward_tc(p, d, ws.ids, st) : simt_fwd_any<float>(p, d, st);
   if (rc || d.splits == 1) return rc;
   const long long rows = (long long)d.B * d.H * d.Nq;
   return d.bf16 ? xlaunch(xattn_combine_kernel<__nv_bfloat16>, (rows + 7) / 8, 256, 0, st, p)

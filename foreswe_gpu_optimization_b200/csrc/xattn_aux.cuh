@@ -29,6 +29,19 @@ __global__ void __launch_bounds__(256) distance_buckets_kernel(int nq, const dou
   ids[x] = km > max_km ? (uint8_t)kNoPair : (uint8_t)n;
 }
 
+// out[i][j] = ids[i][j], rows padded to `ldo` (a multiple of 16) with kNoPair: what 16-byte loads need.
+__global__ void __launch_bounds__(256) ids_pad_kernel(const uint8_t* __restrict__ ids, long long ld, int nq, int nk,
+                                                      int ldo, uint8_t* __restrict__ out) {
+  const long long x = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (x >= (long long)nq * ldo) return;
+  const long long i = x / ldo;
+  const int j = (int)(x % ldo);
+  uint32_t w = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w |= (uint32_t)(j + e < nk ? ids[i * ld + j + e] : (uint8_t)kNoPair) << (8 * e);
+  *reinterpret_cast<uint32_t*>(out + x) = w;
+}
+
 // idsT[j][i] = ids[i][j], padded to [nkp][nqp] with kNoPair.
 __global__ void __launch_bounds__(256) ids_transpose_kernel(const uint8_t* __restrict__ ids, long long ld, int nq,
                                                             int nk, int nqp, uint8_t* __restrict__ idsT) {

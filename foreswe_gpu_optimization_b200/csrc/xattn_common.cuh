@@ -44,6 +44,7 @@ struct XParams {
   void* ds;                 // dS^T [units * G heads][nkp][nqp] of the launch's units
   int nqp, nkp;             // Nq, Nk rounded up to 64 and 128
   int u0;                   // first (batch, key head) unit of this launch
+  int pack;                 // forward, tensor cores: a tile holds the G * Nq rows of a key head's group
   int splits;               // > 1: key ranges per row, joined by xattn_combine_kernel
   float* part_o;            // [splits][B*H*Nq][D]
   float* part_ml;           // [splits][B*H*Nq][2]: running max (log2 units) and sum

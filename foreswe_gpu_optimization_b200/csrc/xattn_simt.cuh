@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_fwd_kernel(const XPar
       if (drop.thr) {
         const uint32_t kb = drop.keep8(i, (j0 + tx * 4) >> 3, bh) >> ((tx & 1) * 4);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) s[r][c] = (kb >> c) & 1 ? s[r][c] * drop.scale : 0.f;
+        for (int c = 0; c < 4; ++c) s[r][c] = (kb >> c) & 1 ? s[r][c] : 0.f;
       }
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) acc[r][c] *= corr;
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_fwd_kernel(const XPar
         p.part_ml[at * 2 + 1] = l[r];
       }
     } else {
-      const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+      const float inv = l[r] == 0.f ? 0.f : (drop.thr ? drop.scale : 1.f) / l[r];
       E* O = reinterpret_cast<E*>(p.o.p) + b * p.o.s[0] + h * p.o.s[1] + i * p.o.s[2];
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) {
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(256) xattn_combine_kernel(const XParams p) {
     const float* ml = p.part_ml + (s * rows + row) * 2;
     l += ml[1] * xex2(ml[0] - base);
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = l == 0.f ? 0.f : (p.drop_thr ? p.drop_scale : 1.f) / l;
   const int i = (int)(row % p.Nq), bh = (int)(row / p.Nq), h = bh % p.H, b = bh / p.H;
   E* O = reinterpret_cast<E*>(p.o.p) + b * p.o.s[0] + h * p.o.s[1] + i * p.o.s[2];
   for (int d = lane; d < p.D; d += 32) {

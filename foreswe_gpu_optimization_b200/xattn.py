@@ -113,7 +113,7 @@ def cross_attention(q, k, v, *, buckets=None, bias_table=None, kv_lens=None, key
     kv_lens: int32 or int64 [B], keys of each batch entry (clamped to 0..Nk). key_mask: bool [B, Nk], True = present.
         What absent keys hold is not used (NaN included) and their gradients are zero.
     dropout_p, rng: dropout on the attention weights; rng as in `dropout`.
-    scale: of the scores, 1/sqrt(D) by default.
+    scale: of the scores, positive, 1/sqrt(D) by default.
     A row with no key left gives zeros. Differentiable (once) in q, k, v and bias_table; the results do not depend on
     the order of any concurrent sums."""
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
@@ -143,9 +143,9 @@ def cross_attention(q, k, v, *, buckets=None, bias_table=None, kv_lens=None, key
     thr = _threshold(dropout_p)
     if thr and rng is None:
         raise ValueError("dropout_p > 0 needs rng")
-    scale = 1.0 / math.sqrt(D) if scale is None and D else float(scale or 0.0)
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
+    scale = (1.0 / math.sqrt(D) if D else 1.0) if scale is None else float(scale)
+    if not 0.0 < scale < math.inf and D:
+        raise ValueError("scale must be positive and finite, got %r" % (scale,))
     if not q.is_cuda:
         raise RuntimeError("cross attention runs on CUDA tensors only (no CPU path)")
     for name, t in (("k", k), ("v", v), ("buckets", buckets), ("bias_table", bias_table), ("kv_lens", kv_lens),

@@ -70,6 +70,9 @@ def _qkv(B=2, H=4, Hkv=2, Nq=3, Nk=5, D=8, dtype=BF):
     (lambda q, k, v: dict(dropout_p=1.1, rng=torch.zeros(2, dtype=torch.int64)), ValueError),
     (lambda q, k, v: dict(dropout_p=float("nan"), rng=torch.zeros(2, dtype=torch.int64)), ValueError),
     (lambda q, k, v: dict(scale=math.inf), ValueError),
+    (lambda q, k, v: dict(scale=math.nan), ValueError),
+    (lambda q, k, v: dict(scale=0.0), ValueError),
+    (lambda q, k, v: dict(scale=-1.0), ValueError),
     (lambda q, k, v: {}, RuntimeError),                              # CPU tensors
 ])
 def test_cross_attention_refusals(bad, error):
