@@ -58,7 +58,7 @@ int check_xshape(const GeoXattnShape* s, XDims& d) {
   d.splits = forward_splits(d);
   const long long qt = (d.Nq + 63) / 64, kt = (d.Nk + 31) / 32;
   if (qt * d.B * d.H * d.splits > (1ll << 30) || kt * d.B * d.Hkv > (1ll << 30)) return GEOATTN_ERR_UNSUPPORTED;
-  d.ds_unit = (size_t)d.G * d.nkp * d.nqp * 4;
+  d.ds_unit = (size_t)d.G * d.nkp * d.nqp * (d.bf16 ? 2 : 4);
   const long long units = (long long)d.B * d.Hkv;
   long long per = (long long)(kDsCap / d.ds_unit);
   per = per < 1 ? 1 : per > units ? units : per;
@@ -95,7 +95,7 @@ size_t xfwd_ws(const XDims& d, uint8_t* base, XFwdWs* w) {
 
 struct XBwdWs {
   int* status;
-  float* delta;
+  float *delta, *rec;
   void* ds;
   uint8_t* idsT;
   float* part;
@@ -109,7 +109,8 @@ size_t xbwd_ws(const XDims& d, uint8_t* base, XBwdWs* w) {
   };
   XBwdWs t{};
   t.status = reinterpret_cast<int*>(take(sizeof(int)));
-  t.delta = reinterpret_cast<float*>(take((size_t)d.B * d.H * d.Nq * 4));
+  if (d.bf16) t.rec = reinterpret_cast<float*>(take((size_t)d.B * d.H * d.nqp * 3 * 4));
+  else t.delta = reinterpret_cast<float*>(take((size_t)d.B * d.H * d.Nq * 4));
   t.ds = take(d.ds_unit * d.units_per_launch);
   if (d.T) {
     t.idsT = take((size_t)d.nkp * d.nqp);
@@ -117,6 +118,13 @@ size_t xbwd_ws(const XDims& d, uint8_t* base, XBwdWs* w) {
   }
   if (w) *w = t;
   return off;
+}
+
+// Makes the current device's context current in this thread: the driver's tensor-map encoder wants one, and a thread
+// whose first CUDA call this is (autograd's, a user's worker) may have none yet.
+bool bind_context() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
 }
 
 int status_of(cudaError_t e) { return e == cudaSuccess ? GEOATTN_OK : GEOATTN_ERR_LAUNCH; }
@@ -166,28 +174,25 @@ int xlaunch(K kernel, long long grid, int threads, int smem, cudaStream_t st, co
   return status_of(cudaGetLastError());
 }
 
-template <class E, int DP>
+template <int DP>
 int simt_fwd(const XParams& p, cudaStream_t st) {
-  return xlaunch(xattn_simt_fwd_kernel<E, DP>, (long long)((p.Nq + 127) / 128) * p.B * p.H * p.splits, kSimtThreads,
+  return xlaunch(xattn_simt_fwd_kernel<DP>, (long long)((p.Nq + 127) / 128) * p.B * p.H * p.splits, kSimtThreads,
                  SimtFwd<DP>::SMEM, st, p);
 }
-template <class E>
-int simt_fwd_any(const XParams& p, const XDims& d, cudaStream_t st) {
-  return d.DP == 64 ? simt_fwd<E, 64>(p, st) : d.DP == 128 ? simt_fwd<E, 128>(p, st) : simt_fwd<E, 192>(p, st);
+int forward_simt(const XParams& p, const XDims& d, cudaStream_t st) {
+  return d.DP == 64 ? simt_fwd<64>(p, st) : d.DP == 128 ? simt_fwd<128>(p, st) : simt_fwd<192>(p, st);
 }
-template <class E, int DP>
+template <int DP>
 int simt_bwd(const XParams& p, int units, cudaStream_t st) {
   using C = SimtBwd<DP>;
-  int rc = xlaunch(xattn_simt_bwd_keys_kernel<E, DP>, (long long)((p.Nk + C::TK - 1) / C::TK) * units, kSimtThreads,
+  int rc = xlaunch(xattn_simt_bwd_keys_kernel<DP>, (long long)((p.Nk + C::TK - 1) / C::TK) * units, kSimtThreads,
                    C::SMEM, st, p);
   if (rc) return rc;
-  return xlaunch(xattn_simt_bwd_dq_kernel<E, DP>, (long long)((p.Nq + 63) / 64) * units * p.G, kSimtThreads,
+  return xlaunch(xattn_simt_bwd_dq_kernel<DP>, (long long)((p.Nq + 63) / 64) * units * p.G, kSimtThreads,
                  SimtDq<DP>::SMEM, st, p);
 }
-template <class E>
-int simt_bwd_any(const XParams& p, const XDims& d, int units, cudaStream_t st) {
-  return d.DP == 64 ? simt_bwd<E, 64>(p, units, st)
-                    : d.DP == 128 ? simt_bwd<E, 128>(p, units, st) : simt_bwd<E, 192>(p, units, st);
+int backward_simt(const XParams& p, const XDims& d, int units, cudaStream_t st) {
+  return d.DP == 64 ? simt_bwd<64>(p, units, st) : d.DP == 128 ? simt_bwd<128>(p, units, st) : simt_bwd<192>(p, units, st);
 }
 
 // TMA map over a bf16 tensor [batch, heads, rows, D] (box: 64 columns x `rows` rows x `heads` heads).
@@ -240,6 +245,42 @@ int forward_tc(XParams& p, const XDims& d, uint8_t* ids, cudaStream_t st) {
                     : d.DP == 128 ? tc_fwd<128>(maps, p, grid, st) : tc_fwd<192>(maps, p, grid, st);
 }
 
+int backward_maps(xa::XMaps& maps, const XParams& p, const XDims& d) {
+  int rc;
+  if ((rc = xmap(&maps.q, p.q, d.D, d.Nq, d.H, d.B, 64, 1)) || (rc = xmap(&maps.dout, p.dout, d.D, d.Nq, d.H, d.B, 64, 1)) ||
+      (rc = xmap(&maps.k, p.k, d.D, d.Nk, d.Hkv, d.B, 64, 1)) || (rc = xmap(&maps.v, p.v, d.D, d.Nk, d.Hkv, d.B, 64, 1)))
+    return rc;
+  const uint64_t dims[3] = {(uint64_t)d.nqp, (uint64_t)d.nkp, (uint64_t)d.units_per_launch * d.G};
+  const uint64_t str[2] = {(uint64_t)d.nqp * 2, (uint64_t)d.nqp * d.nkp * 2};
+  const uint32_t box[3] = {64, 64, 1};
+  return make_tmap(&maps.ds, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, p.ds, dims, str, box) ? GEOATTN_OK : GEOATTN_ERR_TMA;
+}
+
+template <int DP>
+int tc_bwd(const xa::XMaps& maps, const XParams& p, int units, cudaStream_t st) {
+  using C = xa::KeysCfg<DP>;
+  const long long grid = (long long)((p.Nk + 127) / 128) * units;
+  auto keys = p.ids ? (p.drop_thr ? xa::xattn_bwd_keys_kernel<DP, true, true> : xa::xattn_bwd_keys_kernel<DP, true, false>)
+                    : (p.drop_thr ? xa::xattn_bwd_keys_kernel<DP, false, true> : xa::xattn_bwd_keys_kernel<DP, false, false>);
+  if (int rc = tc_launch(keys, grid, C::THREADS, C::SMEM, st, maps, p)) return rc;
+  return tc_launch(xa::xattn_bwd_dq_kernel<DP>, (long long)((p.Nq + 127) / 128) * units * p.G, xa::DqCfg<DP>::THREADS,
+                   xa::DqCfg<DP>::SMEM, st, maps, p);
+}
+
+int backward_tc(const xa::XMaps& maps, const XParams& p, const XDims& d, int units, cudaStream_t st) {
+  return d.DP == 64 ? tc_bwd<64>(maps, p, units, st)
+                    : d.DP == 128 ? tc_bwd<128>(maps, p, units, st) : tc_bwd<192>(maps, p, units, st);
+}
+
+template <class S>
+int table_grad(const XParams& p, const XDims& d, int units, float* part, cudaStream_t st) {
+  if (cudaFuncSetAttribute(table_grad_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBuckets * 1024) !=
+      cudaSuccess)
+    return GEOATTN_ERR_LAUNCH;
+  table_grad_kernel<S><<<dim3(d.chunks, d.H), 256, d.T * 1024, st>>>(p, units, part);
+  return status_of(cudaGetLastError());
+}
+
 }  // namespace
 }  // namespace geoattn
 
@@ -264,13 +305,14 @@ int geoattn_xattn_fwd(const GeoXattnFwdArgs* a, void* stream) {
   if (int rc = check_inputs(a->in, d)) return rc;
   if (!dev_ptr(a->o) || (a->stats && !dev_ptr(a->stats)) || !dev_ptr(a->workspace)) return GEOATTN_ERR_INVALID;
   if (a->o_stride[3] != 1 || (reinterpret_cast<uintptr_t>(a->workspace) & (kAlign - 1))) return GEOATTN_ERR_ALIGNMENT;
+  if (!bind_context()) return GEOATTN_ERR_LAUNCH;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   XFwdWs ws;
   xfwd_ws(d, reinterpret_cast<uint8_t*>(a->workspace), &ws);
   XParams p = xparams(a->in, d);
   p.o = xt(a->o, a->o_stride), p.stats = reinterpret_cast<float2*>(a->stats);
   p.splits = d.splits, p.part_o = ws.part_o, p.part_ml = ws.part_ml, p.status = ws.status;
-  int rc = d.bf16 ? forward_tc(p, d, ws.ids, st) : simt_fwd_any<float>(p, d, st);
+  int rc = d.bf16 ? forward_tc(p, d, ws.ids, st) : forward_simt(p, d, st);
   if (rc || d.splits == 1) return rc;
   const long long rows = (long long)d.B * d.H * d.Nq;
   return d.bf16 ? xlaunch(xattn_combine_kernel<__nv_bfloat16>, (rows + 7) / 8, 256, 0, st, p)
@@ -288,16 +330,22 @@ int geoattn_xattn_bwd(const GeoXattnBwdArgs* a, void* stream) {
   if (a->o.stride[3] != 1 || a->dout.stride[3] != 1 || a->dq_stride[3] != 1 || a->dk_stride[3] != 1 ||
       a->dv_stride[3] != 1 || (reinterpret_cast<uintptr_t>(a->workspace) & (kAlign - 1)))
     return GEOATTN_ERR_ALIGNMENT;
+  if (!bind_context()) return GEOATTN_ERR_LAUNCH;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   XBwdWs ws;
   xbwd_ws(d, reinterpret_cast<uint8_t*>(a->workspace), &ws);
   XParams p = xparams(a->in, d);
   p.o = xt(a->o.data, a->o.stride), p.dout = xt(a->dout.data, a->dout.stride);
   p.dq = xt(a->dq, a->dq_stride), p.dk = xt(a->dk, a->dk_stride), p.dv = xt(a->dv, a->dv_stride);
-  p.stats = reinterpret_cast<float2*>(const_cast<float*>(a->stats)), p.delta = ws.delta, p.ds = ws.ds, p.idsT = ws.idsT, p.status = ws.status;
-  const long long rows = (long long)d.B * d.H * d.Nq;
-  int rc = d.bf16 ? xlaunch(xattn_delta_kernel<__nv_bfloat16>, (rows + 7) / 8, 256, 0, st, p)
-                  : xlaunch(xattn_delta_kernel<float>, (rows + 7) / 8, 256, 0, st, p);
+  p.stats = reinterpret_cast<float2*>(const_cast<float*>(a->stats)), p.delta = ws.delta, p.rec = ws.rec, p.ds = ws.ds;
+  p.idsT = ws.idsT, p.status = ws.status;
+  xa::XMaps maps;
+  std::memset(&maps, 0, sizeof(maps));
+  int rc = d.bf16 ? backward_maps(maps, p, d) : GEOATTN_OK;
+  if (rc) return rc;
+  if (cudaMemsetAsync(ws.status, 0, sizeof(int), st) != cudaSuccess) return GEOATTN_ERR_LAUNCH;
+  rc = d.bf16 ? xlaunch(xa::xattn_records_kernel, ((long long)d.B * d.H * d.nqp + 7) / 8, 256, 0, st, p)
+              : xlaunch(xattn_delta_kernel, ((long long)d.B * d.H * d.Nq + 7) / 8, 256, 0, st, p);
   if (rc) return rc;
   if (d.T) {
     ids_transpose_kernel<<<dim3(d.nqp / 64, d.nkp / 64), 256, 0, st>>>(p.ids, p.ids_ld, d.Nq, d.Nk, d.nqp, ws.idsT);
@@ -307,15 +355,12 @@ int geoattn_xattn_bwd(const GeoXattnBwdArgs* a, void* stream) {
   for (int l = 0; l < d.launches; ++l) {
     p.u0 = l * d.units_per_launch;
     const int nu = units - p.u0 < d.units_per_launch ? units - p.u0 : d.units_per_launch;
-    rc = d.bf16 ? simt_bwd_any<__nv_bfloat16>(p, d, nu, st) : simt_bwd_any<float>(p, d, nu, st);
+    rc = d.bf16 ? backward_tc(maps, p, d, nu, st) : backward_simt(p, d, nu, st);
     if (rc) return rc;
     if (d.T) {
       float* part = ws.part + (size_t)l * d.H * d.chunks * d.T;
-      if (cudaFuncSetAttribute(table_grad_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               kMaxBuckets * 1024) != cudaSuccess)
-        return GEOATTN_ERR_LAUNCH;
-      table_grad_kernel<float><<<dim3(d.chunks, d.H), 256, d.T * 1024, st>>>(p, nu, part);
-      if ((rc = status_of(cudaGetLastError()))) return rc;
+      rc = d.bf16 ? table_grad<__nv_bfloat16>(p, d, nu, part, st) : table_grad<float>(p, d, nu, part, st);
+      if (rc) return rc;
     }
   }
   if (d.T) {

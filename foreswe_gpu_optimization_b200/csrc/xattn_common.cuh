@@ -40,7 +40,8 @@ struct XParams {
   float scale, scale_log2;  // scale, scale * log2(e)
   float2* stats;            // (m_i, 1 / l_i) [B*H][Nq]; (0, 0) for a row with nothing left. Kept apart: in m + log2(l)
                             // a bias near the type's lowest value would swallow log2(l)
-  float* delta;             // [B*H][Nq]
+  float* delta;             // [B*H][Nq] (fp32)
+  float* rec;               // row records (bf16, xattn_records_kernel)
   void* ds;                 // dS^T [units * G heads][nkp][nqp] of the launch's units
   int nqp, nkp;             // Nq, Nk rounded up to 64 and 128
   int u0;                   // first (batch, key head) unit of this launch

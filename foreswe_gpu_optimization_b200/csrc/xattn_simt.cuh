@@ -13,21 +13,21 @@ namespace geoattn {
 constexpr int kSimtThreads = 256;
 
 // dst[d][r] = row r of `src` (zero where r >= n, d >= D or !live[r]); 4 consecutive d per load where `vec`.
-template <int ROWS, int DP, int ST, class E>
-__device__ __forceinline__ void simt_load_t(float* dst, const E* src, long long ld, int n, int D, bool vec,
+template <int ROWS, int DP, int ST>
+__device__ __forceinline__ void simt_load_t(float* dst, const float* src, long long ld, int n, int D, bool vec,
                                             const float* live) {
   for (int x = threadIdx.x; x < ROWS * (DP / 4); x += kSimtThreads) {
     const int r = x % ROWS, d = (x / ROWS) * 4;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     if (r < n && d < D && (!live || live[r] == 0.f)) {
-      const E* s = src + (long long)r * ld + d;
-      if (vec && sizeof(E) == 4) {
+      const float* s = src + (long long)r * ld + d;
+      if (vec) {
         const float4 f = *reinterpret_cast<const float4*>(s);
         v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (d + i < D) v[i] = to_f(s[i]);
+          if (d + i < D) v[i] = s[i];
       }
     }
 #pragma unroll
@@ -36,30 +36,29 @@ __device__ __forceinline__ void simt_load_t(float* dst, const E* src, long long 
 }
 
 // dst[r][d], row stride DP, as above.
-template <int ROWS, int DP, class E>
-__device__ __forceinline__ void simt_load_n(float* dst, const E* src, long long ld, int n, int D, bool vec,
+template <int ROWS, int DP>
+__device__ __forceinline__ void simt_load_n(float* dst, const float* src, long long ld, int n, int D, bool vec,
                                             const float* live) {
   for (int x = threadIdx.x; x < ROWS * (DP / 4); x += kSimtThreads) {
     const int r = x / (DP / 4), d = (x % (DP / 4)) * 4;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     if (r < n && d < D && (!live || live[r] == 0.f)) {
-      const E* s = src + (long long)r * ld + d;
-      if (vec && sizeof(E) == 4) {
+      const float* s = src + (long long)r * ld + d;
+      if (vec) {
         const float4 f = *reinterpret_cast<const float4*>(s);
         v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (d + i < D) v[i] = to_f(s[i]);
+          if (d + i < D) v[i] = s[i];
       }
     }
     *reinterpret_cast<float4*>(dst + r * DP + d) = make_float4(v[0], v[1], v[2], v[3]);
   }
 }
 
-template <class E>
 __device__ __forceinline__ bool simt_vec(const XTensor& t, int D) {
-  return sizeof(E) == 4 && D % 4 == 0 && (reinterpret_cast<uintptr_t>(t.p) & 15) == 0 && t.s[0] % 4 == 0 &&
+  return D % 4 == 0 && (reinterpret_cast<uintptr_t>(t.p) & 15) == 0 && t.s[0] % 4 == 0 &&
          t.s[1] % 4 == 0 && t.s[2] % 4 == 0;
 }
 
@@ -74,7 +73,7 @@ struct SimtFwd {
   static constexpr int SMEM = FLOATS * 4;
 };
 
-template <class E, int DP>
+template <int DP>
 __global__ void __launch_bounds__(kSimtThreads) xattn_simt_fwd_kernel(const XParams p) {
   using C = SimtFwd<DP>;
   extern __shared__ float4 simt_smem[];
@@ -91,10 +90,10 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_fwd_kernel(const XPar
   const int n = key_count(p, b);
   const int ntiles = (n + C::BN - 1) / C::BN;
   const int t0 = (int)((long long)ntiles * split / p.splits), t1 = (int)((long long)ntiles * (split + 1) / p.splits);
-  const E* Q = reinterpret_cast<const E*>(p.q.p) + b * p.q.s[0] + h * p.q.s[1];
-  const E* K = reinterpret_cast<const E*>(p.k.p) + b * p.k.s[0] + kh * p.k.s[1];
-  const E* V = reinterpret_cast<const E*>(p.v.p) + b * p.v.s[0] + kh * p.v.s[1];
-  const bool vq = simt_vec<E>(p.q, p.D), vk = simt_vec<E>(p.k, p.D), vv = simt_vec<E>(p.v, p.D);
+  const float* Q = reinterpret_cast<const float*>(p.q.p) + b * p.q.s[0] + h * p.q.s[1];
+  const float* K = reinterpret_cast<const float*>(p.k.p) + b * p.k.s[0] + kh * p.k.s[1];
+  const float* V = reinterpret_cast<const float*>(p.v.p) + b * p.v.s[0] + kh * p.v.s[1];
+  const bool vq = simt_vec(p.q, p.D), vk = simt_vec(p.k, p.D), vv = simt_vec(p.v, p.D);
   const AttnDrop drop = attn_drop(p.rng, p.drop_thr, p.drop_scale);
 
   if (p.ids) tab[threadIdx.x] = table_log2(p, h, threadIdx.x);
@@ -202,11 +201,11 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_fwd_kernel(const XPar
       }
     } else {
       const float inv = l[r] == 0.f ? 0.f : (drop.thr ? drop.scale : 1.f) / l[r];
-      E* O = reinterpret_cast<E*>(p.o.p) + b * p.o.s[0] + h * p.o.s[1] + i * p.o.s[2];
+      float* O = reinterpret_cast<float*>(p.o.p) + b * p.o.s[0] + h * p.o.s[1] + i * p.o.s[2];
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) {
         const int d = (c / 4) * 64 + tx * 4 + c % 4;
-        if (d < p.D) O[d] = from_f<E>(acc[r][c] * inv);
+        if (d < p.D) O[d] = acc[r][c] * inv;
       }
       if (tx == 0 && p.stats) p.stats[row] = row_stats(m[r], l[r]);
     }
@@ -241,17 +240,16 @@ __global__ void __launch_bounds__(256) xattn_combine_kernel(const XParams p) {
 }
 
 // delta_i = dO_i . O_i, one warp per row.
-template <class E>
 __global__ void __launch_bounds__(256) xattn_delta_kernel(const XParams p) {
   const long long rows = (long long)p.B * p.H * p.Nq;
   const long long row = (long long)blockIdx.x * 8 + threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
   if (row >= rows) return;
   const int i = (int)(row % p.Nq), bh = (int)(row / p.Nq), h = bh % p.H, b = bh / p.H;
-  const E* O = reinterpret_cast<const E*>(p.o.p) + b * p.o.s[0] + h * p.o.s[1] + i * p.o.s[2];
-  const E* G = reinterpret_cast<const E*>(p.dout.p) + b * p.dout.s[0] + h * p.dout.s[1] + i * p.dout.s[2];
+  const float* O = reinterpret_cast<const float*>(p.o.p) + b * p.o.s[0] + h * p.o.s[1] + i * p.o.s[2];
+  const float* G = reinterpret_cast<const float*>(p.dout.p) + b * p.dout.s[0] + h * p.dout.s[1] + i * p.dout.s[2];
   float x = 0.f;
-  for (int d = lane; d < p.D; d += 32) x = fmaf(to_f(O[d]), to_f(G[d]), x);
+  for (int d = lane; d < p.D; d += 32) x = fmaf(O[d], G[d], x);
 #pragma unroll
   for (int w = 16; w; w /= 2) x += __shfl_xor_sync(0xffffffffu, x, w);
   if (lane == 0) p.delta[row] = x;
@@ -268,7 +266,7 @@ struct SimtBwd {
   static constexpr int SMEM = FLOATS * 4;
 };
 
-template <class E, int DP>
+template <int DP>
 __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_keys_kernel(const XParams p) {
   using C = SimtBwd<DP>;
   constexpr int KT = C::KT, NC = DP / 16;
@@ -299,15 +297,15 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_keys_kernel(const
   if (j0 < n) {
     if (threadIdx.x < C::TK) live[threadIdx.x] = key_live(p, b, j0 + threadIdx.x, n) ? 0.f : -INFINITY;
     __syncthreads();
-    const E* K = reinterpret_cast<const E*>(p.k.p) + b * p.k.s[0] + kh * p.k.s[1] + (long long)j0 * p.k.s[2];
-    const E* V = reinterpret_cast<const E*>(p.v.p) + b * p.v.s[0] + kh * p.v.s[1] + (long long)j0 * p.v.s[2];
-    simt_load_t<C::TK, DP, C::SK>(kt, K, p.k.s[2], n - j0, p.D, simt_vec<E>(p.k, p.D), live);
-    simt_load_t<C::TK, DP, C::SK>(vt, V, p.v.s[2], n - j0, p.D, simt_vec<E>(p.v, p.D), live);
+    const float* K = reinterpret_cast<const float*>(p.k.p) + b * p.k.s[0] + kh * p.k.s[1] + (long long)j0 * p.k.s[2];
+    const float* V = reinterpret_cast<const float*>(p.v.p) + b * p.v.s[0] + kh * p.v.s[1] + (long long)j0 * p.v.s[2];
+    simt_load_t<C::TK, DP, C::SK>(kt, K, p.k.s[2], n - j0, p.D, simt_vec(p.k, p.D), live);
+    simt_load_t<C::TK, DP, C::SK>(vt, V, p.v.s[2], n - j0, p.D, simt_vec(p.v, p.D), live);
     const int nqt = (p.Nq + C::BQ - 1) / C::BQ;
     for (int it = 0; it < nqt * p.G; ++it) {
       const int h = kh * p.G + it / nqt, i0 = (it % nqt) * C::BQ, bh = b * p.H + h;
-      const E* Q = reinterpret_cast<const E*>(p.q.p) + b * p.q.s[0] + h * p.q.s[1] + (long long)i0 * p.q.s[2];
-      const E* G = reinterpret_cast<const E*>(p.dout.p) + b * p.dout.s[0] + h * p.dout.s[1] + (long long)i0 * p.dout.s[2];
+      const float* Q = reinterpret_cast<const float*>(p.q.p) + b * p.q.s[0] + h * p.q.s[1] + (long long)i0 * p.q.s[2];
+      const float* G = reinterpret_cast<const float*>(p.dout.p) + b * p.dout.s[0] + h * p.dout.s[1] + (long long)i0 * p.dout.s[2];
       __syncthreads();  // the last tile's products have read qt, gt, pt, st
       if (p.ids && it % nqt == 0) tab[threadIdx.x] = table_log2(p, h, threadIdx.x);
       if (threadIdx.x < C::BQ) {
@@ -317,8 +315,8 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_keys_kernel(const
         inv[threadIdx.x] = st.y;
         del[threadIdx.x] = i < p.Nq ? p.delta[(long long)bh * p.Nq + i] : 0.f;
       }
-      simt_load_t<C::BQ, DP, C::SQ>(qt, Q, p.q.s[2], p.Nq - i0, p.D, simt_vec<E>(p.q, p.D), nullptr);
-      simt_load_t<C::BQ, DP, C::SQ>(gt, G, p.dout.s[2], p.Nq - i0, p.D, simt_vec<E>(p.dout, p.D), nullptr);
+      simt_load_t<C::BQ, DP, C::SQ>(qt, Q, p.q.s[2], p.Nq - i0, p.D, simt_vec(p.q, p.D), nullptr);
+      simt_load_t<C::BQ, DP, C::SQ>(gt, G, p.dout.s[2], p.Nq - i0, p.D, simt_vec(p.dout, p.D), nullptr);
       __syncthreads();
       float s[4][KT] = {}, dp[4][KT] = {};
 #pragma unroll 4
@@ -397,14 +395,14 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_keys_kernel(const
   for (int x = 0; x < KT; ++x) {
     const int j = j0 + ty * KT + x;
     if (j >= p.Nk) continue;
-    E* dK = reinterpret_cast<E*>(p.dk.p) + b * p.dk.s[0] + kh * p.dk.s[1] + (long long)j * p.dk.s[2];
-    E* dV = reinterpret_cast<E*>(p.dv.p) + b * p.dv.s[0] + kh * p.dv.s[1] + (long long)j * p.dv.s[2];
+    float* dK = reinterpret_cast<float*>(p.dk.p) + b * p.dk.s[0] + kh * p.dk.s[1] + (long long)j * p.dk.s[2];
+    float* dV = reinterpret_cast<float*>(p.dv.p) + b * p.dv.s[0] + kh * p.dv.s[1] + (long long)j * p.dv.s[2];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int d = tx + 16 * c;
       if (d < p.D) {
-        dK[d] = from_f<E>(ak[x][c] * p.scale);
-        dV[d] = from_f<E>(av[x][c]);
+        dK[d] = ak[x][c] * p.scale;
+        dV[d] = av[x][c];
       }
     }
   }
@@ -419,7 +417,7 @@ struct SimtDq {
   static constexpr int SMEM = (BK * BQ + BK * DP + BK) * 4;
 };
 
-template <class E, int DP>
+template <int DP>
 __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_dq_kernel(const XParams p) {
   using C = SimtDq<DP>;
   extern __shared__ float4 simt_smem[];
@@ -431,7 +429,7 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_dq_kernel(const X
   const int unit = p.u0 + ul / p.G, b = unit / p.Hkv, kh = unit % p.Hkv, h = kh * p.G + ul % p.G;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   const int n = key_count(p, b);
-  const E* K = reinterpret_cast<const E*>(p.k.p) + b * p.k.s[0] + kh * p.k.s[1];
+  const float* K = reinterpret_cast<const float*>(p.k.p) + b * p.k.s[0] + kh * p.k.s[1];
   const float* S = reinterpret_cast<const float*>(p.ds) + (long long)ul * p.nkp * p.nqp + i0;
   float acc[4][DP / 16];
 #pragma unroll
@@ -448,7 +446,7 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_dq_kernel(const X
                      : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     __syncthreads();
-    simt_load_n<C::BK, DP>(kn, K + (long long)j0 * p.k.s[2], p.k.s[2], n - j0, p.D, simt_vec<E>(p.k, p.D), live);
+    simt_load_n<C::BK, DP>(kn, K + (long long)j0 * p.k.s[2], p.k.s[2], n - j0, p.D, simt_vec(p.k, p.D), live);
     __syncthreads();
 #pragma unroll 4
     for (int j = 0; j < C::BK; ++j) {
@@ -471,11 +469,11 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_dq_kernel(const X
   for (int r = 0; r < 4; ++r) {
     const int i = i0 + ty * 4 + r;
     if (i >= p.Nq) continue;
-    E* dQ = reinterpret_cast<E*>(p.dq.p) + b * p.dq.s[0] + h * p.dq.s[1] + (long long)i * p.dq.s[2];
+    float* dQ = reinterpret_cast<float*>(p.dq.p) + b * p.dq.s[0] + h * p.dq.s[1] + (long long)i * p.dq.s[2];
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
       const int d = (c / 4) * 64 + tx * 4 + c % 4;
-      if (d < p.D) dQ[d] = from_f<E>(acc[r][c] * p.scale);
+      if (d < p.D) dQ[d] = acc[r][c] * p.scale;
     }
   }
 }

@@ -22,6 +22,11 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const 
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, ctx));
 }
 
+// Barrier `id` among `threads` threads.
+__device__ __forceinline__ void named_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -354,6 +359,416 @@ __global__ void __launch_bounds__(192, 2) xattn_fwd_kernel(const __grid_constant
         p.part_ml[part * 2 + 1] = l;
       } else if (row && p.stats) {
         p.stats[stat] = row_stats(m, l);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == C::MMA_WARP) tmem_dealloc(tmem, C::TM_COLS);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Backward, row records: chunks of 64 query rows, rec[b*h][chunk][3][64] floats:
+//   without the bias  -(m + log2 l), unused, delta        with it  -m, 1 / l, delta (the bias may dwarf log2 l)
+// so that P = 2^(t + rec0) or 2^(t + rec0) rec1; rows past Nq and rows with nothing left get P = 0. One warp per row.
+// ---------------------------------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) xattn_records_kernel(const XParams p) {
+  const int per = p.nqp;
+  const long long x = (long long)blockIdx.x * 8 + threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  if (x >= (long long)p.B * p.H * per) return;
+  const int i = (int)(x % per), bh = (int)(x / per), h = bh % p.H, b = bh / p.H;
+  float d = 0.f;
+  if (i < p.Nq) {
+    const __nv_bfloat16* O =
+        reinterpret_cast<const __nv_bfloat16*>(p.o.p) + b * p.o.s[0] + h * p.o.s[1] + (long long)i * p.o.s[2];
+    const __nv_bfloat16* G = reinterpret_cast<const __nv_bfloat16*>(p.dout.p) + b * p.dout.s[0] + h * p.dout.s[1] +
+                             (long long)i * p.dout.s[2];
+    if (vec_rows(p.o) && vec_rows(p.dout)) {
+      const int c = lane * 8;
+      if (c + 8 <= p.D) {
+        const uint4 a = *reinterpret_cast<const uint4*>(O + c), g = *reinterpret_cast<const uint4*>(G + c);
+        const __nv_bfloat162 *av = reinterpret_cast<const __nv_bfloat162*>(&a),
+                             *gv = reinterpret_cast<const __nv_bfloat162*>(&g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 u = __bfloat1622float2(av[e]), v = __bfloat1622float2(gv[e]);
+          d = fmaf(u.x, v.x, fmaf(u.y, v.y, d));
+        }
+      } else {
+        for (int e = c; e < p.D; ++e) d = fmaf(to_f(O[e]), to_f(G[e]), d);
+      }
+    } else {
+      for (int e = lane; e < p.D; e += 32) d = fmaf(to_f(O[e]), to_f(G[e]), d);
+    }
+  }
+#pragma unroll
+  for (int w = 16; w; w /= 2) d += __shfl_xor_sync(0xffffffffu, d, w);
+  if (lane == 0) {
+    const float2 st = i < p.Nq ? p.stats[(long long)bh * p.Nq + i] : make_float2(0.f, 0.f);
+    float* rec = p.rec + ((long long)bh * (per / 64) + i / 64) * 192 + i % 64;
+    rec[0] = p.ids ? -st.x : st.y == 0.f ? -INFINITY : log2f(st.y) - st.x;
+    rec[64] = st.y;
+    rec[128] = d;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Backward, key pass. One CTA per (128 keys, key head, batch); loops over chunks of 64 queries of the heads that share
+// the key head. Scores are formed transposed (keys in the lanes), so that P^T and dS^T are written over them in tensor
+// memory as the A operands of
+//   dV += P^T dO,  dK += dS^T Q
+// and a thread owns one key's 32 queries of a piece; dS^T also goes to the scratch for dQ and the table's gradient.
+//   MMA warp       S^T(c + 1), dP^T(c + 1), then dV, dK of chunk c
+//   EW warpgroups  P, dS of chunk c (piece w of 32 queries to warpgroup w mod EW)
+// DP = 64 fits two CTAs per SM (one score buffer each); DP = 128 takes the SM with two buffers, DP = 192 with one.
+// Dropout: a Philox call covers one query and 8 keys. Each lane makes the calls of 4 queries for its octet of keys and
+// the 8 x 8 bit blocks are transposed among 8 lanes (3 shuffles per 32 x 32 bits), so no call is made twice.
+// ---------------------------------------------------------------------------------------------------------------
+template <int DP>
+struct KeysCfg {
+  static constexpr int EW = DP == 64 ? 1 : 2, CTAS = DP == 64 ? 2 : 1;
+  static constexpr int NB = DP == 128 ? 2 : 1;                 // score buffers (S^T and dP^T)
+  static constexpr int NST = DP == 192 ? 2 : 4;                // chunks of Q, dO and records in flight
+  static constexpr int K_BYTES = DP / 64 * 128 * 128, Q_BYTES = DP / 64 * 64 * 128, REC_BYTES = 768;
+  static constexpr int STAGE = 2 * Q_BYTES;
+  static constexpr int OFF_V = K_BYTES, OFF_ST = 2 * K_BYTES, OFF_REC = OFF_ST + NST * STAGE,
+                       OFF_TAB = OFF_REC + NST * REC_BYTES, SMEM = OFF_TAB + 1024;
+  static constexpr int TM_DK = 0, TM_DV = DP, TM_S = 2 * DP, TM_COLS = CTAS == 2 ? 256 : 512;
+  static constexpr int THREADS = EW * 128 + 64, TMA_WARP = EW * 4, MMA_WARP = EW * 4 + 1;
+};
+
+// acc[128 x DP] (+)= A[128 x 64] B[64 x DP]: A's 32-wide pieces at the start of their own 32 score columns.
+template <int DP>
+__device__ __forceinline__ void mma_pieces(uint32_t acc, uint32_t a, uint32_t b, bool accumulate) {
+  constexpr uint32_t idesc = instr_desc(1, 0, 1, 128, DP);
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+    mma_ts<Kind::kF16>(acc, a + (s / 2) * 32 + (s % 2) * 8, smem_desc_sw128(b + s * 16 * 128, 64 * 128, 1024), idesc,
+                       accumulate || s > 0);
+}
+
+// Keep bits of 32 queries (i0 ..) for this lane's key j0 + lane: bit q of the result.
+__device__ __forceinline__ uint32_t keep_column(const AttnDrop& drop, uint32_t i0, uint32_t j0, uint32_t bh) {
+  const int lane = threadIdx.x & 31;
+  uint32_t x = 0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) x |= drop.keep8(i0 + 8 * c + (lane & 7), (j0 >> 3) + (lane >> 3), bh) << (8 * c);
+#pragma unroll
+  for (int s = 1; s < 8; s *= 2) {
+    const uint32_t low = s == 1 ? 0x55555555u : s == 2 ? 0x33333333u : 0x0F0F0F0Fu;
+    const uint32_t y = __shfl_xor_sync(0xffffffffu, x, s);
+    x = lane & s ? (x & ~low) | ((y >> s) & low) : (x & low) | ((y << s) & ~low);
+  }
+  return x;
+}
+
+template <int DP, bool BIAS, bool DROP>
+__global__ void __launch_bounds__(KeysCfg<DP>::THREADS, KeysCfg<DP>::CTAS)
+    xattn_bwd_keys_kernel(const __grid_constant__ XMaps maps, const XParams p) {
+  using C = KeysCfg<DP>;
+  constexpr int NB = C::NB, NST = C::NST;
+  __shared__ uint64_t bar_k, bar_full[NST], bar_empty[NST], bar_s[NB], bar_p[NB], bar_done;
+  __shared__ uint32_t tmem_sh;
+  __shared__ int abort_flag;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int nkt = (p.Nk + 127) / 128, kt = blockIdx.x % nkt, ul = blockIdx.x / nkt, unit = p.u0 + ul;
+  const int b = unit / p.Hkv, kh = unit % p.Hkv, j0 = kt * 128;
+  const int n = key_count(p, b);
+  const int nqc = p.nqp / 64, nc = nqc * p.G;
+  WaitCtx ctx{&abort_flag, p.status};
+  __nv_bfloat16* dK = reinterpret_cast<__nv_bfloat16*>(p.dk.p) + b * p.dk.s[0] + kh * p.dk.s[1];
+  __nv_bfloat16* dV = reinterpret_cast<__nv_bfloat16*>(p.dv.p) + b * p.dv.s[0] + kh * p.dv.s[1];
+
+  if (j0 >= n) {  // no key of this tile exists: zero gradients, and the scratch is not read here
+    for (int x = threadIdx.x; x < 128 * p.D; x += C::THREADS) {
+      const int j = j0 + x / p.D, d = x % p.D;
+      if (j < p.Nk) {
+        dK[(long long)j * p.dk.s[2] + d] = __float2bfloat16_rn(0.f);
+        dV[(long long)j * p.dv.s[2] + d] = __float2bfloat16_rn(0.f);
+      }
+    }
+    return;
+  }
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    mbar_init(&bar_k, 1);
+    for (int i = 0; i < NST; ++i) {
+      mbar_init(&bar_full[i], 1);
+      mbar_init(&bar_empty[i], 1);
+    }
+    for (int i = 0; i < NB; ++i) {
+      mbar_init(&bar_s[i], 1);
+      mbar_init(&bar_p[i], C::EW * 128);
+    }
+    mbar_init(&bar_done, 1);
+    fence_barrier_init();
+  }
+  if (warp == C::MMA_WARP) {
+    tmem_alloc(&tmem_sh, C::TM_COLS);
+    tmem_relinquish();
+  }
+  float* tab = reinterpret_cast<float*>(xsmem + C::OFF_TAB);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_sh, sbase = smem_u32(xsmem);
+
+  if (warp == C::TMA_WARP) {
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&bar_k, 2 * C::K_BYTES);
+      for (int x = 0; x < 128; x += 64) {  // the maps' boxes hold 64 rows
+        load_rows<DP>(xsmem + x * 128, &maps.k, &bar_k, 128 * 128, j0 + x, kh, b);
+        load_rows<DP>(xsmem + C::OFF_V + x * 128, &maps.v, &bar_k, 128 * 128, j0 + x, kh, b);
+      }
+      for (int c = 0; c < nc; ++c) {
+        const int st = c % NST, h = kh * p.G + c / nqc, qc = c % nqc;
+        if (!mbar_wait(&bar_empty[st], ((c / NST) & 1) ^ 1, ctx)) break;
+        uint8_t* dst = xsmem + C::OFF_ST + st * C::STAGE;
+        mbar_arrive_expect_tx(&bar_full[st], C::STAGE + C::REC_BYTES);
+        load_rows<DP>(dst, &maps.q, &bar_full[st], 64 * 128, qc * 64, h, b);
+        load_rows<DP>(dst + C::Q_BYTES, &maps.dout, &bar_full[st], 64 * 128, qc * 64, h, b);
+        bulk_load(xsmem + C::OFF_REC + st * C::REC_BYTES, p.rec + ((long long)(b * p.H + h) * nqc + qc) * 192,
+                  C::REC_BYTES, &bar_full[st]);
+      }
+    }
+  } else if (warp == C::MMA_WARP) {
+    if (lane == 0) {
+      bool ok = mbar_wait(&bar_k, 0, ctx);
+      auto scores = [&](int c) {
+        const int st = c % NST;
+        if (!(ok = ok && mbar_wait(&bar_full[st], (c / NST) & 1, ctx))) return;
+        tc_fence_after();
+        const uint32_t q = sbase + C::OFF_ST + st * C::STAGE, acc = tmem + C::TM_S + (c % NB) * 128;
+        mma_scores<DP>(acc, sbase, q);
+        mma_scores<DP>(acc + 64, sbase + C::OFF_V, q + C::Q_BYTES);
+        mma_commit(&bar_s[c % NB]);
+      };
+      scores(0);
+      for (int c = 0; c < nc && ok; ++c) {
+        if (NB == 2 && c + 1 < nc) scores(c + 1);
+        const int st = c % NST;
+        if (!(ok = ok && mbar_wait(&bar_p[c % NB], (c / NB) & 1, ctx))) break;
+        tc_fence_after();
+        const uint32_t q = sbase + C::OFF_ST + st * C::STAGE, acc = tmem + C::TM_S + (c % NB) * 128;
+        mma_pieces<DP>(tmem + C::TM_DV, acc, q + C::Q_BYTES, c > 0);
+        mma_pieces<DP>(tmem + C::TM_DK, acc + 64, q, c > 0);
+        mma_commit(&bar_empty[st]);
+        if (NB == 1 && c + 1 < nc) scores(c + 1);
+      }
+      if (ok) mma_commit(&bar_done);
+    }
+  } else {
+    const int wg = C::EW == 1 ? 0 : warp / 4, r = (warp & 3) * 32 + lane, j = j0 + r;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const bool check_keys = p.kmask != nullptr || j0 + 128 > n, live = key_live(p, b, j, n);
+    const AttnDrop drop = attn_drop(p.rng, DROP ? p.drop_thr : 0, p.drop_scale);
+    bool ok = true;
+    for (int c = 0; c < nc; ++c) {
+      const int st = c % NST, g = c / nqc, i0 = (c % nqc) * 64, bh = b * p.H + kh * p.G + g;
+      if (BIAS && c % nqc == 0) {  // the next head's bias
+        named_sync(1, C::EW * 128);
+        for (int t = threadIdx.x; t < 256; t += C::EW * 128) tab[t] = table_log2(p, kh * p.G + g, t);
+        named_sync(1, C::EW * 128);
+      }
+      uint4 id4[2 / C::EW * 2];
+      if (BIAS) {
+#pragma unroll
+        for (int x = 0; x < 2 / C::EW * 2; ++x)
+          id4[x] = __ldg(reinterpret_cast<const uint4*>(p.idsT + (long long)j * p.nqp + i0 + wg * 32) + x);
+      }
+      const uint32_t sbuf = lanes + C::TM_S + (c % NB) * 128;
+      // bar_s follows bar_full, so the records are there too; the wait on bar_full makes their copy visible here
+      if (ok) ok = warp_wait(&bar_full[st], (c / NST) & 1, ctx) && warp_wait(&bar_s[c % NB], (c / NB) & 1, ctx);
+      if (!ok) continue;  // given up: only the barrier above is still met
+      tc_fence_after();
+      const float* rec = reinterpret_cast<const float*>(xsmem + C::OFF_REC + st * C::REC_BYTES);
+      __nv_bfloat16* ds = reinterpret_cast<__nv_bfloat16*>(p.ds) + (long long)(ul * p.G + g) * p.nkp * p.nqp +
+                          (long long)j * p.nqp + i0;
+#pragma unroll
+      for (int piece = wg; piece < 2; piece += C::EW) {
+        uint32_t s[32], dp[32];
+        tmem_ld32_issue(sbuf + piece * 32, s);
+        tmem_ld32_issue(sbuf + 64 + piece * 32, dp);
+        uint32_t keep = 0;
+        if (DROP) keep = keep_column(drop, i0 + piece * 32, j0 + (warp & 3) * 32, bh);
+        tmem_wait32(s);
+        tmem_pin32(dp);
+        uint32_t wp[16], wd[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 r0 = *reinterpret_cast<const float4*>(rec + piece * 32 + e);
+          const float4 r2 = *reinterpret_cast<const float4*>(rec + 128 + piece * 32 + e);
+          const float a0[4] = {r0.x, r0.y, r0.z, r0.w}, dl[4] = {r2.x, r2.y, r2.z, r2.w};
+          float a1[4] = {1.f, 1.f, 1.f, 1.f};
+          if (BIAS) {
+            const float4 r1 = *reinterpret_cast<const float4*>(rec + 64 + piece * 32 + e);
+            a1[0] = r1.x, a1[1] = r1.y, a1[2] = r1.z, a1[3] = r1.w;
+          }
+          float pv[4], dv[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            float t = __uint_as_float(s[e + u]);
+            if (BIAS) {
+              const uint32_t* w = reinterpret_cast<const uint32_t*>(id4) + (piece / C::EW) * 8;
+              t = fmaf(t, p.scale_log2, tab[(w[e / 4] >> (8 * u)) & 255]);
+              t = xex2(t + a0[u]) * a1[u];
+            } else {
+              t = xex2(fmaf(t, p.scale_log2, a0[u]));
+            }
+            const float da = __uint_as_float(dp[e + u]);
+            if (DROP) {
+              const bool k = (keep >> (e + u)) & 1;
+              pv[u] = k ? t : 0.f;
+              dv[u] = t * (k ? fmaf(da, drop.scale, -dl[u]) : -dl[u]);
+            } else {
+              pv[u] = t;
+              dv[u] = t * (da - dl[u]);
+            }
+          }
+          wp[e / 2] = pack_bf16(pv[0], pv[1]), wp[e / 2 + 1] = pack_bf16(pv[2], pv[3]);
+          wd[e / 2] = pack_bf16(dv[0], dv[1]), wd[e / 2 + 1] = pack_bf16(dv[2], dv[3]);
+        }
+        if (check_keys) {  // an absent key's row is 0 whatever K and V hold there
+#pragma unroll
+          for (int e = 0; e < 16; ++e) wp[e] = live ? wp[e] : 0u, wd[e] = live ? wd[e] : 0u;
+        }
+        tmem_st16(sbuf + piece * 32, wp);
+        tmem_st16(sbuf + 64 + piece * 32, wd);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          reinterpret_cast<uint4*>(ds + piece * 32)[e] = make_uint4(wd[4 * e], wd[4 * e + 1], wd[4 * e + 2], wd[4 * e + 3]);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&bar_p[c % NB]);
+    }
+    if (ok) ok = warp_wait(&bar_done, 0, ctx);
+    tc_fence_after();
+    const bool vk = vec_rows(p.dk), vv = vec_rows(p.dv);
+    const float fv = DROP ? p.drop_scale : 1.f;
+    if (ok) {
+#pragma unroll 1
+      for (int d = wg * 32; d < DP; d += C::EW * 32) {
+        float x[32];
+        tmem_ld32(lanes + C::TM_DK + d, x);
+        if (j < p.Nk && d < p.D) store_row(dK + (long long)j * p.dk.s[2] + d, x, p.scale, p.D - d, vk);
+        tmem_ld32(lanes + C::TM_DV + d, x);
+        if (j < p.Nk && d < p.D) store_row(dV + (long long)j * p.dv.s[2] + d, x, fv, p.D - d, vv);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == C::MMA_WARP) tmem_dealloc(tmem, C::TM_COLS);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// dQ = scale dS K from the dS^T scratch: one CTA per (128 queries, head of the launch's units), over 64-key chunks;
+// dS^T is read as an A operand with queries contiguous. Bound by reading the scratch. Two of the epilogue's warps clear
+// the rows of absent keys first (0 * NaN).
+// ---------------------------------------------------------------------------------------------------------------
+template <int DP>
+struct DqCfg {
+  static constexpr int NST = DP == 64 ? 4 : DP == 128 ? 3 : 2;
+  static constexpr int A_BYTES = 2 * 64 * 128, B_BYTES = DP / 64 * 64 * 128, STAGE = A_BYTES + B_BYTES;
+  static constexpr int SMEM = NST * STAGE;
+  static constexpr int TM_COLS = DP == 64 ? 64 : DP == 128 ? 128 : 256;
+  static constexpr int THREADS = 192, TMA_WARP = 4, MMA_WARP = 5;
+};
+
+template <int DP>
+__global__ void __launch_bounds__(192, 2) xattn_bwd_dq_kernel(const __grid_constant__ XMaps maps, const XParams p) {
+  using C = DqCfg<DP>;
+  constexpr int NST = C::NST;
+  __shared__ uint64_t bar_full[NST], bar_clean[NST], bar_empty[NST], bar_done;
+  __shared__ uint32_t tmem_sh;
+  __shared__ int abort_flag;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int nqt = (p.Nq + 127) / 128, qt = blockIdx.x % nqt, ul = blockIdx.x / nqt;
+  const int unit = p.u0 + ul / p.G, b = unit / p.Hkv, kh = unit % p.Hkv, h = kh * p.G + ul % p.G;
+  const int n = key_count(p, b), nc = (n + 63) / 64;
+  WaitCtx ctx{&abort_flag, p.status};
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < NST; ++i) {
+      mbar_init(&bar_full[i], 1);
+      mbar_init(&bar_clean[i], 64);
+      mbar_init(&bar_empty[i], 1);
+    }
+    mbar_init(&bar_done, 1);
+    fence_barrier_init();
+  }
+  if (warp == C::MMA_WARP) {
+    tmem_alloc(&tmem_sh, C::TM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_sh, sbase = smem_u32(xsmem);
+
+  if (warp == C::TMA_WARP) {
+    if (lane == 0) {
+      for (int c = 0; c < nc; ++c) {
+        const int st = c % NST;
+        if (!mbar_wait(&bar_empty[st], ((c / NST) & 1) ^ 1, ctx)) break;
+        uint8_t* dst = xsmem + st * C::STAGE;
+        mbar_arrive_expect_tx(&bar_full[st], C::STAGE);
+        tma_load_3d(dst, &maps.ds, &bar_full[st], qt * 128, c * 64, ul);
+        tma_load_3d(dst + 64 * 128, &maps.ds, &bar_full[st], qt * 128 + 64, c * 64, ul);
+        load_rows<DP>(dst + C::A_BYTES, &maps.k, &bar_full[st], 64 * 128, c * 64, kh, b);
+      }
+    }
+  } else if (warp == C::MMA_WARP) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = instr_desc(1, 1, 1, 128, DP);
+      bool ok = true;
+      for (int c = 0; c < nc; ++c) {
+        const int st = c % NST;
+        // every chunk is handed on by the clearing warps, whether it held an absent key or not
+        if (!(ok = mbar_wait(&bar_clean[st], (c / NST) & 1, ctx))) break;
+        tc_fence_after();
+        const uint32_t a = sbase + st * C::STAGE, k = a + C::A_BYTES;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          mma_ss<Kind::kF16>(tmem, smem_desc_sw128(a + s * 16 * 128, 64 * 128, 1024),
+                             smem_desc_sw128(k + s * 16 * 128, 64 * 128, 1024), idesc, c + s > 0);
+        mma_commit(&bar_empty[st]);
+      }
+      if (ok) mma_commit(&bar_done);
+    }
+  } else {
+    bool ok = true;
+    if (warp < 2) {
+      for (int c = 0; c < nc; ++c) {
+        const int st = c % NST, j = c * 64 + threadIdx.x;
+        const bool live = key_live(p, b, j, n);
+        if (!(ok = warp_wait(&bar_full[st], (c / NST) & 1, ctx))) break;
+        if (!live) {
+          clear_row<DP>(xsmem + st * C::STAGE + C::A_BYTES, threadIdx.x);
+          fence_proxy_async_smem();
+        }
+        mbar_arrive(&bar_clean[st]);
+      }
+    }
+    if (ok) ok = warp_wait(&bar_done, 0, ctx);
+    tc_fence_after();
+    const int i = qt * 128 + warp * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    const bool vec = vec_rows(p.dq);
+    __nv_bfloat16* dQ = reinterpret_cast<__nv_bfloat16*>(p.dq.p) + b * p.dq.s[0] + h * p.dq.s[1];
+    if (ok) {
+#pragma unroll 1
+      for (int d = 0; d < DP; d += 32) {
+        float x[32];
+        if (nc > 0) {
+          tmem_ld32(lanes + d, x);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = 0.f;
+        }
+        if (i < p.Nq && d < p.D) store_row(dQ + (long long)i * p.dq.s[2] + d, x, p.scale, p.D - d, vec);
       }
     }
   }

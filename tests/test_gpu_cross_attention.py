@@ -382,6 +382,17 @@ def test_other_streams():
             assert torch.equal(a, b)
 
 
+def test_a_thread_of_its_own():
+    """Forward and backward as the first CUDA work of a thread."""
+    import threading
+    x, kw = make(1, 2, 2, 70, 90, 64, BF, seed=5)
+    want, got = run(x, kw), {}
+    t = threading.Thread(target=lambda: got.update(run(x, kw)))
+    t.start()
+    t.join()
+    assert got and all(torch.equal(got[n], want[n]) for n in want)
+
+
 @pytest.mark.parametrize("nq, n, T", [(1, 1, 1), (70, 130, 20), (257, 64, 64)])
 def test_distance_buckets(nq, n, T):
     import foreswe_gpu_optimization_b200 as g
