@@ -43,15 +43,40 @@ __device__ __forceinline__ uint32_t keep_bits8(uint4 w, uint32_t thr) {
   return m;
 }
 
+// Two elements at once: bit 15 of the result is set where the low half of x is >= the low half of t (an unsigned
+// 16-bit comparison), bit 31 for the high halves; the other bits are arbitrary. t holds the threshold twice.
+__device__ __forceinline__ uint32_t keep_pair(uint32_t x, uint32_t t) {
+  // the low 15 bits are compared by a subtraction that cannot borrow across the halves, the top bits by logic
+  const uint32_t low = (x | 0x80008000u) - (t & 0x7FFF7FFFu);
+  return (x & ~t) | (~(x ^ t) & low);
+}
+// 0xFFFF in each half whose bit 15 / 31 is set; all ones where bit 15 (HALF = 0) or bit 31 (HALF = 1) is.
+// (prmt with bit 3 of a selector set replicates the chosen byte's sign.)
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t spread_signs(uint32_t d) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, 0, %2;" : "=r"(r) : "r"(d), "n"(SEL));
+  return r;
+}
+__device__ __forceinline__ uint32_t spread_pair(uint32_t d) { return spread_signs<0xBB99>(d); }
+template <int HALF>
+__device__ __forceinline__ uint32_t spread_one(uint32_t d) {
+  return spread_signs<HALF ? 0xBBBB : 0x9999>(d);
+}
+
 // Attention weights: element (b, h, i, j) is bit j % 8 of counter (j / 8, i, b * H + h, offset low) under the key
 // (seed low, seed high ^ offset high). `rng` is (seed, offset) in device memory, so a captured graph sees new values.
 struct AttnDrop {
   PhiloxKey key;
   uint32_t off, thr;
-  float scale;  // 65536 / (65536 - thr); 0 where nothing is kept
+  float scale;  // 65536 / (65536 - thr)
   __device__ __forceinline__ uint32_t keep8(uint32_t i, uint32_t j8, uint32_t bh) const {
     return keep_bits8(philox7(j8, i, bh, off, key), thr);
   }
+  __device__ __forceinline__ uint4 words(uint32_t i, uint32_t j8, uint32_t bh) const {
+    return philox7(j8, i, bh, off, key);
+  }
+  __device__ __forceinline__ uint32_t pair() const { return thr * 0x10001u; }  // the threshold (< 65536) in both halves
 };
 
 __device__ __forceinline__ AttnDrop attn_drop(const long long* rng, int thr, float scale) {

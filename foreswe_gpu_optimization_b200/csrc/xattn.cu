@@ -142,7 +142,7 @@ int check_inputs(const GeoXattnInputs& a, const XDims& d) {
   if (a.kv_lens && !dev_ptr(a.kv_lens)) return GEOATTN_ERR_INVALID;
   if (a.key_mask && (!dev_ptr(a.key_mask) || a.key_mask_ld < d.Nk)) return GEOATTN_ERR_INVALID;
   if (!(a.scale > 0.f) || std::isinf(a.scale)) return GEOATTN_ERR_INVALID;
-  if (a.drop_threshold < 0 || a.drop_threshold > 65536 || (a.drop_threshold > 0 && !dev_ptr(a.rng)))
+  if (a.drop_threshold < 0 || a.drop_threshold > 65535 || (a.drop_threshold > 0 && !dev_ptr(a.rng)))
     return GEOATTN_ERR_INVALID;
   for (const GeoAttnTensor* t : {&a.q, &a.k, &a.v})
     if (t->stride[3] != 1) return GEOATTN_ERR_ALIGNMENT;
@@ -160,7 +160,7 @@ XParams xparams(const GeoXattnInputs& a, const XDims& d) {
   }
   p.lens = a.kv_lens, p.kmask = a.key_mask, p.kmask_ld = a.key_mask_ld;
   p.rng = a.rng, p.drop_thr = a.drop_threshold;
-  p.drop_scale = a.drop_threshold >= 65536 ? 0.f : (float)(65536.0 / (65536 - a.drop_threshold));
+  p.drop_scale = (float)(65536.0 / (65536 - a.drop_threshold));
   p.scale = a.scale, p.scale_log2 = (float)((double)a.scale * 1.4426950408889634);
   p.nqp = d.nqp, p.nkp = d.nkp, p.splits = 1;
   return p;
@@ -218,8 +218,9 @@ int tc_launch(K kernel, long long grid, int threads, int smem, cudaStream_t st, 
 template <int DP>
 int tc_fwd(const xa::XMaps& maps, const XParams& p, long long grid, cudaStream_t st) {
   using C = xa::FwdCfg<DP>;
-  return p.ids ? tc_launch(xa::xattn_fwd_kernel<DP, true>, grid, C::THREADS, C::SMEM, st, maps, p)
-               : tc_launch(xa::xattn_fwd_kernel<DP, false>, grid, C::THREADS, C::SMEM, st, maps, p);
+  auto fwd = p.ids ? (p.drop_thr ? xa::xattn_fwd_kernel<DP, true, true> : xa::xattn_fwd_kernel<DP, true, false>)
+                   : (p.drop_thr ? xa::xattn_fwd_kernel<DP, false, true> : xa::xattn_fwd_kernel<DP, false, false>);
+  return tc_launch(fwd, grid, C::THREADS, C::SMEM, st, maps, p);
 }
 
 // 16-byte loads of ids rows: the caller's own where they allow it, else a padded copy.

@@ -33,6 +33,44 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return r;
 }
 
+// Two fp32 values in one 64-bit register: one instruction works on both.
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unf2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Barrier `id` among `threads` threads that also tells each whether any of them said yes.
+__device__ __forceinline__ bool named_any(int id, int threads, bool yes) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbarrier.cta.red.or.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(threads), "r"((uint32_t)yes)
+      : "memory");
+  return r != 0;
+}
+
 // NKB regions of `rows` x 128 bytes.
 template <int DP>
 __device__ __forceinline__ void load_rows(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int region, int row,
@@ -53,13 +91,15 @@ __device__ __forceinline__ void mma_scores(uint32_t acc, uint32_t a, uint32_t b)
                          smem_desc_sw128(b + kb * (64 * 128) + s * 32, 16, 1024), idesc, kb + s > 0);
 }
 
-// acc[128 x DP] (+)= A[128 x 64] B[64 x DP]: A in tensor memory (two bf16 per column), B with its rows along K.
+// acc[128 x DP] (+)= A[128 x 64] B[64 x DP]: A in tensor memory (two bf16 per column), each 32-wide piece at the start
+// of the 32 score columns that it replaces (another warpgroup may still read its own); B with its rows along K.
 template <int DP>
-__device__ __forceinline__ void mma_weights(uint32_t acc, uint32_t a, uint32_t b, bool accumulate) {
+__device__ __forceinline__ void mma_pieces(uint32_t acc, uint32_t a, uint32_t b, bool accumulate) {
   constexpr uint32_t idesc = instr_desc(1, 0, 1, 128, DP);
 #pragma unroll
   for (int s = 0; s < 4; ++s)
-    mma_ts<Kind::kF16>(acc, a + s * 8, smem_desc_sw128(b + s * 16 * 128, 64 * 128, 1024), idesc, accumulate || s > 0);
+    mma_ts<Kind::kF16>(acc, a + (s / 2) * 32 + (s % 2) * 8, smem_desc_sw128(b + s * 16 * 128, 64 * 128, 1024), idesc,
+                       accumulate || s > 0);
 }
 
 // Set row `r` of a 64-row tile to zero.
@@ -70,13 +110,6 @@ __device__ __forceinline__ void clear_row(uint8_t* tile, int r) {
 #pragma unroll
     for (int c = 0; c < 8; ++c)
       *reinterpret_cast<uint4*>(tile + kb * (64 * 128) + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
-}
-
-// Liveness of 64 keys from j0 on as two words, the same in every lane of the warp.
-__device__ __forceinline__ void live_words(const XParams& p, int b, int j0, int n, uint32_t (&w)[2]) {
-  const int lane = threadIdx.x & 31;
-  w[0] = __ballot_sync(0xffffffffu, key_live(p, b, j0 + lane, n));
-  w[1] = __ballot_sync(0xffffffffu, key_live(p, b, j0 + 32 + lane, n));
 }
 
 template <int N>
@@ -102,31 +135,34 @@ __device__ __forceinline__ bool vec_rows(const XTensor& t) {
 
 // ---------------------------------------------------------------------------------------------------------------
 // Forward. One CTA per (128 query rows, head, batch, key split), keys in chunks of 64:
-//   MMA warp   S(c + 1) = Q K^T into the other score buffer, then O += P(c) V(c)
-//   4 warps    P(c) = 2^(t - m), a row per thread; bf16, written over its scores
-// The running maximum moves only when it would grow by more than 2^kLazy (P stays below that, l and O are fp32), so O
-// is rescaled rarely; it then waits for O's product c - 1, the only one that can be in flight there (S(c) was issued
-// after product c - 2).
+//   MMA warp       S(c + 1) = Q K^T into the other score buffer, then O += P(c) V(c)
+//   2 warpgroups   P(c) = 2^(t - m): thread r of warpgroup w has row r and keys 32 w .. 32 w + 31 of the chunk; P goes
+//                  in bf16 over the scores it came from
+// m is one per row and moves only when a chunk would pass it by more than kLazy (P stays below 2^kLazy; l and O are
+// fp32): one barrier per chunk tells both warpgroups whether any row has to move, and only then do they exchange their
+// maxima and rescale O, after O's product c - 1 (the only one that can be in flight: S(c) was issued after c - 2).
 // Few queries of heads that share a key head (G * Nq <= 128) are packed into one tile's rows.
 // DP = 192 has room for one score buffer and one chunk of K and V; S(c + 1) then follows O's product c.
 // ---------------------------------------------------------------------------------------------------------------
 template <int DP>
 struct FwdCfg {
-  static constexpr int NSB = DP == 192 ? 1 : 2;              // score buffers
+  static constexpr int NSB = DP == 192 ? 1 : 2;                  // score buffers
   static constexpr int NKV = DP == 192 ? 1 : DP == 128 ? 2 : 4;  // chunks of K, and of V, in flight
   static constexpr int Q_BYTES = DP / 64 * 128 * 128, KV_BYTES = DP / 64 * 64 * 128;
   static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + NKV * KV_BYTES, OFF_TAB = OFF_V + NKV * KV_BYTES;
-  static constexpr int SMEM = OFF_TAB + 1024;
+  static constexpr int OFF_ROW = OFF_TAB + 1024;                 // [2][128] floats: what the warpgroups exchange
+  static constexpr int SMEM = OFF_ROW + 1024;
   static constexpr int TM_S = 0, TM_O = NSB * 64, TM_COLS = 256;
-  static constexpr int THREADS = 192, TMA_WARP = 4, MMA_WARP = 5;
+  static constexpr int EWT = 256, THREADS = EWT + 64, TMA_WARP = 8, MMA_WARP = 9;
 };
 constexpr float kLazy = 8.f;
 
-template <int DP, bool BIAS>
-__global__ void __launch_bounds__(192, 2) xattn_fwd_kernel(const __grid_constant__ XMaps maps, const XParams p) {
+template <int DP, bool BIAS, bool DROP>
+__global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant__ XMaps maps, const XParams p) {
   using C = FwdCfg<DP>;
   constexpr int NKV = C::NKV, NSB = C::NSB;
-  __shared__ uint64_t bar_q, bar_kfull[NKV], bar_kempty[NKV], bar_vfull[NKV], bar_vempty[NKV], bar_s[NSB], bar_p[NSB], bar_pv[2];
+  __shared__ uint64_t bar_q, bar_kfull[NKV], bar_kempty[NKV], bar_vfull[NKV], bar_vempty[NKV], bar_s[NSB], bar_p[NSB],
+      bar_pv[2];
   __shared__ uint32_t tmem_sh;
   __shared__ int abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -153,7 +189,7 @@ __global__ void __launch_bounds__(192, 2) xattn_fwd_kernel(const __grid_constant
     }
     for (int i = 0; i < NSB; ++i) {
       mbar_init(&bar_s[i], 1);
-      mbar_init(&bar_p[i], 128);
+      mbar_init(&bar_p[i], C::EWT);
     }
     for (int i = 0; i < 2; ++i) mbar_init(&bar_pv[i], 1);
     fence_barrier_init();
@@ -163,8 +199,7 @@ __global__ void __launch_bounds__(192, 2) xattn_fwd_kernel(const __grid_constant
     tmem_relinquish();
   }
   float* tab = reinterpret_cast<float*>(xsmem + C::OFF_TAB);
-  if (BIAS)
-    for (int t = threadIdx.x; t < 256; t += C::THREADS) tab[t] = table_log2(p, hx, t);
+  if (BIAS && threadIdx.x < 256) tab[threadIdx.x] = table_log2(p, hx, threadIdx.x);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -205,117 +240,147 @@ __global__ void __launch_bounds__(192, 2) xattn_fwd_kernel(const __grid_constant
       for (int c = 0; c < nc && ok; ++c) {
         if (NSB == 2 && c + 1 < nc) scores(c + 1);
         const int st = c % NKV;
-        if (!(ok = ok && mbar_wait(&bar_p[c % NSB], (c / NSB) & 1, ctx) && mbar_wait(&bar_vfull[st], (c / NKV) & 1, ctx))) break;
+        if (!(ok = ok && mbar_wait(&bar_p[c % NSB], (c / NSB) & 1, ctx) && mbar_wait(&bar_vfull[st], (c / NKV) & 1, ctx)))
+          break;
         tc_fence_after();
-        mma_weights<DP>(tmem + C::TM_O, tmem + C::TM_S + (c % NSB) * 64, sbase + C::OFF_V + st * C::KV_BYTES, c > 0);
+        mma_pieces<DP>(tmem + C::TM_O, tmem + C::TM_S + (c % NSB) * 64, sbase + C::OFF_V + st * C::KV_BYTES, c > 0);
         mma_commit(&bar_vempty[st]);
         mma_commit(&bar_pv[c & 1]);
         if (NSB == 1 && c + 1 < nc) scores(c + 1);
       }
     }
   } else {
-    const int r = warp * 32 + lane;
-    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    const int wg = warp / 4, r = (warp & 3) * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const int i = pack ? r % p.Nq : qt * 128 + r;
     const int h = pack ? kh * p.G + r / p.Nq : hx;
     const bool row = pack ? r < p.G * p.Nq : i < p.Nq;
     const bool any_row = __any_sync(0xffffffffu, row);
     const int bh = b * p.H + h;
-    const AttnDrop drop = attn_drop(p.rng, p.drop_thr, p.drop_scale);
+    const AttnDrop drop = attn_drop(p.rng, DROP ? p.drop_thr : 0, p.drop_scale);
+    const uint32_t thr2 = drop.pair();
     const uint8_t* idrow = BIAS ? p.ids + (long long)(row ? i : 0) * p.ids_ld : nullptr;
-    const bool check_keys = p.kmask != nullptr;
+    float* xrow = reinterpret_cast<float*>(xsmem + C::OFF_ROW);
+    const uint64_t sc2 = f2(p.scale_log2, p.scale_log2);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int c = 0; c < nc; ++c) {
-      const int j0 = (c0 + c) * 64;
-      uint32_t live[2] = {~0u, ~0u};
-      if (check_keys || j0 + 64 > n) live_words(p, b, j0, n, live);
-      uint4 id4[4];
-      if (BIAS) {  // 16 ids per load; the last ones of a row may lie past Nk: excluded
+    // this thread's 32 ids and this lane's key of the next chunk, fetched a chunk ahead
+    uint4 id4[2];
+    bool live_next = false;
+    auto fetch = [&](int c) {
+      const int j0 = (c0 + c) * 64 + wg * 32;
+      live_next = key_live(p, b, j0 + lane, n);
+      if (BIAS) {  // 16 ids per load; keys past Nk are excluded
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
+        for (int x = 0; x < 2; ++x)
           id4[x] = j0 + x * 16 < p.Nk ? __ldg(reinterpret_cast<const uint4*>(idrow + j0) + x)
                                       : make_uint4(~0u, ~0u, ~0u, ~0u);
       }
-      const uint32_t sbuf = lanes + C::TM_S + (c % NSB) * 64;
+    };
+    if (nc > 0) fetch(0);
+    for (int c = 0; c < nc; ++c) {
+      const int j0 = (c0 + c) * 64 + wg * 32;
+      const uint32_t live = __ballot_sync(0xffffffffu, live_next);
+      const uint32_t sbuf = lanes + C::TM_S + (c % NSB) * 64 + wg * 32;
       if (ok) ok = warp_wait(&bar_s[c % NSB], (c / NSB) & 1, ctx);
-      if (!ok) break;
       tc_fence_after();
-      if (any_row) {
-        uint32_t lo[32], hi[32];
-        tmem_ld32_issue(sbuf, lo);
-        tmem_ld32_issue(sbuf + 32, hi);
-        tmem_wait32(lo);
-        tmem_pin32(hi);
-        float x[64];
+      uint64_t x[16];
+      float mx = -INFINITY;
+      if (ok && any_row) {
+        uint32_t s[32];
+        tmem_ld32_issue(sbuf, s);
+        tmem_wait32(s);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          x[e] = __uint_as_float(lo[e]);
-          x[e + 32] = __uint_as_float(hi[e]);
+        for (int e = 0; e < 16; ++e) {
+          float a = __uint_as_float(s[2 * e]), d = __uint_as_float(s[2 * e + 1]);
+          x[e] = f2(a, d);
+          if (BIAS) {
+            const uint32_t w = reinterpret_cast<const uint32_t*>(id4)[e / 2] >> (16 * (e & 1));
+            x[e] = fma2(x[e], sc2, f2(tab[w & 255], tab[(w >> 8) & 255]));
+          }
         }
-        if (BIAS) {
-          const uint32_t* w = reinterpret_cast<const uint32_t*>(id4);
+        if (live != ~0u) {
 #pragma unroll
-          for (int e = 0; e < 64; ++e) x[e] = fmaf(x[e], p.scale_log2, tab[(w[e / 4] >> (8 * (e % 4))) & 255]);
+          for (int e = 0; e < 16; ++e) {
+            float a, d;
+            unf2(x[e], a, d);
+            x[e] = f2((live >> (2 * e)) & 1 ? a : -INFINITY, (live >> (2 * e + 1)) & 1 ? d : -INFINITY);
+          }
         }
-        if ((live[0] & live[1]) != ~0u) {
+        float y[4];
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (!((live[e / 32] >> (e % 32)) & 1)) x[e] = -INFINITY;
+        for (int e = 0; e < 4; ++e) {
+          float a, d, g, f;
+          unf2(x[e], a, d);
+          unf2(x[e + 4], g, f);
+          y[e] = max3(fmaxf(a, d), g, f);
+          unf2(x[e + 8], a, d);
+          y[e] = max3(y[e], a, d);
+          unf2(x[e + 12], a, d);
+          y[e] = max3(y[e], a, d);
         }
-        float mx = x[0];
-#pragma unroll
-        for (int e = 1; e < 64; ++e) mx = fmaxf(mx, x[e]);
+        mx = fmaxf(max3(y[0], y[1], y[2]), y[3]);
         if (!BIAS) mx *= p.scale_log2;  // x is still the raw product (scale > 0: the order and -inf stay)
-        const bool grow = mx > m + kLazy || (m == -INFINITY && mx > m);
-        if (__any_sync(0xffffffffu, grow && l > 0.f)) {  // O holds something to rescale
-          if (!(ok = warp_wait(&bar_pv[(c - 1) & 1], ((c - 1) >> 1) & 1, ctx))) break;
+      }
+      if (c + 1 < nc) fetch(c + 1);
+      if (named_any(1, C::EWT, row && (mx > m + kLazy || (m == -INFINITY && mx > m)))) {
+        xrow[wg * 128 + r] = mx;
+        named_sync(2, C::EWT);
+        const float top = fmaxf(mx, xrow[(wg ^ 1) * 128 + r]);
+        const bool grow = top > m + kLazy || (m == -INFINITY && top > m);
+        const float f = grow ? xex2(m - top) : 1.f;
+        l *= f;
+        m = grow ? top : m;
+        if (c > 0) {
+          if (ok) ok = warp_wait(&bar_pv[(c - 1) & 1], ((c - 1) >> 1) & 1, ctx);
           tc_fence_after();
-          const float f = grow ? xex2(m - mx) : 1.f;
-          l *= f;
+          if (ok && __any_sync(0xffffffffu, grow)) {
 #pragma unroll 1
-          for (int d = 0; d < DP; d += 16) {
-            uint32_t o[16];
-            tmem_ld16_issue(lanes + C::TM_O + d, o);
-            tmem_wait16(o);
+            for (int d = wg * (DP / 2); d < (wg + 1) * (DP / 2); d += 16) {
+              uint32_t o[16];
+              tmem_ld16_issue(lanes + C::TM_O + d, o);
+              tmem_wait16(o);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st16(lanes + C::TM_O + d, o);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st16(lanes + C::TM_O + d, o);
+            }
           }
-          tmem_wait_st();
         }
-        if (grow) m = mx;
+      }
+      if (ok && any_row) {
         const float base = m == -INFINITY ? 0.f : m;
-        float sum = 0.f;
+        const uint64_t nb2 = f2(-base, -base);
+        uint64_t sum[2] = {0, 0};  // two pairs of zeros
+        uint32_t w[16];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t w[16];
+        for (int g = 0; g < 4; ++g) {
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float t = x[half * 32 + g * 8 + e];
-              v[e] = xex2(BIAS ? t - base : fmaf(t, p.scale_log2, -base));
-              sum += v[e];
-            }
-            if (drop.thr) {
-              const uint32_t keep = drop.keep8(i, (j0 >> 3) + half * 4 + g, bh);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] = (keep >> e) & 1 ? v[e] : 0.f;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[g * 4 + e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+          for (int e = 0; e < 4; ++e) {
+            const uint64_t t = BIAS ? add2(x[4 * g + e], nb2) : fma2(x[4 * g + e], sc2, nb2);
+            float a, d;
+            unf2(t, a, d);
+            a = xex2(a), d = xex2(d);
+            sum[e & 1] = add2(sum[e & 1], f2(a, d));
+            w[g * 4 + e] = pack_bf16(a, d);
           }
-          tmem_st16(sbuf + half * 16, w);
+          if (DROP) {
+            const uint4 u = drop.words(i, (j0 >> 3) + g, bh);
+            w[g * 4] &= spread_pair(keep_pair(u.x, thr2));
+            w[g * 4 + 1] &= spread_pair(keep_pair(u.y, thr2));
+            w[g * 4 + 2] &= spread_pair(keep_pair(u.z, thr2));
+            w[g * 4 + 3] &= spread_pair(keep_pair(u.w, thr2));
+          }
         }
-        l += sum;
+        tmem_st16(sbuf, w);
+        float a, d;
+        unf2(add2(sum[0], sum[1]), a, d);
+        l += a + d;
         tmem_wait_st();
       }
-      if ((live[0] & live[1]) != ~0u) {  // what absent keys hold must not reach the product: 0 * NaN
-        if (!(ok = warp_wait(&bar_vfull[c % NKV], (c / NKV) & 1, ctx))) break;
-        if (r < 64 && !((live[r / 32] >> (r % 32)) & 1)) {
-          clear_row<DP>(xsmem + C::OFF_V + (c % NKV) * C::KV_BYTES, r);
+      if (live != ~0u) {  // what absent keys hold must not reach the product: 0 * NaN
+        if (ok) ok = warp_wait(&bar_vfull[c % NKV], (c / NKV) & 1, ctx);
+        if (ok && (warp & 3) == 0 && !((live >> lane) & 1)) {
+          clear_row<DP>(xsmem + C::OFF_V + (c % NKV) * C::KV_BYTES, wg * 32 + lane);
           fence_proxy_async_smem();
         }
       }
@@ -324,41 +389,42 @@ __global__ void __launch_bounds__(192, 2) xattn_fwd_kernel(const __grid_constant
     }
     if (ok && nc > 0) ok = warp_wait(&bar_pv[(nc - 1) & 1], ((nc - 1) >> 1) & 1, ctx);
     tc_fence_after();
+    named_sync(2, C::EWT);  // the last exchange has been read
+    xrow[wg * 128 + r] = l;
+    named_sync(2, C::EWT);
+    l += xrow[(wg ^ 1) * 128 + r];
     const long long stat = (long long)bh * p.Nq + i;
     const long long part = (long long)split * p.B * p.H * p.Nq + stat;
-    const float f = l == 0.f ? 0.f : (p.drop_thr ? p.drop_scale : 1.f) / l;
+    const float f = l == 0.f ? 0.f : (DROP ? p.drop_scale : 1.f) / l;
     const bool vec = vec_rows(p.o);
     if (ok && any_row) {
 #pragma unroll 1
-      for (int d = 0; d < DP; d += 32) {
+      for (int d = wg * (DP / 2); d < (wg + 1) * (DP / 2); d += 32) {
         float o[32];
-        if (nc > 0) {
-          tmem_ld32(lanes + C::TM_O + d, o);
-        } else {
+        if (nc > 0) tmem_ld32(lanes + C::TM_O + d, o);
+        if (!row || d >= p.D) continue;
+        if (l == 0.f) {  // a row with nothing left (or no chunk at all)
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0.f;
         }
-        if (!row || d >= p.D) continue;
         if (p.splits > 1) {
           float* dst = p.part_o + part * p.D + d;
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if (d + e < p.D) dst[e] = l == 0.f ? 0.f : o[e];
+            if (d + e < p.D) dst[e] = o[e];
         } else {
           __nv_bfloat16* dst =
               reinterpret_cast<__nv_bfloat16*>(p.o.p) + b * p.o.s[0] + h * p.o.s[1] + (long long)i * p.o.s[2] + d;
-          if (l == 0.f) {  // a row with nothing left
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0.f;
-          }
           store_row(dst, o, f, p.D - d, vec);
         }
       }
-      if (row && p.splits > 1) {
-        p.part_ml[part * 2] = m;
-        p.part_ml[part * 2 + 1] = l;
-      } else if (row && p.stats) {
-        p.stats[stat] = row_stats(m, l);
+      if (row && wg == 0) {
+        if (p.splits > 1) {
+          p.part_ml[part * 2] = m;
+          p.part_ml[part * 2 + 1] = l;
+        } else if (p.stats) {
+          p.stats[stat] = row_stats(m, l);
+        }
       }
     }
   }
@@ -437,16 +503,6 @@ struct KeysCfg {
   static constexpr int TM_DK = 0, TM_DV = DP, TM_S = 2 * DP, TM_COLS = CTAS == 2 ? 256 : 512;
   static constexpr int THREADS = EW * 128 + 64, TMA_WARP = EW * 4, MMA_WARP = EW * 4 + 1;
 };
-
-// acc[128 x DP] (+)= A[128 x 64] B[64 x DP]: A's 32-wide pieces at the start of their own 32 score columns.
-template <int DP>
-__device__ __forceinline__ void mma_pieces(uint32_t acc, uint32_t a, uint32_t b, bool accumulate) {
-  constexpr uint32_t idesc = instr_desc(1, 0, 1, 128, DP);
-#pragma unroll
-  for (int s = 0; s < 4; ++s)
-    mma_ts<Kind::kF16>(acc, a + (s / 2) * 32 + (s % 2) * 8, smem_desc_sw128(b + s * 16 * 128, 64 * 128, 1024), idesc,
-                       accumulate || s > 0);
-}
 
 // Keep bits of 32 queries (i0 ..) for this lane's key j0 + lane: bit q of the result.
 __device__ __forceinline__ uint32_t keep_column(const AttnDrop& drop, uint32_t i0, uint32_t j0, uint32_t bh) {

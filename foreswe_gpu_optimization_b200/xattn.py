@@ -57,7 +57,7 @@ def _inputs(q, k, v, table, ids, lens, mask, rng, thr, scale):
 
 def _forward(q, k, v, table, ids, lens, mask, rng, thr, scale, need_stats):
     o = _like(q)
-    if k.shape[2] == 0:
+    if k.shape[2] == 0 or thr == 65536:  # no key, or no weight is kept
         return o.zero_(), None
     q, k, v = _ready(q), _ready(k), _ready(v)
     L = _lib.lib()
@@ -72,8 +72,8 @@ def _forward(q, k, v, table, ids, lens, mask, rng, thr, scale, need_stats):
 def _backward(q, k, v, table, ids, lens, mask, rng, thr, scale, o, stats, do):
     dq, dk, dv = _like(q), _like(k), _like(v)
     dtable = torch.empty_like(table, memory_format=torch.contiguous_format) if table is not None else None
-    if k.shape[2] == 0:
-        return dq.zero_(), dk, dv, None if dtable is None else dtable.zero_()
+    if k.shape[2] == 0 or thr == 65536:
+        return dq.zero_(), dk.zero_(), dv.zero_(), None if dtable is None else dtable.zero_()
     q, k, v, do = _ready(q), _ready(k), _ready(v), _ready(do)
     L = _lib.lib()
     inp = _inputs(q, k, v, table, ids, lens, mask, rng, thr, scale)

@@ -159,7 +159,7 @@ typedef struct {
   const unsigned char* key_mask; /* [batch][key_mask_ld], 0 = absent, or NULL */
   long long key_mask_ld;
   const long long* rng;         /* device (seed, offset) of the dropout generator; read when drop_threshold > 0 */
-  int drop_threshold;           /* round(65536 p): 0 = no dropout, 65536 = nothing kept */
+  int drop_threshold;           /* round(65536 p), 0..65535; 0 = no dropout */
   float scale;
 } GeoXattnInputs;
 
