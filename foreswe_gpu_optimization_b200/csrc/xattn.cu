@@ -55,6 +55,7 @@ int check_xshape(const GeoXattnShape* s, XDims& d) {
   if (d.Nq > (1 << 30) || d.Nk > (1 << 30) || (long long)d.B * d.H > (1 << 30)) return GEOATTN_ERR_UNSUPPORTED;
   d.nqp = (d.Nq + 63) / 64 * 64;
   d.nkp = (d.Nk + 127) / 128 * 128;
+  if (d.T && (d.nqp / 64 > 65535 || d.nkp / 64 > 65535)) return GEOATTN_ERR_UNSUPPORTED;  // grid of the ids' tiles
   d.splits = forward_splits(d);
   const long long qt = (d.Nq + 63) / 64, kt = (d.Nk + 31) / 32;
   if (qt * d.B * d.H * d.splits > (1ll << 30) || kt * d.B * d.Hkv > (1ll << 30)) return GEOATTN_ERR_UNSUPPORTED;
@@ -64,7 +65,7 @@ int check_xshape(const GeoXattnShape* s, XDims& d) {
   per = per < 1 ? 1 : per > units ? units : per;
   d.units_per_launch = (int)per;
   d.launches = (int)((units + per - 1) / per);
-  const long long want = (8ll * kSMs + d.H - 1) / d.H, most = ((long long)d.Nk * d.nqp / 4 + 255) / 256;
+  const long long want = (16ll * kSMs + d.H - 1) / d.H, most = (long long)d.nkp * d.nqp / (d.bf16 ? 8 : 4) / 256;
   d.chunks = (int)(want < most ? want : most);
   return GEOATTN_OK;
 }
@@ -88,7 +89,7 @@ size_t xfwd_ws(const XDims& d, uint8_t* base, XFwdWs* w) {
     t.part_o = reinterpret_cast<float*>(take(rows * d.D * 4));
     t.part_ml = reinterpret_cast<float*>(take(rows * 2 * 4));
   }
-  if (d.T && d.bf16) t.ids = take((size_t)d.Nq * d.nkp);
+  if (d.T && d.bf16) t.ids = take((size_t)d.nqp * d.nkp);
   if (w) *w = t;
   return off;
 }
@@ -223,13 +224,11 @@ int tc_fwd(const xa::XMaps& maps, const XParams& p, long long grid, cudaStream_t
   return tc_launch(fwd, grid, C::THREADS, C::SMEM, st, maps, p);
 }
 
-// 16-byte loads of ids rows: the caller's own where they allow it, else a padded copy.
-int aligned_ids(XParams& p, const XDims& d, uint8_t* copy, cudaStream_t st) {
-  if (!p.ids || ((p.ids_ld | d.Nk | (long long)reinterpret_cast<uintptr_t>(p.ids)) & 15) == 0) return GEOATTN_OK;
-  const long long blocks = ((long long)d.Nq * d.nkp / 4 + 255) / 256;
-  ids_pad_kernel<<<(unsigned)blocks, 256, 0, st>>>(p.ids, p.ids_ld, d.Nq, d.Nk, d.nkp, copy);
-  p.ids = copy, p.ids_ld = d.nkp;
-  return status_of(cudaGetLastError());
+// Store maps of the outputs that TMA can write (box: 64 columns x 128 rows, or a packed tile's rows); the others leave
+// by plain stores.
+void out_map(CUtensorMap* m, int* flags, int bit, const XTensor& t, int D, int n, int heads, int batch, int rows = 128,
+             int box_heads = 1) {
+  if (xmap(m, t, D, n, heads, batch, rows, box_heads) == GEOATTN_OK) *flags |= bit;
 }
 
 int forward_tc(XParams& p, const XDims& d, uint8_t* ids, cudaStream_t st) {
@@ -238,23 +237,40 @@ int forward_tc(XParams& p, const XDims& d, uint8_t* ids, cudaStream_t st) {
   p.pack = packs_rows(d);
   int rc;
   if ((rc = p.pack ? xmap(&maps.q, p.q, d.D, d.Nq, d.H, d.B, d.Nq, d.G) : xmap(&maps.q, p.q, d.D, d.Nq, d.H, d.B, 128, 1)) ||
-      (rc = xmap(&maps.k, p.k, d.D, d.Nk, d.Hkv, d.B, 64, 1)) || (rc = xmap(&maps.v, p.v, d.D, d.Nk, d.Hkv, d.B, 64, 1)) ||
-      (rc = aligned_ids(p, d, ids, st)))
+      (rc = xmap(&maps.k, p.k, d.D, d.Nk, d.Hkv, d.B, 64, 1)) || (rc = xmap(&maps.v, p.v, d.D, d.Nk, d.Hkv, d.B, 64, 1)))
     return rc;
+  if (p.pack) out_map(&maps.o, &p.out_tma, 1, p.o, d.D, d.Nq, d.H, d.B, d.Nq, d.G);
+  else out_map(&maps.o, &p.out_tma, 1, p.o, d.D, d.Nq, d.H, d.B);
+  if (d.T) {
+    ids_tile_kernel<false><<<dim3(d.nkp / 64, d.nqp / 64), 256, 0, st>>>(p.ids, p.ids_ld, d.Nq, d.Nk, d.nkp, ids);
+    p.ids = ids;
+    if ((rc = status_of(cudaGetLastError()))) return rc;
+  }
   const long long grid = (long long)d.splits * d.B * (p.pack ? d.Hkv : (long long)((d.Nq + 127) / 128) * d.H);
   return d.DP == 64 ? tc_fwd<64>(maps, p, grid, st)
                     : d.DP == 128 ? tc_fwd<128>(maps, p, grid, st) : tc_fwd<192>(maps, p, grid, st);
 }
 
-int backward_maps(xa::XMaps& maps, const XParams& p, const XDims& d) {
+int backward_maps(xa::XMaps& maps, XParams& p, const XDims& d) {
   int rc;
   if ((rc = xmap(&maps.q, p.q, d.D, d.Nq, d.H, d.B, 64, 1)) || (rc = xmap(&maps.dout, p.dout, d.D, d.Nq, d.H, d.B, 64, 1)) ||
       (rc = xmap(&maps.k, p.k, d.D, d.Nk, d.Hkv, d.B, 64, 1)) || (rc = xmap(&maps.v, p.v, d.D, d.Nk, d.Hkv, d.B, 64, 1)))
     return rc;
-  const uint64_t dims[3] = {(uint64_t)d.nqp, (uint64_t)d.nkp, (uint64_t)d.units_per_launch * d.G};
-  const uint64_t str[2] = {(uint64_t)d.nqp * 2, (uint64_t)d.nqp * d.nkp * 2};
-  const uint32_t box[3] = {64, 64, 1};
-  return make_tmap(&maps.ds, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, p.ds, dims, str, box) ? GEOATTN_OK : GEOATTN_ERR_TMA;
+  out_map(&maps.dq, &p.out_tma, 1, p.dq, d.D, d.Nq, d.H, d.B);
+  out_map(&maps.dk, &p.out_tma, 2, p.dk, d.D, d.Nk, d.Hkv, d.B);
+  out_map(&maps.dv, &p.out_tma, 4, p.dv, d.D, d.Nk, d.Hkv, d.B);
+  return GEOATTN_OK;
+}
+
+int records(const XParams& p, const XDims& d, cudaStream_t st) {
+  // 16 bytes per lane, a row per 8, 16 or 32 lanes, 4 rows per lane in flight
+  const long long rows = (long long)d.B * d.H * d.nqp, per = 8 * 4 * (d.DP == 64 ? 4 : d.DP == 128 ? 2 : 1);
+  const unsigned grid = (unsigned)((rows + per - 1) / per);
+  const int heads_first = p.o.s[1] < p.o.s[2];
+  if (d.DP == 64) xa::xattn_records_kernel<8><<<grid, 256, 0, st>>>(p, heads_first);
+  else if (d.DP == 128) xa::xattn_records_kernel<16><<<grid, 256, 0, st>>>(p, heads_first);
+  else xa::xattn_records_kernel<32><<<grid, 256, 0, st>>>(p, heads_first);
+  return status_of(cudaGetLastError());
 }
 
 template <int DP>
@@ -345,11 +361,11 @@ int geoattn_xattn_bwd(const GeoXattnBwdArgs* a, void* stream) {
   int rc = d.bf16 ? backward_maps(maps, p, d) : GEOATTN_OK;
   if (rc) return rc;
   if (cudaMemsetAsync(ws.status, 0, sizeof(int), st) != cudaSuccess) return GEOATTN_ERR_LAUNCH;
-  rc = d.bf16 ? xlaunch(xa::xattn_records_kernel, ((long long)d.B * d.H * d.nqp + 7) / 8, 256, 0, st, p)
+  rc = d.bf16 ? records(p, d, st)
               : xlaunch(xattn_delta_kernel, ((long long)d.B * d.H * d.Nq + 7) / 8, 256, 0, st, p);
   if (rc) return rc;
   if (d.T) {
-    ids_transpose_kernel<<<dim3(d.nqp / 64, d.nkp / 64), 256, 0, st>>>(p.ids, p.ids_ld, d.Nq, d.Nk, d.nqp, ws.idsT);
+    ids_tile_kernel<true><<<dim3(d.nqp / 64, d.nkp / 64), 256, 0, st>>>(p.ids, p.ids_ld, d.Nq, d.Nk, d.nqp, ws.idsT);
     if ((rc = status_of(cudaGetLastError()))) return rc;
   }
   const int units = d.B * d.Hkv;

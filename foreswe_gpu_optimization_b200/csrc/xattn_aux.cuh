@@ -29,63 +29,74 @@ __global__ void __launch_bounds__(256) distance_buckets_kernel(int nq, const dou
   ids[x] = km > max_km ? (uint8_t)kNoPair : (uint8_t)n;
 }
 
-// out[i][j] = ids[i][j], rows padded to `ldo` (a multiple of 16) with kNoPair: what 16-byte loads need.
-__global__ void __launch_bounds__(256) ids_pad_kernel(const uint8_t* __restrict__ ids, long long ld, int nq, int nk,
-                                                      int ldo, uint8_t* __restrict__ out) {
-  const long long x = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (x >= (long long)nq * ldo) return;
-  const long long i = x / ldo;
-  const int j = (int)(x % ldo);
-  uint32_t w = 0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) w |= (uint32_t)(j + e < nk ? ids[i * ld + j + e] : (uint8_t)kNoPair) << (8 * e);
-  *reinterpret_cast<uint32_t*>(out + x) = w;
-}
-
-// idsT[j][i] = ids[i][j], padded to [nkp][nqp] with kNoPair.
-__global__ void __launch_bounds__(256) ids_transpose_kernel(const uint8_t* __restrict__ ids, long long ld, int nq,
-                                                            int nk, int nqp, uint8_t* __restrict__ idsT) {
-  __shared__ uint8_t tile[64][65];
-  const int i0 = blockIdx.x * 64, j0 = blockIdx.y * 64;
+// Tiled copy of the bucket ids, out[row / 64][col / 8][row % 64][8], padded with kNoPair to [rows_p][cols_p]: a warp
+// whose lanes are consecutive rows reads 8 columns as one contiguous block (row-major rows cost a cache line per lane).
+// TRANS: rows are the keys and columns the queries (backward), else the other way round. A 64 x 64 tile per CTA.
+template <bool TRANS>
+__global__ void __launch_bounds__(256) ids_tile_kernel(const uint8_t* __restrict__ ids, long long ld, int nq, int nk,
+                                                       int cols_p, uint8_t* __restrict__ out) {
+  __shared__ uint8_t tile[64][68];  // [query][key]
+  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+  const int i0 = TRANS ? c0 : r0, j0 = TRANS ? r0 : c0;
   for (int x = threadIdx.x; x < 64 * 64; x += 256) {
-    const int r = x / 64, c = x % 64;
-    tile[r][c] = i0 + r < nq && j0 + c < nk ? ids[(long long)(i0 + r) * ld + j0 + c] : (uint8_t)kNoPair;
+    const int i = x / 64, j = x % 64;
+    tile[i][j] = i0 + i < nq && j0 + j < nk ? ids[(long long)(i0 + i) * ld + j0 + j] : (uint8_t)kNoPair;
   }
   __syncthreads();
-  for (int x = threadIdx.x; x < 64 * 16; x += 256) {
-    const int r = x / 16, c = (x % 16) * 4;
-    const uint32_t w = tile[c][r] | tile[c + 1][r] << 8 | tile[c + 2][r] << 16 | (uint32_t)tile[c + 3][r] << 24;
-    *reinterpret_cast<uint32_t*>(idsT + (long long)(j0 + r) * nqp + i0 + c) = w;
+  uint2* dst = reinterpret_cast<uint2*>(out) + ((long long)blockIdx.y * (cols_p / 8) + c0 / 8) * 64;
+  for (int x = threadIdx.x; x < 64 * 8; x += 256) {
+    const int r = x % 64, g = x / 64;
+    uint32_t w[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      w[k] = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int c = g * 8 + k * 4 + e;
+        w[k] |= (uint32_t)(TRANS ? tile[c][r] : tile[r][c]) << (8 * e);
+      }
+    }
+    dst[(long long)g * 64 + r] = make_uint2(w[0], w[1]);
   }
 }
 
 // Bias gradient of one launch's units: part[h][chunk][t] = sum of dS over the chunk's pairs of bucket t and the
-// launch's batches. A thread sums its pairs over the batch first and then adds them to its own column of the
-// shared histogram (hist[t][thread]: no atomics, no bank conflicts, a fixed order). Bound by reading dS once.
+// launch's batches. dS lies as the ids do, [key / 64][query / 8][key % 64][8] per head; a thread takes 16 bytes of it,
+// sums them over the batch first (8 loads in flight) and then adds them to its own column of the shared histogram
+// (hist[t][thread]: no atomics, no bank conflicts, a fixed order). Bound by reading dS once.
 template <class S>
 __global__ void __launch_bounds__(256) table_grad_kernel(const XParams p, int units, float* __restrict__ part) {
   constexpr int VEC = 16 / (int)sizeof(S);
   extern __shared__ float hist[];  // [T][256]
   const int h = blockIdx.y, kh = h / p.G, chunks = gridDim.x;
   for (int t = 0; t < p.T; ++t) hist[t * 256 + threadIdx.x] = 0.f;
-  const long long per_row = p.nqp / VEC, total = (long long)p.Nk * per_row;
+  const long long slab = (long long)p.nkp * p.nqp, total = slab / VEC;
   const long long c0 = total * blockIdx.x / chunks, c1 = total * (blockIdx.x + 1) / chunks;
-  const long long slab = (long long)p.nkp * p.nqp;
   const int first = (kh - p.u0 % p.Hkv + p.Hkv) % p.Hkv;  // first local unit of this key head
+  const long long step = (long long)p.Hkv * p.G * slab;
   for (long long x = c0 + threadIdx.x; x < c1; x += 256) {
-    const int j = (int)(x / per_row);
-    const long long at = (long long)j * p.nqp + (x % per_row) * VEC;
+    const long long at = x * VEC;
+    const int j = (int)(at / (64ll * p.nqp)) * 64 + (int)(at / 8 % 64);
+    const S* src = reinterpret_cast<const S*>(p.ds) + (long long)(first * p.G + h % p.G) * slab + at;
     float sum[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) sum[e] = 0.f;
-#pragma unroll 4
-    for (int ul = first; ul < units; ul += p.Hkv) {
-      if (p.lens && j >= key_count(p, (p.u0 + ul) / p.Hkv)) continue;  // rows that the key pass left out
-      const S* s = reinterpret_cast<const S*>(p.ds) + (long long)(ul * p.G + h % p.G) * slab + at;
-      const uint4 w = *reinterpret_cast<const uint4*>(s);
-      const S* v = reinterpret_cast<const S*>(&w);
+    for (int ul = first; ul < units; ul += 8 * p.Hkv) {
+      uint4 w[8];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) sum[e] += to_f(v[e]);
+      for (int k = 0; k < 8; ++k) {
+        const int u = ul + k * p.Hkv;
+        // keys that the key pass left out hold nothing
+        w[k] = u < units && j < key_count(p, (p.u0 + u) / p.Hkv) ? __ldcs(reinterpret_cast<const uint4*>(src + k * step))
+                                                                 : make_uint4(0, 0, 0, 0);
+      }
+      src += 8 * step;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const S* v = reinterpret_cast<const S*>(&w[k]);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum[e] += to_f(v[e]);
+      }
     }
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {

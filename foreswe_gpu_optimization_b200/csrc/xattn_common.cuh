@@ -26,9 +26,9 @@ struct XTensor {
 struct XParams {
   int B, H, Hkv, G, Nq, Nk, D, T;
   XTensor q, k, v, o, dout, dq, dk, dv;
-  const uint8_t* ids;       // [Nq][ids_ld] or null
+  const uint8_t* ids;       // [Nq][ids_ld] or null; bf16 forward: tiled, rows = queries, columns padded to nkp
   long long ids_ld;
-  const uint8_t* idsT;      // [nkp][nqp], padded with kNoPair (backward)
+  const uint8_t* idsT;      // tiled, rows = keys (nkp), columns = queries (nqp) (backward)
   const void* table;        // [H][T], bf16 or fp32
   int table_bf16;
   const int* lens;          // [B] or null
@@ -42,9 +42,10 @@ struct XParams {
                             // a bias near the type's lowest value would swallow log2(l)
   float* delta;             // [B*H][Nq] (fp32)
   float* rec;               // row records (bf16, xattn_records_kernel)
-  void* ds;                 // dS^T [units * G heads][nkp][nqp] of the launch's units
+  void* ds;                 // dS of the launch's units, [unit * G + head][key / 64][query / 8][key % 64][8] (padded)
   int nqp, nkp;             // Nq, Nk rounded up to 64 and 128
   int u0;                   // first (batch, key head) unit of this launch
+  int out_tma;              // bit x: output x leaves through TMA stores (o; or dq, dk, dv)
   int pack;                 // forward, tensor cores: a tile holds the G * Nq rows of a key head's group
   int splits;               // > 1: key ranges per row, joined by xattn_combine_kernel
   float* part_o;            // [splits][B*H*Nq][D]

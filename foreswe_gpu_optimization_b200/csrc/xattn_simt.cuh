@@ -360,14 +360,15 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_keys_kernel(const
           dp[r][c] = live[tx * KT + c] == 0.f ? pr * (g - dl) : 0.f;
         }
       }
-      float* ds = reinterpret_cast<float*>(p.ds) + (long long)(ul * p.G + it / nqt) * p.nkp * p.nqp;
+      float* ds = reinterpret_cast<float*>(p.ds) + (long long)(ul * p.G + it / nqt) * p.nkp * p.nqp +
+                  ((long long)(j0 / 64) * (p.nqp / 8) + (i0 + ty * 4) / 8) * 512 + (ty & 1) * 4;
 #pragma unroll
       for (int c = 0; c < KT; ++c) {
         const float4 a4 = make_float4(s[0][c], s[1][c], s[2][c], s[3][c]);
         const float4 d4 = make_float4(dp[0][c], dp[1][c], dp[2][c], dp[3][c]);
         *reinterpret_cast<float4*>(pt + (tx * KT + c) * C::SQ + ty * 4) = a4;
         *reinterpret_cast<float4*>(st + (tx * KT + c) * C::SQ + ty * 4) = d4;
-        *reinterpret_cast<float4*>(ds + (long long)(j0 + tx * KT + c) * p.nqp + i0 + ty * 4) = d4;
+        *reinterpret_cast<float4*>(ds + (j0 % 64 + tx * KT + c) * 8) = d4;
       }
       __syncthreads();
 #pragma unroll 2
@@ -430,7 +431,7 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_dq_kernel(const X
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   const int n = key_count(p, b);
   const float* K = reinterpret_cast<const float*>(p.k.p) + b * p.k.s[0] + kh * p.k.s[1];
-  const float* S = reinterpret_cast<const float*>(p.ds) + (long long)ul * p.nkp * p.nqp + i0;
+  const float* S = reinterpret_cast<const float*>(p.ds) + (long long)ul * p.nkp * p.nqp;
   float acc[4][DP / 16];
 #pragma unroll
   for (int r = 0; r < 4; ++r)
@@ -442,7 +443,8 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_dq_kernel(const X
     for (int x = threadIdx.x; x < C::BK * C::BQ / 4; x += kSimtThreads) {
       const int r = x / (C::BQ / 4), c = (x % (C::BQ / 4)) * 4;
       *reinterpret_cast<float4*>(ds + r * C::BQ + c) =
-          j0 + r < n ? *reinterpret_cast<const float4*>(S + (long long)(j0 + r) * p.nqp + c)
+          j0 + r < n ? *reinterpret_cast<const float4*>(
+                           S + ((long long)((j0 + r) / 64) * (p.nqp / 8) + (i0 + c) / 8) * 512 + (j0 + r) % 64 * 8 + c % 8)
                      : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     __syncthreads();

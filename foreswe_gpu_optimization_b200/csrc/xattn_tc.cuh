@@ -15,7 +15,7 @@ namespace xa {
 extern __shared__ __align__(1024) uint8_t xsmem[];
 
 struct XMaps {
-  CUtensorMap q, k, v, dout, ds;
+  CUtensorMap q, k, v, dout, o, dq, dk, dv;
 };
 
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const WaitCtx& ctx) {
@@ -79,6 +79,13 @@ __device__ __forceinline__ void load_rows(uint8_t* dst, const CUtensorMap* map, 
   for (int kb = 0; kb < DP / 64; ++kb) tma_load_4d(dst + kb * region, map, bar, kb * 64, row, h, b);
 }
 
+// Descriptor of an operand without swizzle, M or N contiguous: 8 x 8 matrices of 8 rows (along K) x 16 bytes, `lbo`
+// bytes apart along K and `sbo` along M or N.
+__device__ __forceinline__ uint64_t smem_desc_plain(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)((lbo >> 4) & 0x3FFF) << 16 |
+         (uint64_t)((sbo >> 4) & 0x3FFF) << 32 | (uint64_t)1 << 46;
+}
+
 // acc[128 x 64] = A[128 x DP] B[64 x DP]^T, both K-major: the score-shaped product.
 template <int DP>
 __device__ __forceinline__ void mma_scores(uint32_t acc, uint32_t a, uint32_t b) {
@@ -128,6 +135,23 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* dst, const float (&v)[N
     }
   }
 }
+// 32 columns d0 .. d0 + 31 of row r, in bf16, into a 128-row tile for a TMA store (regions of 64 columns).
+__device__ __forceinline__ void stage_row32(uint8_t* tile, int r, int d0, const float (&v)[32], float f) {
+  uint8_t* dst = tile + (d0 / 64) * (128 * 128) + (r >> 3) * 1024 + (r & 7) * 128;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    *reinterpret_cast<uint4*>(dst + ((((d0 % 64) / 8 + c) ^ (r & 7)) << 4)) =
+        make_uint4(pack_bf16(v[8 * c] * f, v[8 * c + 1] * f), pack_bf16(v[8 * c + 2] * f, v[8 * c + 3] * f),
+                   pack_bf16(v[8 * c + 4] * f, v[8 * c + 5] * f), pack_bf16(v[8 * c + 6] * f, v[8 * c + 7] * f));
+}
+// The staged tile leaves (one thread, after a barrier of the threads that staged it and their proxy fence).
+template <int DP>
+__device__ __forceinline__ void store_tile(const CUtensorMap* map, const uint8_t* tile, int D, int row, int h, int b) {
+  for (int kb = 0; kb < DP / 64 && kb * 64 < D; ++kb)
+    tma_store_4d(map, tile + kb * (128 * 128), kb * 64, row, h, b);
+  bulk_commit();
+}
+
 __device__ __forceinline__ bool vec_rows(const XTensor& t) {
   return ((reinterpret_cast<uintptr_t>(t.p) | (uintptr_t)(t.s[0] * 2) | (uintptr_t)(t.s[1] * 2) |
            (uintptr_t)(t.s[2] * 2)) & 15) == 0;
@@ -259,22 +283,21 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
     const int bh = b * p.H + h;
     const AttnDrop drop = attn_drop(p.rng, DROP ? p.drop_thr : 0, p.drop_scale);
     const uint32_t thr2 = drop.pair();
-    const uint8_t* idrow = BIAS ? p.ids + (long long)(row ? i : 0) * p.ids_ld : nullptr;
+    const uint2* idrow = BIAS ? reinterpret_cast<const uint2*>(p.ids) + (long long)(i / 64) * (p.nkp / 8) * 64 + i % 64
+                              : nullptr;
     float* xrow = reinterpret_cast<float*>(xsmem + C::OFF_ROW);
     const uint64_t sc2 = f2(p.scale_log2, p.scale_log2);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     // this thread's 32 ids and this lane's key of the next chunk, fetched a chunk ahead
-    uint4 id4[2];
+    uint2 id8[4];
     bool live_next = false;
     auto fetch = [&](int c) {
       const int j0 = (c0 + c) * 64 + wg * 32;
       live_next = key_live(p, b, j0 + lane, n);
-      if (BIAS) {  // 16 ids per load; keys past Nk are excluded
+      if (BIAS && i < p.nqp) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-          id4[x] = j0 + x * 16 < p.Nk ? __ldg(reinterpret_cast<const uint4*>(idrow + j0) + x)
-                                      : make_uint4(~0u, ~0u, ~0u, ~0u);
+        for (int x = 0; x < 4; ++x) id8[x] = __ldg(idrow + (long long)(j0 / 8 + x) * 64);
       }
     };
     if (nc > 0) fetch(0);
@@ -295,7 +318,7 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
           float a = __uint_as_float(s[2 * e]), d = __uint_as_float(s[2 * e + 1]);
           x[e] = f2(a, d);
           if (BIAS) {
-            const uint32_t w = reinterpret_cast<const uint32_t*>(id4)[e / 2] >> (16 * (e & 1));
+            const uint32_t w = reinterpret_cast<const uint32_t*>(id8)[e / 2] >> (16 * (e & 1));
             x[e] = fma2(x[e], sc2, f2(tab[w & 255], tab[(w >> 8) & 255]));
           }
         }
@@ -396,18 +419,20 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
     const long long stat = (long long)bh * p.Nq + i;
     const long long part = (long long)split * p.B * p.H * p.Nq + stat;
     const float f = l == 0.f ? 0.f : (DROP ? p.drop_scale : 1.f) / l;
-    const bool vec = vec_rows(p.o);
+    const bool vec = vec_rows(p.o), tma = p.splits == 1 && p.out_tma;
     if (ok && any_row) {
 #pragma unroll 1
       for (int d = wg * (DP / 2); d < (wg + 1) * (DP / 2); d += 32) {
         float o[32];
         if (nc > 0) tmem_ld32(lanes + C::TM_O + d, o);
-        if (!row || d >= p.D) continue;
+        if (!tma && (!row || d >= p.D)) continue;
         if (l == 0.f) {  // a row with nothing left (or no chunk at all)
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0.f;
         }
-        if (p.splits > 1) {
+        if (tma) {  // Q's tile is free: every product has completed
+          stage_row32(xsmem, r, d, o, f);
+        } else if (p.splits > 1) {
           float* dst = p.part_o + part * p.D + d;
 #pragma unroll
           for (int e = 0; e < 32; ++e)
@@ -427,6 +452,15 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
         }
       }
     }
+    if (tma) {
+      fence_proxy_async_smem();
+      named_sync(2, C::EWT);
+      if (threadIdx.x == 0 && ok) {
+        if (pack) store_tile<DP>(&maps.o, xsmem, p.D, 0, kh * p.G, b);
+        else store_tile<DP>(&maps.o, xsmem, p.D, qt * 128, hx, b);
+        bulk_wait_read0();
+      }
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -435,47 +469,66 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
 
 // ---------------------------------------------------------------------------------------------------------------
 // Backward, row records: chunks of 64 query rows, rec[b*h][chunk][3][64] floats:
-//   without the bias  -(m + log2 l), unused, delta        with it  -m, 1 / l, delta (the bias may dwarf log2 l)
-// so that P = 2^(t + rec0) or 2^(t + rec0) rec1; rows past Nq and rows with nothing left get P = 0. One warp per row.
+//   without the bias  -(m + log2 l), unused, -delta       with it  -m, 1 / l, -delta (the bias may dwarf log2 l)
+// so that P = 2^(t + rec0) or 2^(t + rec0) rec1; rows past Nq and rows with nothing left get P = 0. Bound by reading o
+// and dO once: rows are taken in the order they lie in memory, with 8 loads of 16 bytes in flight per lane.
 // ---------------------------------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) xattn_records_kernel(const XParams p) {
-  const int per = p.nqp;
-  const long long x = (long long)blockIdx.x * 8 + threadIdx.x / 32;
-  const int lane = threadIdx.x % 32;
-  if (x >= (long long)p.B * p.H * per) return;
-  const int i = (int)(x % per), bh = (int)(x / per), h = bh % p.H, b = bh / p.H;
-  float d = 0.f;
-  if (i < p.Nq) {
-    const __nv_bfloat16* O =
-        reinterpret_cast<const __nv_bfloat16*>(p.o.p) + b * p.o.s[0] + h * p.o.s[1] + (long long)i * p.o.s[2];
-    const __nv_bfloat16* G = reinterpret_cast<const __nv_bfloat16*>(p.dout.p) + b * p.dout.s[0] + h * p.dout.s[1] +
-                             (long long)i * p.dout.s[2];
-    if (vec_rows(p.o) && vec_rows(p.dout)) {
-      const int c = lane * 8;
-      if (c + 8 <= p.D) {
-        const uint4 a = *reinterpret_cast<const uint4*>(O + c), g = *reinterpret_cast<const uint4*>(G + c);
-        const __nv_bfloat162 *av = reinterpret_cast<const __nv_bfloat162*>(&a),
-                             *gv = reinterpret_cast<const __nv_bfloat162*>(&g);
+template <int LPR>  // lanes per row: 8 columns each
+__global__ void __launch_bounds__(256) xattn_records_kernel(const XParams p, int heads_first) {
+  constexpr int RPW = 32 / LPR, UNROLL = 4;  // rows per warp and step, steps in flight
+  const int lane = threadIdx.x % 32, sub = lane / LPR, c = (lane % LPR) * 8;
+  const long long total = (long long)p.B * p.H * p.nqp;
+  const long long x0 = ((long long)blockIdx.x * 8 + threadIdx.x / 32) * (RPW * UNROLL);
+  const bool vec = vec_rows(p.o) && vec_rows(p.dout);
+  uint4 a[UNROLL], g[UNROLL];
+  int ri[UNROLL], rbh[UNROLL];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 u = __bfloat1622float2(av[e]), v = __bfloat1622float2(gv[e]);
-          d = fmaf(u.x, v.x, fmaf(u.y, v.y, d));
-        }
-      } else {
-        for (int e = c; e < p.D; ++e) d = fmaf(to_f(O[e]), to_f(G[e]), d);
-      }
+  for (int u = 0; u < UNROLL; ++u) {
+    const long long x = x0 + u * RPW + sub;
+    a[u] = g[u] = make_uint4(0, 0, 0, 0);
+    ri[u] = -1;
+    if (x >= total) continue;
+    // rows in the order of memory: heads side by side in a row, or rows of one head
+    const int lo = heads_first ? p.H : p.nqp;
+    const long long hi = x / lo;
+    const int in = (int)(x % lo), h = heads_first ? in : (int)(hi % p.H), b = (int)(heads_first ? hi / p.nqp : hi / p.H);
+    const int i = heads_first ? (int)(hi % p.nqp) : in;
+    ri[u] = i;
+    rbh[u] = b * p.H + h;
+    if (i >= p.Nq || c >= p.D) continue;
+    const __nv_bfloat16* O =
+        reinterpret_cast<const __nv_bfloat16*>(p.o.p) + b * p.o.s[0] + h * p.o.s[1] + (long long)i * p.o.s[2] + c;
+    const __nv_bfloat16* G = reinterpret_cast<const __nv_bfloat16*>(p.dout.p) + b * p.dout.s[0] + h * p.dout.s[1] +
+                             (long long)i * p.dout.s[2] + c;
+    if (vec && c + 8 <= p.D) {
+      a[u] = *reinterpret_cast<const uint4*>(O);
+      g[u] = *reinterpret_cast<const uint4*>(G);
     } else {
-      for (int e = lane; e < p.D; e += 32) d = fmaf(to_f(O[e]), to_f(G[e]), d);
+      __nv_bfloat16 *av = reinterpret_cast<__nv_bfloat16*>(&a[u]), *gv = reinterpret_cast<__nv_bfloat16*>(&g[u]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c + e < p.D) av[e] = O[e], gv[e] = G[e];
     }
   }
 #pragma unroll
-  for (int w = 16; w; w /= 2) d += __shfl_xor_sync(0xffffffffu, d, w);
-  if (lane == 0) {
-    const float2 st = i < p.Nq ? p.stats[(long long)bh * p.Nq + i] : make_float2(0.f, 0.f);
-    float* rec = p.rec + ((long long)bh * (per / 64) + i / 64) * 192 + i % 64;
+  for (int u = 0; u < UNROLL; ++u) {
+    const __nv_bfloat162 *av = reinterpret_cast<const __nv_bfloat162*>(&a[u]),
+                         *gv = reinterpret_cast<const __nv_bfloat162*>(&g[u]);
+    float d = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 s = __bfloat1622float2(av[e]), t = __bfloat1622float2(gv[e]);
+      d = fmaf(s.x, t.x, fmaf(s.y, t.y, d));
+    }
+#pragma unroll
+    for (int w = LPR / 2; w; w /= 2) d += __shfl_xor_sync(0xffffffffu, d, w);
+    if (lane % LPR || ri[u] < 0) continue;
+    const int i = ri[u];
+    const float2 st = i < p.Nq ? p.stats[(long long)rbh[u] * p.Nq + i] : make_float2(0.f, 0.f);
+    float* rec = p.rec + ((long long)rbh[u] * (p.nqp / 64) + i / 64) * 192 + i % 64;
     rec[0] = p.ids ? -st.x : st.y == 0.f ? -INFINITY : log2f(st.y) - st.x;
     rec[64] = st.y;
-    rec[128] = d;
+    rec[128] = -d;
   }
 }
 
@@ -504,19 +557,26 @@ struct KeysCfg {
   static constexpr int THREADS = EW * 128 + 64, TMA_WARP = EW * 4, MMA_WARP = EW * 4 + 1;
 };
 
-// Keep bits of 32 queries (i0 ..) for this lane's key j0 + lane: bit q of the result.
-__device__ __forceinline__ uint32_t keep_column(const AttnDrop& drop, uint32_t i0, uint32_t j0, uint32_t bh) {
+// Keep bits of 32 queries (i0 ..) for this lane's key j0 + lane: query 8 c + 2 i + e at bit 15 - (4 c + i) + 16 e. A
+// lane makes the calls of queries 8 c + lane % 8 for keys 8 (lane / 8) ..; bit (c, i, e) there is key 2 i + e, and three
+// exchanges transpose the 8 x 8 bits of each octet of lanes.
+__device__ __forceinline__ uint32_t keep_column(const AttnDrop& drop, uint32_t thr2, uint32_t i0, uint32_t j0,
+                                                uint32_t bh) {
   const int lane = threadIdx.x & 31;
   uint32_t x = 0;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) x |= drop.keep8(i0 + 8 * c + (lane & 7), (j0 >> 3) + (lane >> 3), bh) << (8 * c);
+  for (int c = 0; c < 4; ++c) {
+    const uint4 u = drop.words(i0 + 8 * c + (lane & 7), (j0 >> 3) + (lane >> 3), bh);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int s = 1; s < 8; s *= 2) {
-    const uint32_t low = s == 1 ? 0x55555555u : s == 2 ? 0x33333333u : 0x0F0F0F0Fu;
-    const uint32_t y = __shfl_xor_sync(0xffffffffu, x, s);
-    x = lane & s ? (x & ~low) | ((y >> s) & low) : (x & low) | ((y << s) & ~low);
+    for (int i = 0; i < 4; ++i) x |= (keep_pair(w[i], thr2) >> (4 * c + i)) & (0x80008000u >> (4 * c + i));
   }
-  return x;
+  uint32_t y = __shfl_xor_sync(0xffffffffu, x, 1);
+  x = lane & 1 ? (x & 0xFFFF0000u) | (y >> 16) : (x & 0x0000FFFFu) | (y << 16);
+  y = __shfl_xor_sync(0xffffffffu, x, 2);
+  x = lane & 2 ? (x & 0x55555555u) | ((y << 1) & 0xAAAAAAAAu) : (x & 0xAAAAAAAAu) | ((y >> 1) & 0x55555555u);
+  y = __shfl_xor_sync(0xffffffffu, x, 4);
+  return lane & 4 ? (x & 0x33333333u) | ((y << 2) & 0xCCCCCCCCu) : (x & 0xCCCCCCCCu) | ((y >> 2) & 0x33333333u);
 }
 
 template <int DP, bool BIAS, bool DROP>
@@ -619,6 +679,17 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, KeysCfg<DP>::CTAS)
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const bool check_keys = p.kmask != nullptr || j0 + 128 > n, live = key_live(p, b, j, n);
     const AttnDrop drop = attn_drop(p.rng, DROP ? p.drop_thr : 0, p.drop_scale);
+    const uint32_t thr2 = drop.pair();
+    const uint64_t sc2 = f2(p.scale_log2, p.scale_log2), ds2 = f2(drop.scale, drop.scale);
+    const long long tile = ((long long)(j / 64) * (p.nqp / 8)) * 64 + j % 64;  // of ids and dS, in granules of 8
+    constexpr int IDS = 2 / C::EW * 4;
+    uint2 id8[IDS];
+    auto fetch = [&](int c) {  // a chunk ahead
+#pragma unroll
+      for (int x = 0; x < IDS; ++x)
+        id8[x] = __ldg(reinterpret_cast<const uint2*>(p.idsT) + tile + (long long)((c % nqc) * 8 + wg * 4 + x) * 64);
+    };
+    if (BIAS) fetch(0);
     bool ok = true;
     for (int c = 0; c < nc; ++c) {
       const int st = c % NST, g = c / nqc, i0 = (c % nqc) * 64, bh = b * p.H + kh * p.G + g;
@@ -627,63 +698,63 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, KeysCfg<DP>::CTAS)
         for (int t = threadIdx.x; t < 256; t += C::EW * 128) tab[t] = table_log2(p, kh * p.G + g, t);
         named_sync(1, C::EW * 128);
       }
-      uint4 id4[2 / C::EW * 2];
-      if (BIAS) {
-#pragma unroll
-        for (int x = 0; x < 2 / C::EW * 2; ++x)
-          id4[x] = __ldg(reinterpret_cast<const uint4*>(p.idsT + (long long)j * p.nqp + i0 + wg * 32) + x);
-      }
       const uint32_t sbuf = lanes + C::TM_S + (c % NB) * 128;
       // bar_s follows bar_full, so the records are there too; the wait on bar_full makes their copy visible here
       if (ok) ok = warp_wait(&bar_full[st], (c / NST) & 1, ctx) && warp_wait(&bar_s[c % NB], (c / NB) & 1, ctx);
       if (!ok) continue;  // given up: only the barrier above is still met
       tc_fence_after();
       const float* rec = reinterpret_cast<const float*>(xsmem + C::OFF_REC + st * C::REC_BYTES);
-      __nv_bfloat16* ds = reinterpret_cast<__nv_bfloat16*>(p.ds) + (long long)(ul * p.G + g) * p.nkp * p.nqp +
-                          (long long)j * p.nqp + i0;
+      uint4* ds = reinterpret_cast<uint4*>(p.ds) + (long long)(ul * p.G + g) * (p.nkp / 8) * p.nqp + tile +
+                  (long long)(i0 / 8) * 64;
 #pragma unroll
       for (int piece = wg; piece < 2; piece += C::EW) {
         uint32_t s[32], dp[32];
         tmem_ld32_issue(sbuf + piece * 32, s);
         tmem_ld32_issue(sbuf + 64 + piece * 32, dp);
         uint32_t keep = 0;
-        if (DROP) keep = keep_column(drop, i0 + piece * 32, j0 + (warp & 3) * 32, bh);
+        if (DROP) keep = keep_column(drop, thr2, i0 + piece * 32, j0 + (warp & 3) * 32, bh);
         tmem_wait32(s);
         tmem_pin32(dp);
         uint32_t wp[16], wd[16];
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const float4 r0 = *reinterpret_cast<const float4*>(rec + piece * 32 + e);
-          const float4 r2 = *reinterpret_cast<const float4*>(rec + 128 + piece * 32 + e);
-          const float a0[4] = {r0.x, r0.y, r0.z, r0.w}, dl[4] = {r2.x, r2.y, r2.z, r2.w};
-          float a1[4] = {1.f, 1.f, 1.f, 1.f};
-          if (BIAS) {
-            const float4 r1 = *reinterpret_cast<const float4*>(rec + 64 + piece * 32 + e);
-            a1[0] = r1.x, a1[1] = r1.y, a1[2] = r1.z, a1[3] = r1.w;
-          }
-          float pv[4], dv[4];
+        for (int e = 0; e < 16; e += 2) {  // two pairs of queries
+          const ulonglong2 r0 = *reinterpret_cast<const ulonglong2*>(rec + piece * 32 + 2 * e);
+          const ulonglong2 r2 = *reinterpret_cast<const ulonglong2*>(rec + 128 + piece * 32 + 2 * e);
+          const uint64_t a0[2] = {r0.x, r0.y}, nd[2] = {r2.x, r2.y};
+          ulonglong2 r1 = make_ulonglong2(0, 0);
+          if (BIAS) r1 = *reinterpret_cast<const ulonglong2*>(rec + 64 + piece * 32 + 2 * e);
+          const uint64_t a1[2] = {r1.x, r1.y};
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            float t = __uint_as_float(s[e + u]);
+          for (int u = 0; u < 2; ++u) {
+            const int q = e + u;  // queries 2 q, 2 q + 1 of the piece
+            uint64_t t = f2(__uint_as_float(s[2 * q]), __uint_as_float(s[2 * q + 1]));
             if (BIAS) {
-              const uint32_t* w = reinterpret_cast<const uint32_t*>(id4) + (piece / C::EW) * 8;
-              t = fmaf(t, p.scale_log2, tab[(w[e / 4] >> (8 * u)) & 255]);
-              t = xex2(t + a0[u]) * a1[u];
+              const uint32_t w = reinterpret_cast<const uint32_t*>(id8)[(piece / C::EW) * 8 + q / 2] >> (16 * (q & 1));
+              t = add2(fma2(t, sc2, f2(tab[w & 255], tab[(w >> 8) & 255])), a0[u]);
             } else {
-              t = xex2(fmaf(t, p.scale_log2, a0[u]));
+              t = fma2(t, sc2, a0[u]);
             }
-            const float da = __uint_as_float(dp[e + u]);
+            float x, y;
+            unf2(t, x, y);
+            x = xex2(x), y = xex2(y);
+            uint64_t pr = f2(x, y);
+            if (BIAS) {
+              pr = mul2(pr, a1[u]);
+              unf2(pr, x, y);
+            }
+            wp[q] = pack_bf16(x, y);
+            uint64_t da;
             if (DROP) {
-              const bool k = (keep >> (e + u)) & 1;
-              pv[u] = k ? t : 0.f;
-              dv[u] = t * (k ? fmaf(da, drop.scale, -dl[u]) : -dl[u]);
+              const uint32_t k = keep << ((q / 4) * 4 + q % 4);
+              wp[q] &= spread_pair(k);
+              da = f2(__uint_as_float(dp[2 * q] & spread_one<0>(k)), __uint_as_float(dp[2 * q + 1] & spread_one<1>(k)));
+              da = fma2(da, ds2, nd[u]);
             } else {
-              pv[u] = t;
-              dv[u] = t * (da - dl[u]);
+              da = add2(f2(__uint_as_float(dp[2 * q]), __uint_as_float(dp[2 * q + 1])), nd[u]);
             }
+            unf2(mul2(pr, da), x, y);
+            wd[q] = pack_bf16(x, y);
           }
-          wp[e / 2] = pack_bf16(pv[0], pv[1]), wp[e / 2 + 1] = pack_bf16(pv[2], pv[3]);
-          wd[e / 2] = pack_bf16(dv[0], dv[1]), wd[e / 2 + 1] = pack_bf16(dv[2], dv[3]);
         }
         if (check_keys) {  // an absent key's row is 0 whatever K and V hold there
 #pragma unroll
@@ -693,25 +764,35 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, KeysCfg<DP>::CTAS)
         tmem_st16(sbuf + 64 + piece * 32, wd);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          reinterpret_cast<uint4*>(ds + piece * 32)[e] = make_uint4(wd[4 * e], wd[4 * e + 1], wd[4 * e + 2], wd[4 * e + 3]);
+          ds[(piece * 4 + e) * 64] = make_uint4(wd[4 * e], wd[4 * e + 1], wd[4 * e + 2], wd[4 * e + 3]);
       }
+      if (BIAS && c + 1 < nc) fetch(c + 1);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&bar_p[c % NB]);
     }
     if (ok) ok = warp_wait(&bar_done, 0, ctx);
     tc_fence_after();
-    const bool vk = vec_rows(p.dk), vv = vec_rows(p.dv);
+    const bool vk = vec_rows(p.dk), vv = vec_rows(p.dv), tk = p.out_tma & 2, tv = p.out_tma & 4;
     const float fv = DROP ? p.drop_scale : 1.f;
-    if (ok) {
+    if (ok) {  // K's and V's tiles are free: every product has completed
 #pragma unroll 1
       for (int d = wg * 32; d < DP; d += C::EW * 32) {
         float x[32];
         tmem_ld32(lanes + C::TM_DK + d, x);
-        if (j < p.Nk && d < p.D) store_row(dK + (long long)j * p.dk.s[2] + d, x, p.scale, p.D - d, vk);
+        if (tk) stage_row32(xsmem, r, d, x, p.scale);
+        else if (j < p.Nk && d < p.D) store_row(dK + (long long)j * p.dk.s[2] + d, x, p.scale, p.D - d, vk);
         tmem_ld32(lanes + C::TM_DV + d, x);
-        if (j < p.Nk && d < p.D) store_row(dV + (long long)j * p.dv.s[2] + d, x, fv, p.D - d, vv);
+        if (tv) stage_row32(xsmem + C::OFF_V, r, d, x, fv);
+        else if (j < p.Nk && d < p.D) store_row(dV + (long long)j * p.dv.s[2] + d, x, fv, p.D - d, vv);
       }
+    }
+    fence_proxy_async_smem();
+    named_sync(1, C::EW * 128);
+    if (threadIdx.x == 0 && ok) {
+      if (tk) store_tile<DP>(&maps.dk, xsmem, p.D, j0, kh, b);
+      if (tv) store_tile<DP>(&maps.dv, xsmem + C::OFF_V, p.D, j0, kh, b);
+      bulk_wait_read0();
     }
   }
   tc_fence_before();
@@ -720,15 +801,17 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, KeysCfg<DP>::CTAS)
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// dQ = scale dS K from the dS^T scratch: one CTA per (128 queries, head of the launch's units), over 64-key chunks;
-// dS^T is read as an A operand with queries contiguous. Bound by reading the scratch. Two of the epilogue's warps clear
-// the rows of absent keys first (0 * NaN).
+// dQ = scale dS K from the dS scratch: one CTA per (128 queries, head of the launch's units), over 64-key chunks. The
+// scratch's granules of 8 queries x 64 keys are the tensor core's unswizzled tiles with M contiguous (8 x 8 matrices of
+// 128 bytes, 8 keys apart by 128 and 8 queries apart by 1024), so a chunk's A operand is one contiguous copy of 16 KB.
+// Bound by reading the scratch. Two of the epilogue's warps clear the rows of absent keys first (0 * NaN).
 // ---------------------------------------------------------------------------------------------------------------
 template <int DP>
 struct DqCfg {
   static constexpr int NST = DP == 64 ? 4 : DP == 128 ? 3 : 2;
-  static constexpr int A_BYTES = 2 * 64 * 128, B_BYTES = DP / 64 * 64 * 128, STAGE = A_BYTES + B_BYTES;
+  static constexpr int A_BYTES = 16 * 1024, B_BYTES = DP / 64 * 64 * 128, STAGE = A_BYTES + B_BYTES;
   static constexpr int SMEM = NST * STAGE;
+  static_assert(SMEM >= DP / 64 * 128 * 128, "the epilogue's tile");
   static constexpr int TM_COLS = DP == 64 ? 64 : DP == 128 ? 128 : 256;
   static constexpr int THREADS = 192, TMA_WARP = 4, MMA_WARP = 5;
 };
@@ -766,13 +849,15 @@ __global__ void __launch_bounds__(192, 2) xattn_bwd_dq_kernel(const __grid_const
 
   if (warp == C::TMA_WARP) {
     if (lane == 0) {
+      // 16 granules of 8 queries, 8 in a last tile of 64 rows (what its other rows yield is not stored)
+      const int bytes = (p.nqp - qt * 128 < 128 ? 8 : 16) * 1024;
+      const uint4* ds = reinterpret_cast<const uint4*>(p.ds) + (long long)ul * (p.nkp / 8) * p.nqp + (long long)qt * 16 * 64;
       for (int c = 0; c < nc; ++c) {
         const int st = c % NST;
         if (!mbar_wait(&bar_empty[st], ((c / NST) & 1) ^ 1, ctx)) break;
         uint8_t* dst = xsmem + st * C::STAGE;
-        mbar_arrive_expect_tx(&bar_full[st], C::STAGE);
-        tma_load_3d(dst, &maps.ds, &bar_full[st], qt * 128, c * 64, ul);
-        tma_load_3d(dst + 64 * 128, &maps.ds, &bar_full[st], qt * 128 + 64, c * 64, ul);
+        mbar_arrive_expect_tx(&bar_full[st], bytes + C::B_BYTES);
+        bulk_load(dst, ds + (long long)c * (p.nqp / 8) * 64, bytes, &bar_full[st]);
         load_rows<DP>(dst + C::A_BYTES, &maps.k, &bar_full[st], 64 * 128, c * 64, kh, b);
       }
     }
@@ -788,7 +873,7 @@ __global__ void __launch_bounds__(192, 2) xattn_bwd_dq_kernel(const __grid_const
         const uint32_t a = sbase + st * C::STAGE, k = a + C::A_BYTES;
 #pragma unroll
         for (int s = 0; s < 4; ++s)
-          mma_ss<Kind::kF16>(tmem, smem_desc_sw128(a + s * 16 * 128, 64 * 128, 1024),
+          mma_ss<Kind::kF16>(tmem, smem_desc_plain(a + s * 2 * 128, 128, 1024),
                              smem_desc_sw128(k + s * 16 * 128, 64 * 128, 1024), idesc, c + s > 0);
         mma_commit(&bar_empty[st]);
       }
@@ -812,7 +897,7 @@ __global__ void __launch_bounds__(192, 2) xattn_bwd_dq_kernel(const __grid_const
     tc_fence_after();
     const int i = qt * 128 + warp * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-    const bool vec = vec_rows(p.dq);
+    const bool vec = vec_rows(p.dq), tma = p.out_tma & 1;
     __nv_bfloat16* dQ = reinterpret_cast<__nv_bfloat16*>(p.dq.p) + b * p.dq.s[0] + h * p.dq.s[1];
     if (ok) {
 #pragma unroll 1
@@ -824,7 +909,16 @@ __global__ void __launch_bounds__(192, 2) xattn_bwd_dq_kernel(const __grid_const
 #pragma unroll
           for (int e = 0; e < 32; ++e) x[e] = 0.f;
         }
-        if (i < p.Nq && d < p.D) store_row(dQ + (long long)i * p.dq.s[2] + d, x, p.scale, p.D - d, vec);
+        if (tma) stage_row32(xsmem, warp * 32 + lane, d, x, p.scale);
+        else if (i < p.Nq && d < p.D) store_row(dQ + (long long)i * p.dq.s[2] + d, x, p.scale, p.D - d, vec);
+      }
+    }
+    if (tma) {
+      fence_proxy_async_smem();
+      named_sync(1, 128);
+      if (threadIdx.x == 0 && ok) {
+        store_tile<DP>(&maps.dq, xsmem, p.D, qt * 128, h, b);
+        bulk_wait_read0();
       }
     }
   }
