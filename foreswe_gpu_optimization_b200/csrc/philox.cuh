@@ -83,8 +83,11 @@ __device__ __forceinline__ AttnDrop attn_drop(const long long* rng, int thr, flo
   AttnDrop d{{0, 0}, 0, (uint32_t)thr, scale};
   if (thr > 0) {
     const unsigned long long seed = (unsigned long long)rng[0], off = (unsigned long long)rng[1];
-    d.key = {(uint32_t)seed, (uint32_t)(seed >> 32) ^ (uint32_t)(off >> 32)};
-    d.off = (uint32_t)off;
+    // the same in every lane; a warp-wide reduction puts the words into uniform registers, where the rounds' keys cost
+    // the vector units nothing
+    d.key = {__reduce_or_sync(0xffffffffu, (uint32_t)seed),
+             __reduce_or_sync(0xffffffffu, (uint32_t)(seed >> 32) ^ (uint32_t)(off >> 32))};
+    d.off = __reduce_or_sync(0xffffffffu, (uint32_t)off);
   }
   return d;
 }

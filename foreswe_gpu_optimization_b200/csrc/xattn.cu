@@ -55,6 +55,7 @@ int check_xshape(const GeoXattnShape* s, XDims& d) {
   if (d.Nq > (1 << 30) || d.Nk > (1 << 30) || (long long)d.B * d.H > (1 << 30)) return GEOATTN_ERR_UNSUPPORTED;
   d.nqp = (d.Nq + 63) / 64 * 64;
   d.nkp = (d.Nk + 127) / 128 * 128;
+  if (d.B > 65535 || (long long)d.H * d.nqp >= (1ll << 31)) return GEOATTN_ERR_UNSUPPORTED;  // grid of the row records
   if (d.T && (d.nqp / 64 > 65535 || d.nkp / 64 > 65535)) return GEOATTN_ERR_UNSUPPORTED;  // grid of the ids' tiles
   d.splits = forward_splits(d);
   const long long qt = (d.Nq + 63) / 64, kt = (d.Nk + 31) / 32;
@@ -73,7 +74,7 @@ int check_xshape(const GeoXattnShape* s, XDims& d) {
 struct XFwdWs {
   int* status;
   float *part_o, *part_ml;
-  uint8_t* ids;
+  uint16_t* ids;
 };
 size_t xfwd_ws(const XDims& d, uint8_t* base, XFwdWs* w) {
   size_t off = 0;
@@ -89,7 +90,7 @@ size_t xfwd_ws(const XDims& d, uint8_t* base, XFwdWs* w) {
     t.part_o = reinterpret_cast<float*>(take(rows * d.D * 4));
     t.part_ml = reinterpret_cast<float*>(take(rows * 2 * 4));
   }
-  if (d.T && d.bf16) t.ids = take((size_t)d.nqp * d.nkp);
+  if (d.T && d.bf16) t.ids = reinterpret_cast<uint16_t*>(take((size_t)d.nqp * d.nkp * 2));
   if (w) *w = t;
   return off;
 }
@@ -98,7 +99,7 @@ struct XBwdWs {
   int* status;
   float *delta, *rec;
   void* ds;
-  uint8_t* idsT;
+  uint16_t* idsT;
   float* part;
 };
 size_t xbwd_ws(const XDims& d, uint8_t* base, XBwdWs* w) {
@@ -114,7 +115,7 @@ size_t xbwd_ws(const XDims& d, uint8_t* base, XBwdWs* w) {
   else t.delta = reinterpret_cast<float*>(take((size_t)d.B * d.H * d.Nq * 4));
   t.ds = take(d.ds_unit * d.units_per_launch);
   if (d.T) {
-    t.idsT = take((size_t)d.nkp * d.nqp);
+    t.idsT = reinterpret_cast<uint16_t*>(take((size_t)d.nkp * d.nqp * 2));
     t.part = reinterpret_cast<float*>(take((size_t)d.launches * d.H * d.chunks * d.T * 4));
   }
   if (w) *w = t;
@@ -231,7 +232,7 @@ void out_map(CUtensorMap* m, int* flags, int bit, const XTensor& t, int D, int n
   if (xmap(m, t, D, n, heads, batch, rows, box_heads) == GEOATTN_OK) *flags |= bit;
 }
 
-int forward_tc(XParams& p, const XDims& d, uint8_t* ids, cudaStream_t st) {
+int forward_tc(XParams& p, const XDims& d, uint16_t* ids, cudaStream_t st) {
   xa::XMaps maps;
   std::memset(&maps, 0, sizeof(maps));
   p.pack = packs_rows(d);
@@ -242,8 +243,8 @@ int forward_tc(XParams& p, const XDims& d, uint8_t* ids, cudaStream_t st) {
   if (p.pack) out_map(&maps.o, &p.out_tma, 1, p.o, d.D, d.Nq, d.H, d.B, d.Nq, d.G);
   else out_map(&maps.o, &p.out_tma, 1, p.o, d.D, d.Nq, d.H, d.B);
   if (d.T) {
-    ids_tile_kernel<false><<<dim3(d.nkp / 64, d.nqp / 64), 256, 0, st>>>(p.ids, p.ids_ld, d.Nq, d.Nk, d.nkp, ids);
-    p.ids = ids;
+    ids_tile_kernel<false><<<dim3(d.nkp / 64, d.nqp / 64), 256, 0, st>>>(p.ids, p.ids_ld, d.Nq, d.Nk, d.nkp, d.T, ids);
+    p.idsQ = ids;
     if ((rc = status_of(cudaGetLastError()))) return rc;
   }
   const long long grid = (long long)d.splits * d.B * (p.pack ? d.Hkv : (long long)((d.Nq + 127) / 128) * d.H);
@@ -264,8 +265,8 @@ int backward_maps(xa::XMaps& maps, XParams& p, const XDims& d) {
 
 int records(const XParams& p, const XDims& d, cudaStream_t st) {
   // 16 bytes per lane, a row per 8, 16 or 32 lanes, 4 rows per lane in flight
-  const long long rows = (long long)d.B * d.H * d.nqp, per = 8 * 4 * (d.DP == 64 ? 4 : d.DP == 128 ? 2 : 1);
-  const unsigned grid = (unsigned)((rows + per - 1) / per);
+  const long long rows = (long long)d.H * d.nqp, per = 8 * 4 * (d.DP == 64 ? 4 : d.DP == 128 ? 2 : 1);
+  const dim3 grid((unsigned)((rows + per - 1) / per), d.B);
   const int heads_first = p.o.s[1] < p.o.s[2];
   if (d.DP == 64) xa::xattn_records_kernel<8><<<grid, 256, 0, st>>>(p, heads_first);
   else if (d.DP == 128) xa::xattn_records_kernel<16><<<grid, 256, 0, st>>>(p, heads_first);
@@ -365,7 +366,7 @@ int geoattn_xattn_bwd(const GeoXattnBwdArgs* a, void* stream) {
               : xlaunch(xattn_delta_kernel, ((long long)d.B * d.H * d.Nq + 7) / 8, 256, 0, st, p);
   if (rc) return rc;
   if (d.T) {
-    ids_tile_kernel<true><<<dim3(d.nqp / 64, d.nkp / 64), 256, 0, st>>>(p.ids, p.ids_ld, d.Nq, d.Nk, d.nqp, ws.idsT);
+    ids_tile_kernel<true><<<dim3(d.nqp / 64, d.nkp / 64), 256, 0, st>>>(p.ids, p.ids_ld, d.Nq, d.Nk, d.nqp, d.T, ws.idsT);
     if ((rc = status_of(cudaGetLastError()))) return rc;
   }
   const int units = d.B * d.Hkv;

@@ -29,12 +29,14 @@ __global__ void __launch_bounds__(256) distance_buckets_kernel(int nq, const dou
   ids[x] = km > max_km ? (uint8_t)kNoPair : (uint8_t)n;
 }
 
-// Tiled copy of the bucket ids, out[row / 64][col / 8][row % 64][8], padded with kNoPair to [rows_p][cols_p]: a warp
-// whose lanes are consecutive rows reads 8 columns as one contiguous block (row-major rows cost a cache line per lane).
-// TRANS: rows are the keys and columns the queries (backward), else the other way round. A 64 x 64 tile per CTA.
+// Tiled copy of the bucket ids for the tensor-core kernels, out[row / 64][col / 8][row % 64][8], rows and columns padded:
+// a warp whose lanes are consecutive rows reads 8 columns as one contiguous block (row-major rows cost a cache line per
+// lane). An entry is the byte offset of its bucket in a table of T fp32 values and -inf behind them (kNoPairOffset for
+// ids that exclude their pair), so that a kernel spends one instruction per id. TRANS: rows are the keys and columns the
+// queries (backward), else the other way round. A 64 x 64 tile per CTA.
 template <bool TRANS>
 __global__ void __launch_bounds__(256) ids_tile_kernel(const uint8_t* __restrict__ ids, long long ld, int nq, int nk,
-                                                       int cols_p, uint8_t* __restrict__ out) {
+                                                       int cols_p, int T, uint16_t* __restrict__ out) {
   __shared__ uint8_t tile[64][68];  // [query][key]
   const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
   const int i0 = TRANS ? c0 : r0, j0 = TRANS ? r0 : c0;
@@ -43,20 +45,21 @@ __global__ void __launch_bounds__(256) ids_tile_kernel(const uint8_t* __restrict
     tile[i][j] = i0 + i < nq && j0 + j < nk ? ids[(long long)(i0 + i) * ld + j0 + j] : (uint8_t)kNoPair;
   }
   __syncthreads();
-  uint2* dst = reinterpret_cast<uint2*>(out) + ((long long)blockIdx.y * (cols_p / 8) + c0 / 8) * 64;
+  uint4* dst = reinterpret_cast<uint4*>(out) + ((long long)blockIdx.y * (cols_p / 8) + c0 / 8) * 64;
   for (int x = threadIdx.x; x < 64 * 8; x += 256) {
     const int r = x % 64, g = x / 64;
-    uint32_t w[2];
+    uint32_t w[4];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      w[k] = 0;
+    for (int k = 0; k < 4; ++k) {
+      uint32_t o[2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int c = g * 8 + k * 4 + e;
-        w[k] |= (uint32_t)(TRANS ? tile[c][r] : tile[r][c]) << (8 * e);
+      for (int e = 0; e < 2; ++e) {
+        const int c = g * 8 + k * 2 + e, id = TRANS ? tile[c][r] : tile[r][c];
+        o[e] = id < T ? 4 * id : kNoPairOffset;
       }
+      w[k] = o[0] | o[1] << 16;
     }
-    dst[(long long)g * 64 + r] = make_uint2(w[0], w[1]);
+    dst[(long long)g * 64 + r] = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -100,8 +103,8 @@ __global__ void __launch_bounds__(256) table_grad_kernel(const XParams p, int un
     }
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const int t = p.idsT[at + e];
-      if (t < p.T) hist[t * 256 + threadIdx.x] += sum[e];
+      const int o = p.idsT[at + e];  // 4 * bucket
+      if (o != kNoPairOffset) hist[o * 64 + threadIdx.x] += sum[e];
     }
   }
   __syncthreads();

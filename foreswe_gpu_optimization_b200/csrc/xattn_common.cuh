@@ -26,9 +26,10 @@ struct XTensor {
 struct XParams {
   int B, H, Hkv, G, Nq, Nk, D, T;
   XTensor q, k, v, o, dout, dq, dk, dv;
-  const uint8_t* ids;       // [Nq][ids_ld] or null; bf16 forward: tiled, rows = queries, columns padded to nkp
+  const uint8_t* ids;       // [Nq][ids_ld] or null
   long long ids_ld;
-  const uint8_t* idsT;      // tiled, rows = keys (nkp), columns = queries (nqp) (backward)
+  const uint16_t* idsQ;     // tiled offsets (ids_tile_kernel): rows = queries (nqp), columns = keys (nkp) (bf16 forward)
+  const uint16_t* idsT;     // rows = keys (nkp), columns = queries (nqp) (backward)
   const void* table;        // [H][T], bf16 or fp32
   int table_bf16;
   const int* lens;          // [B] or null
@@ -54,6 +55,7 @@ struct XParams {
 };
 
 constexpr int kNoPair = 255;
+constexpr int kNoPairOffset = 4 * kMaxBuckets;  // byte offset behind the largest table: holds -inf
 
 // Keys of batch b that exist: [0, n) before the key mask.
 __device__ __forceinline__ int key_count(const XParams& p, int b) {

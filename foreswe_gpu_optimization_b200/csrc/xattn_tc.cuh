@@ -71,6 +71,12 @@ __device__ __forceinline__ bool named_any(int id, int threads, bool yes) {
   return r != 0;
 }
 
+// The bias of the two pairs whose byte offsets `w` holds, from the table at `off` in shared memory.
+__device__ __forceinline__ uint64_t table_pair(int off, uint32_t w) {
+  return f2(*reinterpret_cast<const float*>(xsmem + off + (w & 0xFFFF)),
+            *reinterpret_cast<const float*>(xsmem + off + (w >> 16)));
+}
+
 // NKB regions of `rows` x 128 bytes.
 template <int DP>
 __device__ __forceinline__ void load_rows(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int region, int row,
@@ -86,26 +92,28 @@ __device__ __forceinline__ uint64_t smem_desc_plain(uint32_t saddr, uint32_t lbo
          (uint64_t)((sbo >> 4) & 0x3FFF) << 32 | (uint64_t)1 << 46;
 }
 
-// acc[128 x 64] = A[128 x DP] B[64 x DP]^T, both K-major: the score-shaped product.
-template <int DP>
+// acc[128 x N] = A[128 x DP] B[N x DP]^T, both K-major: the score-shaped product. An instruction reads its operands from
+// shared memory at 128 bytes per clock (A 4 KB, B 32 N bytes for K = 16), so N = 64 takes 48 clocks and N = 128 takes 64.
+template <int DP, int N>
 __device__ __forceinline__ void mma_scores(uint32_t acc, uint32_t a, uint32_t b) {
-  constexpr uint32_t idesc = instr_desc(1, 0, 0, 128, 64);
+  constexpr uint32_t idesc = instr_desc(1, 0, 0, 128, N);
 #pragma unroll
   for (int kb = 0; kb < DP / 64; ++kb)
 #pragma unroll
     for (int s = 0; s < 4; ++s)
       mma_ss<Kind::kF16>(acc, smem_desc_sw128(a + kb * (128 * 128) + s * 32, 16, 1024),
-                         smem_desc_sw128(b + kb * (64 * 128) + s * 32, 16, 1024), idesc, kb + s > 0);
+                         smem_desc_sw128(b + kb * (N * 128) + s * 32, 16, 1024), idesc, kb + s > 0);
 }
 
-// acc[128 x DP] (+)= A[128 x 64] B[64 x DP]: A in tensor memory (two bf16 per column), each 32-wide piece at the start
-// of the 32 score columns that it replaces (another warpgroup may still read its own); B with its rows along K.
-template <int DP>
+// acc[128 x DP] (+)= A[128 x K] B[K x DP]: A in tensor memory (two bf16 per column), each piece of PIECE (16 or 32)
+// columns at the start of the score columns that it replaces (another warpgroup may still read its own); B with its rows
+// along K.
+template <int DP, int K, int PIECE>
 __device__ __forceinline__ void mma_pieces(uint32_t acc, uint32_t a, uint32_t b, bool accumulate) {
   constexpr uint32_t idesc = instr_desc(1, 0, 1, 128, DP);
 #pragma unroll
-  for (int s = 0; s < 4; ++s)
-    mma_ts<Kind::kF16>(acc, a + (s / 2) * 32 + (s % 2) * 8, smem_desc_sw128(b + s * 16 * 128, 64 * 128, 1024), idesc,
+  for (int s = 0; s < K / 16; ++s)
+    mma_ts<Kind::kF16>(acc, a + (s * 16 / PIECE) * PIECE + (s * 16 % PIECE) / 2, smem_desc_sw128(b + s * 16 * 128, K * 128, 1024), idesc,
                        accumulate || s > 0);
 }
 
@@ -174,7 +182,7 @@ struct FwdCfg {
   static constexpr int NKV = DP == 192 ? 1 : DP == 128 ? 2 : 4;  // chunks of K, and of V, in flight
   static constexpr int Q_BYTES = DP / 64 * 128 * 128, KV_BYTES = DP / 64 * 64 * 128;
   static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + NKV * KV_BYTES, OFF_TAB = OFF_V + NKV * KV_BYTES;
-  static constexpr int OFF_ROW = OFF_TAB + 1024;                 // [2][128] floats: what the warpgroups exchange
+  static constexpr int OFF_ROW = OFF_TAB + 512;                  // [2][128] floats: what the warpgroups exchange
   static constexpr int SMEM = OFF_ROW + 1024;
   static constexpr int TM_S = 0, TM_O = NSB * 64, TM_COLS = 256;
   static constexpr int EWT = 256, THREADS = EWT + 64, TMA_WARP = 8, MMA_WARP = 9;
@@ -222,8 +230,8 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
     tmem_alloc(&tmem_sh, C::TM_COLS);
     tmem_relinquish();
   }
-  float* tab = reinterpret_cast<float*>(xsmem + C::OFF_TAB);
-  if (BIAS && threadIdx.x < 256) tab[threadIdx.x] = table_log2(p, hx, threadIdx.x);
+  if (BIAS && threadIdx.x <= kMaxBuckets)
+    reinterpret_cast<float*>(xsmem + C::OFF_TAB)[threadIdx.x] = table_log2(p, hx, threadIdx.x);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -256,7 +264,7 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
         const int st = c % NKV;
         if (!(ok = ok && mbar_wait(&bar_kfull[st], (c / NKV) & 1, ctx))) return;
         tc_fence_after();
-        mma_scores<DP>(tmem + C::TM_S + (c % NSB) * 64, sbase, sbase + C::OFF_K + st * C::KV_BYTES);
+        mma_scores<DP, 64>(tmem + C::TM_S + (c % NSB) * 64, sbase, sbase + C::OFF_K + st * C::KV_BYTES);
         mma_commit(&bar_s[c % NSB]);
         mma_commit(&bar_kempty[st]);
       };
@@ -267,7 +275,7 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
         if (!(ok = ok && mbar_wait(&bar_p[c % NSB], (c / NSB) & 1, ctx) && mbar_wait(&bar_vfull[st], (c / NKV) & 1, ctx)))
           break;
         tc_fence_after();
-        mma_pieces<DP>(tmem + C::TM_O, tmem + C::TM_S + (c % NSB) * 64, sbase + C::OFF_V + st * C::KV_BYTES, c > 0);
+        mma_pieces<DP, 64, 32>(tmem + C::TM_O, tmem + C::TM_S + (c % NSB) * 64, sbase + C::OFF_V + st * C::KV_BYTES, c > 0);
         mma_commit(&bar_vempty[st]);
         mma_commit(&bar_pv[c & 1]);
         if (NSB == 1 && c + 1 < nc) scores(c + 1);
@@ -283,21 +291,21 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
     const int bh = b * p.H + h;
     const AttnDrop drop = attn_drop(p.rng, DROP ? p.drop_thr : 0, p.drop_scale);
     const uint32_t thr2 = drop.pair();
-    const uint2* idrow = BIAS ? reinterpret_cast<const uint2*>(p.ids) + (long long)(i / 64) * (p.nkp / 8) * 64 + i % 64
-                              : nullptr;
+    // rows past nqp (in a last tile of 64) read the tile's other half
+    const uint4* idrow = reinterpret_cast<const uint4*>(p.idsQ) +
+                         ((long long)((i < p.nqp ? i : i - 64) / 64) * (p.nkp / 8) + c0 * 8 + wg * 4) * 64 + i % 64;
     float* xrow = reinterpret_cast<float*>(xsmem + C::OFF_ROW);
     const uint64_t sc2 = f2(p.scale_log2, p.scale_log2);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     // this thread's 32 ids and this lane's key of the next chunk, fetched a chunk ahead
-    uint2 id8[4];
-    bool live_next = false;
+    uint4 id[4];
+    bool live_next = true;
     auto fetch = [&](int c) {
-      const int j0 = (c0 + c) * 64 + wg * 32;
-      live_next = key_live(p, b, j0 + lane, n);
-      if (BIAS && i < p.nqp) {
+      if (p.kmask || (c0 + c + 1) * 64 > n) live_next = key_live(p, b, (c0 + c) * 64 + wg * 32 + lane, n);
+      if (BIAS) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) id8[x] = __ldg(idrow + (long long)(j0 / 8 + x) * 64);
+        for (int x = 0; x < 4; ++x) id[x] = __ldg(idrow + c * 512 + x * 64);
       }
     };
     if (nc > 0) fetch(0);
@@ -317,10 +325,7 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
         for (int e = 0; e < 16; ++e) {
           float a = __uint_as_float(s[2 * e]), d = __uint_as_float(s[2 * e + 1]);
           x[e] = f2(a, d);
-          if (BIAS) {
-            const uint32_t w = reinterpret_cast<const uint32_t*>(id8)[e / 2] >> (16 * (e & 1));
-            x[e] = fma2(x[e], sc2, f2(tab[w & 255], tab[(w >> 8) & 255]));
-          }
+          if (BIAS) x[e] = fma2(x[e], sc2, table_pair(C::OFF_TAB, reinterpret_cast<const uint32_t*>(id)[e]));
         }
         if (live != ~0u) {
 #pragma unroll
@@ -477,22 +482,21 @@ template <int LPR>  // lanes per row: 8 columns each
 __global__ void __launch_bounds__(256) xattn_records_kernel(const XParams p, int heads_first) {
   constexpr int RPW = 32 / LPR, UNROLL = 4;  // rows per warp and step, steps in flight
   const int lane = threadIdx.x % 32, sub = lane / LPR, c = (lane % LPR) * 8;
-  const long long total = (long long)p.B * p.H * p.nqp;
-  const long long x0 = ((long long)blockIdx.x * 8 + threadIdx.x / 32) * (RPW * UNROLL);
+  const uint32_t total = (uint32_t)p.H * p.nqp;  // rows of a batch entry (< 2^31)
+  const uint32_t x0 = (blockIdx.x * 8 + threadIdx.x / 32) * (RPW * UNROLL);
+  const int b = blockIdx.y;
   const bool vec = vec_rows(p.o) && vec_rows(p.dout);
   uint4 a[UNROLL], g[UNROLL];
   int ri[UNROLL], rbh[UNROLL];
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
-    const long long x = x0 + u * RPW + sub;
+    const uint32_t x = x0 + u * RPW + sub;
     a[u] = g[u] = make_uint4(0, 0, 0, 0);
     ri[u] = -1;
     if (x >= total) continue;
     // rows in the order of memory: heads side by side in a row, or rows of one head
-    const int lo = heads_first ? p.H : p.nqp;
-    const long long hi = x / lo;
-    const int in = (int)(x % lo), h = heads_first ? in : (int)(hi % p.H), b = (int)(heads_first ? hi / p.nqp : hi / p.H);
-    const int i = heads_first ? (int)(hi % p.nqp) : in;
+    const uint32_t lo = heads_first ? p.H : p.nqp, hi = x / lo, in = x - hi * lo;
+    const int h = heads_first ? in : hi, i = heads_first ? hi : in;
     ri[u] = i;
     rbh[u] = b * p.H + h;
     if (i >= p.Nq || c >= p.D) continue;
@@ -533,39 +537,42 @@ __global__ void __launch_bounds__(256) xattn_records_kernel(const XParams p, int
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Backward, key pass. One CTA per (128 keys, key head, batch); loops over chunks of 64 queries of the heads that share
+// Backward, key pass. One CTA per (128 keys, key head, batch); loops over chunks of BQ queries of the heads that share
 // the key head. Scores are formed transposed (keys in the lanes), so that P^T and dS^T are written over them in tensor
 // memory as the A operands of
 //   dV += P^T dO,  dK += dS^T Q
-// and a thread owns one key's 32 queries of a piece; dS^T also goes to the scratch for dQ and the table's gradient.
-//   MMA warp       S^T(c + 1), dP^T(c + 1), then dV, dK of chunk c
-//   EW warpgroups  P, dS of chunk c (piece w of 32 queries to warpgroup w mod EW)
-// DP = 64 fits two CTAs per SM (one score buffer each); DP = 128 takes the SM with two buffers, DP = 192 with one.
-// Dropout: a Philox call covers one query and 8 keys. Each lane makes the calls of 4 queries for its octet of keys and
-// the 8 x 8 bit blocks are transposed among 8 lanes (3 shuffles per 32 x 32 bits), so no call is made twice.
+// and a thread owns one key's BQ / 4 queries; dS^T also goes to the scratch for dQ and the table's gradient.
+//   MMA warp       dV(c), S^T(c + 1), dK(c), dP^T(c + 1), each as soon as what it reads is there and what it overwrites
+//                  has been read by the product before it
+//   4 warpgroups   P of chunk c while dK(c - 1) and dP^T(c) run, then dS of chunk c while dV(c) and S^T(c + 1) run
+// Bound by the operand feed of the products (S and dP 64 clocks per 16 of the head dim and 128 queries, dV and dK as
+// many per 16 queries at DP = 128): chunks of 128 queries, which halve K's and V's share of it, with one score buffer
+// (S 128, dP 128, dK 128, dV 128 columns) beat chunks of 64 with two. DP = 192 has columns for 64 queries only.
+// Dropout: a Philox call covers one query and 8 keys. Each lane makes the calls of 2 or 4 queries for its octet of keys
+// and the 8 x 8 bit blocks are transposed among 8 lanes (3 shuffles), so no call is made twice.
 // ---------------------------------------------------------------------------------------------------------------
 template <int DP>
 struct KeysCfg {
-  static constexpr int EW = DP == 64 ? 1 : 2, CTAS = DP == 64 ? 2 : 1;
-  static constexpr int NB = DP == 128 ? 2 : 1;                 // score buffers (S^T and dP^T)
-  static constexpr int NST = DP == 192 ? 2 : 4;                // chunks of Q, dO and records in flight
-  static constexpr int K_BYTES = DP / 64 * 128 * 128, Q_BYTES = DP / 64 * 64 * 128, REC_BYTES = 768;
+  static constexpr int BQ = DP == 192 ? 64 : 128, QT = BQ / 4;  // queries per chunk and per thread
+  static constexpr int NST = DP == 64 ? 4 : 2;                  // chunks of Q, dO and records in flight
+  static constexpr int K_BYTES = DP / 64 * 128 * 128, Q_BYTES = DP / 64 * BQ * 128, REC_BYTES = BQ * 12;
   static constexpr int STAGE = 2 * Q_BYTES;
   static constexpr int OFF_V = K_BYTES, OFF_ST = 2 * K_BYTES, OFF_REC = OFF_ST + NST * STAGE,
-                       OFF_TAB = OFF_REC + NST * REC_BYTES, SMEM = OFF_TAB + 1024;
-  static constexpr int TM_DK = 0, TM_DV = DP, TM_S = 2 * DP, TM_COLS = CTAS == 2 ? 256 : 512;
-  static constexpr int THREADS = EW * 128 + 64, TMA_WARP = EW * 4, MMA_WARP = EW * 4 + 1;
+                       OFF_TAB = OFF_REC + NST * REC_BYTES, SMEM = OFF_TAB + 512;
+  static constexpr int TM_DK = 0, TM_DV = DP, TM_S = 2 * DP, TM_DP = TM_S + BQ, TM_COLS = 512;
+  static constexpr int EWT = 512, THREADS = EWT + 64, TMA_WARP = 16, MMA_WARP = 17;
 };
 
-// Keep bits of 32 queries (i0 ..) for this lane's key j0 + lane: query 8 c + 2 i + e at bit 15 - (4 c + i) + 16 e. A
+// Keep bits of 8 CALLS queries (i0 ..) for this lane's key j0 + lane: query 8 c + 2 i + e at bit 15 - (4 c + i) + 16 e. A
 // lane makes the calls of queries 8 c + lane % 8 for keys 8 (lane / 8) ..; bit (c, i, e) there is key 2 i + e, and three
 // exchanges transpose the 8 x 8 bits of each octet of lanes.
+template <int CALLS>
 __device__ __forceinline__ uint32_t keep_column(const AttnDrop& drop, uint32_t thr2, uint32_t i0, uint32_t j0,
                                                 uint32_t bh) {
   const int lane = threadIdx.x & 31;
   uint32_t x = 0;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
+  for (int c = 0; c < CALLS; ++c) {
     const uint4 u = drop.words(i0 + 8 * c + (lane & 7), (j0 >> 3) + (lane >> 3), bh);
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -580,18 +587,18 @@ __device__ __forceinline__ uint32_t keep_column(const AttnDrop& drop, uint32_t t
 }
 
 template <int DP, bool BIAS, bool DROP>
-__global__ void __launch_bounds__(KeysCfg<DP>::THREADS, KeysCfg<DP>::CTAS)
+__global__ void __launch_bounds__(KeysCfg<DP>::THREADS, 1)
     xattn_bwd_keys_kernel(const __grid_constant__ XMaps maps, const XParams p) {
   using C = KeysCfg<DP>;
-  constexpr int NB = C::NB, NST = C::NST;
-  __shared__ uint64_t bar_k, bar_full[NST], bar_empty[NST], bar_s[NB], bar_p[NB], bar_done;
+  constexpr int NST = C::NST, BQ = C::BQ, QT = C::QT;
+  __shared__ uint64_t bar_k, bar_full[NST], bar_empty[NST], bar_s, bar_dp, bar_p, bar_ds, bar_done;
   __shared__ uint32_t tmem_sh;
   __shared__ int abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int nkt = (p.Nk + 127) / 128, kt = blockIdx.x % nkt, ul = blockIdx.x / nkt, unit = p.u0 + ul;
   const int b = unit / p.Hkv, kh = unit % p.Hkv, j0 = kt * 128;
   const int n = key_count(p, b);
-  const int nqc = p.nqp / 64, nc = nqc * p.G;
+  const int nqc = (p.nqp + BQ - 1) / BQ, nc = nqc * p.G;
   WaitCtx ctx{&abort_flag, p.status};
   __nv_bfloat16* dK = reinterpret_cast<__nv_bfloat16*>(p.dk.p) + b * p.dk.s[0] + kh * p.dk.s[1];
   __nv_bfloat16* dV = reinterpret_cast<__nv_bfloat16*>(p.dv.p) + b * p.dv.s[0] + kh * p.dv.s[1];
@@ -613,10 +620,10 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, KeysCfg<DP>::CTAS)
       mbar_init(&bar_full[i], 1);
       mbar_init(&bar_empty[i], 1);
     }
-    for (int i = 0; i < NB; ++i) {
-      mbar_init(&bar_s[i], 1);
-      mbar_init(&bar_p[i], C::EW * 128);
-    }
+    mbar_init(&bar_s, 1);
+    mbar_init(&bar_dp, 1);
+    mbar_init(&bar_p, C::EWT);
+    mbar_init(&bar_ds, C::EWT);
     mbar_init(&bar_done, 1);
     fence_barrier_init();
   }
@@ -624,7 +631,6 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, KeysCfg<DP>::CTAS)
     tmem_alloc(&tmem_sh, C::TM_COLS);
     tmem_relinquish();
   }
-  float* tab = reinterpret_cast<float*>(xsmem + C::OFF_TAB);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -637,139 +643,177 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, KeysCfg<DP>::CTAS)
         load_rows<DP>(xsmem + x * 128, &maps.k, &bar_k, 128 * 128, j0 + x, kh, b);
         load_rows<DP>(xsmem + C::OFF_V + x * 128, &maps.v, &bar_k, 128 * 128, j0 + x, kh, b);
       }
+      const int recs = p.nqp / 64;  // blocks of 64 records per head
       for (int c = 0; c < nc; ++c) {
-        const int st = c % NST, h = kh * p.G + c / nqc, qc = c % nqc;
+        const int st = c % NST, h = kh * p.G + c / nqc, q0 = c % nqc * BQ;
+        // a last chunk of 128 queries may hold 64 padded rows only: no records for the others (`inside` below)
+        const int rec = (p.nqp - q0 < BQ ? 64 : BQ) * 12;
         if (!mbar_wait(&bar_empty[st], ((c / NST) & 1) ^ 1, ctx)) break;
         uint8_t* dst = xsmem + C::OFF_ST + st * C::STAGE;
-        mbar_arrive_expect_tx(&bar_full[st], C::STAGE + C::REC_BYTES);
-        load_rows<DP>(dst, &maps.q, &bar_full[st], 64 * 128, qc * 64, h, b);
-        load_rows<DP>(dst + C::Q_BYTES, &maps.dout, &bar_full[st], 64 * 128, qc * 64, h, b);
-        bulk_load(xsmem + C::OFF_REC + st * C::REC_BYTES, p.rec + ((long long)(b * p.H + h) * nqc + qc) * 192,
-                  C::REC_BYTES, &bar_full[st]);
+        mbar_arrive_expect_tx(&bar_full[st], C::STAGE + rec);
+        for (int x = 0; x < BQ; x += 64) {
+          load_rows<DP>(dst + x * 128, &maps.q, &bar_full[st], BQ * 128, q0 + x, h, b);
+          load_rows<DP>(dst + C::Q_BYTES + x * 128, &maps.dout, &bar_full[st], BQ * 128, q0 + x, h, b);
+        }
+        bulk_load(xsmem + C::OFF_REC + st * C::REC_BYTES, p.rec + ((long long)(b * p.H + h) * recs + q0 / 64) * 192, rec,
+                  &bar_full[st]);
       }
     }
   } else if (warp == C::MMA_WARP) {
     if (lane == 0) {
-      bool ok = mbar_wait(&bar_k, 0, ctx);
-      auto scores = [&](int c) {
-        const int st = c % NST;
-        if (!(ok = ok && mbar_wait(&bar_full[st], (c / NST) & 1, ctx))) return;
+      bool ok = mbar_wait(&bar_k, 0, ctx) && mbar_wait(&bar_full[0], 0, ctx);
+      const uint32_t q0 = sbase + C::OFF_ST;
+      if (ok) {
         tc_fence_after();
-        const uint32_t q = sbase + C::OFF_ST + st * C::STAGE, acc = tmem + C::TM_S + (c % NB) * 128;
-        mma_scores<DP>(acc, sbase, q);
-        mma_scores<DP>(acc + 64, sbase + C::OFF_V, q + C::Q_BYTES);
-        mma_commit(&bar_s[c % NB]);
-      };
-      scores(0);
+        mma_scores<DP, BQ>(tmem + C::TM_S, sbase, q0);
+        mma_commit(&bar_s);
+        mma_scores<DP, BQ>(tmem + C::TM_DP, sbase + C::OFF_V, q0 + C::Q_BYTES);
+        mma_commit(&bar_dp);
+      }
       for (int c = 0; c < nc && ok; ++c) {
-        if (NB == 2 && c + 1 < nc) scores(c + 1);
-        const int st = c % NST;
-        if (!(ok = ok && mbar_wait(&bar_p[c % NB], (c / NB) & 1, ctx))) break;
+        const int st = c % NST, sn = (c + 1) % NST;
+        const uint32_t q = q0 + st * C::STAGE, qn = q0 + sn * C::STAGE;
+        if (!(ok = mbar_wait(&bar_p, c & 1, ctx))) break;
         tc_fence_after();
-        const uint32_t q = sbase + C::OFF_ST + st * C::STAGE, acc = tmem + C::TM_S + (c % NB) * 128;
-        mma_pieces<DP>(tmem + C::TM_DV, acc, q + C::Q_BYTES, c > 0);
-        mma_pieces<DP>(tmem + C::TM_DK, acc + 64, q, c > 0);
+        mma_pieces<DP, BQ, QT>(tmem + C::TM_DV, tmem + C::TM_S, q + C::Q_BYTES, c > 0);
+        if (c + 1 < nc) {
+          if (!(ok = mbar_wait(&bar_full[sn], ((c + 1) / NST) & 1, ctx))) break;
+          tc_fence_after();
+          mma_scores<DP, BQ>(tmem + C::TM_S, sbase, qn);
+          mma_commit(&bar_s);
+        }
+        if (!(ok = mbar_wait(&bar_ds, c & 1, ctx))) break;
+        tc_fence_after();
+        mma_pieces<DP, BQ, QT>(tmem + C::TM_DK, tmem + C::TM_DP, q, c > 0);
         mma_commit(&bar_empty[st]);
-        if (NB == 1 && c + 1 < nc) scores(c + 1);
+        if (c + 1 < nc) {
+          mma_scores<DP, BQ>(tmem + C::TM_DP, sbase + C::OFF_V, qn + C::Q_BYTES);
+          mma_commit(&bar_dp);
+        }
       }
       if (ok) mma_commit(&bar_done);
     }
   } else {
-    const int wg = C::EW == 1 ? 0 : warp / 4, r = (warp & 3) * 32 + lane, j = j0 + r;
+    const int wg = warp / 4, r = (warp & 3) * 32 + lane, j = j0 + r;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t sbuf = lanes + C::TM_S + wg * QT, dbuf = lanes + C::TM_DP + wg * QT;
     const bool check_keys = p.kmask != nullptr || j0 + 128 > n, live = key_live(p, b, j, n);
     const AttnDrop drop = attn_drop(p.rng, DROP ? p.drop_thr : 0, p.drop_scale);
     const uint32_t thr2 = drop.pair();
     const uint64_t sc2 = f2(p.scale_log2, p.scale_log2), ds2 = f2(drop.scale, drop.scale);
-    const long long tile = ((long long)(j / 64) * (p.nqp / 8)) * 64 + j % 64;  // of ids and dS, in granules of 8
-    constexpr int IDS = 2 / C::EW * 4;
-    uint2 id8[IDS];
-    auto fetch = [&](int c) {  // a chunk ahead
+    // ids and dS lie in granules of 8 queries: this key's first granule of a chunk, and 8 BQ granules per chunk
+    const long long tile = ((long long)(j / 64) * (p.nqp / 8) + wg * (QT / 8)) * 64 + j % 64;
+    const uint4* idp = reinterpret_cast<const uint4*>(p.idsT) + tile;
+    uint4* const ds0 = reinterpret_cast<uint4*>(p.ds) + (long long)ul * p.G * (p.nkp / 8) * p.nqp + tile;
+    constexpr uint32_t no = kNoPairOffset * 0x10001u;
+    const uint4 none = make_uint4(no, no, no, no);
+    uint4 id[QT / 8];
+    auto fetch = [&](int qc) {  // a chunk ahead
 #pragma unroll
-      for (int x = 0; x < IDS; ++x)
-        id8[x] = __ldg(reinterpret_cast<const uint2*>(p.idsT) + tile + (long long)((c % nqc) * 8 + wg * 4 + x) * 64);
+      for (int x = 0; x < QT / 8; ++x)
+        id[x] = qc * BQ + wg * QT < p.nqp ? __ldg(idp + qc * (8 * BQ) + x * 64) : none;
     };
     if (BIAS) fetch(0);
     bool ok = true;
+    int qc = 0, g = 0;
     for (int c = 0; c < nc; ++c) {
-      const int st = c % NST, g = c / nqc, i0 = (c % nqc) * 64, bh = b * p.H + kh * p.G + g;
-      if (BIAS && c % nqc == 0) {  // the next head's bias
-        named_sync(1, C::EW * 128);
-        for (int t = threadIdx.x; t < 256; t += C::EW * 128) tab[t] = table_log2(p, kh * p.G + g, t);
-        named_sync(1, C::EW * 128);
+      const int st = c % NST, i0 = qc * BQ + wg * QT, bh = b * p.H + kh * p.G + g;
+      const bool inside = i0 < p.nqp;  // else a last chunk's padding: P = dS = 0, and nothing to store
+      uint4* ds = ds0 + (long long)g * (p.nkp / 8) * p.nqp + qc * (8 * BQ);
+      if (BIAS && qc == 0) {  // the next head's bias
+        named_sync(1, C::EWT);
+        if (threadIdx.x <= kMaxBuckets)
+          reinterpret_cast<float*>(xsmem + C::OFF_TAB)[threadIdx.x] = table_log2(p, kh * p.G + g, threadIdx.x);
+        named_sync(1, C::EWT);
       }
-      const uint32_t sbuf = lanes + C::TM_S + (c % NB) * 128;
+      if (++qc == nqc) qc = 0, ++g;
+      uint32_t keep = 0;
+      if (DROP) keep = keep_column<QT / 8>(drop, thr2, i0, j0 + (warp & 3) * 32, bh);
+      const bool some = (!check_keys || live) && inside;
+      const float* rec = reinterpret_cast<const float*>(xsmem + C::OFF_REC + st * C::REC_BYTES) + wg * QT / 64 * 192 +
+                         wg * QT % 64;
       // bar_s follows bar_full, so the records are there too; the wait on bar_full makes their copy visible here
-      if (ok) ok = warp_wait(&bar_full[st], (c / NST) & 1, ctx) && warp_wait(&bar_s[c % NB], (c / NB) & 1, ctx);
-      if (!ok) continue;  // given up: only the barrier above is still met
+      if (ok) ok = warp_wait(&bar_full[st], (c / NST) & 1, ctx) && warp_wait(&bar_s, c & 1, ctx);
+      if (!ok) continue;  // given up: only the barriers above are still met
       tc_fence_after();
-      const float* rec = reinterpret_cast<const float*>(xsmem + C::OFF_REC + st * C::REC_BYTES);
-      uint4* ds = reinterpret_cast<uint4*>(p.ds) + (long long)(ul * p.G + g) * (p.nkp / 8) * p.nqp + tile +
-                  (long long)(i0 / 8) * 64;
+      uint64_t pr[QT / 2];
 #pragma unroll
-      for (int piece = wg; piece < 2; piece += C::EW) {
-        uint32_t s[32], dp[32];
-        tmem_ld32_issue(sbuf + piece * 32, s);
-        tmem_ld32_issue(sbuf + 64 + piece * 32, dp);
-        uint32_t keep = 0;
-        if (DROP) keep = keep_column(drop, thr2, i0 + piece * 32, j0 + (warp & 3) * 32, bh);
-        tmem_wait32(s);
-        tmem_pin32(dp);
-        uint32_t wp[16], wd[16];
+      for (int k = 0; k < QT / 16; ++k) {
+        uint32_t s[16], w[8];
+        tmem_ld16_issue(sbuf + k * 16, s);
+        tmem_wait16(s);
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {  // two pairs of queries
-          const ulonglong2 r0 = *reinterpret_cast<const ulonglong2*>(rec + piece * 32 + 2 * e);
-          const ulonglong2 r2 = *reinterpret_cast<const ulonglong2*>(rec + 128 + piece * 32 + 2 * e);
-          const uint64_t a0[2] = {r0.x, r0.y}, nd[2] = {r2.x, r2.y};
+        for (int e = 0; e < 8; e += 2) {  // two pairs of queries
+          const ulonglong2 r0 = *reinterpret_cast<const ulonglong2*>(rec + k * 16 + 2 * e);
           ulonglong2 r1 = make_ulonglong2(0, 0);
-          if (BIAS) r1 = *reinterpret_cast<const ulonglong2*>(rec + 64 + piece * 32 + 2 * e);
-          const uint64_t a1[2] = {r1.x, r1.y};
+          if (BIAS) r1 = *reinterpret_cast<const ulonglong2*>(rec + 64 + k * 16 + 2 * e);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const int q = e + u;  // queries 2 q, 2 q + 1 of the piece
+            const int q = e + u;
             uint64_t t = f2(__uint_as_float(s[2 * q]), __uint_as_float(s[2 * q + 1]));
-            if (BIAS) {
-              const uint32_t w = reinterpret_cast<const uint32_t*>(id8)[(piece / C::EW) * 8 + q / 2] >> (16 * (q & 1));
-              t = add2(fma2(t, sc2, f2(tab[w & 255], tab[(w >> 8) & 255])), a0[u]);
-            } else {
-              t = fma2(t, sc2, a0[u]);
-            }
+            if (BIAS)
+              t = add2(fma2(t, sc2, table_pair(C::OFF_TAB, reinterpret_cast<const uint32_t*>(id)[k * 8 + q])), u ? r0.y : r0.x);
+            else
+              t = fma2(t, sc2, u ? r0.y : r0.x);
             float x, y;
             unf2(t, x, y);
-            x = xex2(x), y = xex2(y);
-            uint64_t pr = f2(x, y);
-            if (BIAS) {
-              pr = mul2(pr, a1[u]);
-              unf2(pr, x, y);
-            }
-            wp[q] = pack_bf16(x, y);
-            uint64_t da;
-            if (DROP) {
-              const uint32_t k = keep << ((q / 4) * 4 + q % 4);
-              wp[q] &= spread_pair(k);
-              da = f2(__uint_as_float(dp[2 * q] & spread_one<0>(k)), __uint_as_float(dp[2 * q + 1] & spread_one<1>(k)));
-              da = fma2(da, ds2, nd[u]);
-            } else {
-              da = add2(f2(__uint_as_float(dp[2 * q]), __uint_as_float(dp[2 * q + 1])), nd[u]);
-            }
-            unf2(mul2(pr, da), x, y);
-            wd[q] = pack_bf16(x, y);
+            t = f2(xex2(x), xex2(y));
+            if (BIAS) t = mul2(t, u ? r1.y : r1.x);
+            pr[k * 8 + q] = t;
+            unf2(t, x, y);
+            w[q] = pack_bf16(x, y);
+            if (DROP) w[q] &= spread_pair(keep << (k * 8 + q));
           }
         }
-        if (check_keys) {  // an absent key's row is 0 whatever K and V hold there
+        if (check_keys || !inside) {  // an absent key's row is 0 whatever K and V hold there
 #pragma unroll
-          for (int e = 0; e < 16; ++e) wp[e] = live ? wp[e] : 0u, wd[e] = live ? wd[e] : 0u;
+          for (int e = 0; e < 8; ++e) w[e] = some ? w[e] : 0u;
         }
-        tmem_st16(sbuf + piece * 32, wp);
-        tmem_st16(sbuf + 64 + piece * 32, wd);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          ds[(piece * 4 + e) * 64] = make_uint4(wd[4 * e], wd[4 * e + 1], wd[4 * e + 2], wd[4 * e + 3]);
+        tmem_st8(sbuf + k * 8, w);
       }
-      if (BIAS && c + 1 < nc) fetch(c + 1);
+      if (BIAS && c + 1 < nc) fetch(qc);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&bar_p[c % NB]);
+      mbar_arrive(&bar_p);
+      if (!(ok = warp_wait(&bar_dp, c & 1, ctx))) continue;
+      tc_fence_after();
+#pragma unroll
+      for (int k = 0; k < QT / 16; ++k) {
+        uint32_t dp[16], w[8];
+        tmem_ld16_issue(dbuf + k * 16, dp);
+        tmem_wait16(dp);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const ulonglong2 r2 = *reinterpret_cast<const ulonglong2*>(rec + 128 + k * 16 + 2 * e);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int q = e + u;
+            uint64_t da;
+            if (DROP) {
+              const uint32_t kb = keep << (k * 8 + q);
+              da = f2(__uint_as_float(dp[2 * q] & spread_one<0>(kb)), __uint_as_float(dp[2 * q + 1] & spread_one<1>(kb)));
+              da = fma2(da, ds2, u ? r2.y : r2.x);
+            } else {
+              da = add2(f2(__uint_as_float(dp[2 * q]), __uint_as_float(dp[2 * q + 1])), u ? r2.y : r2.x);
+            }
+            float x, y;
+            unf2(mul2(pr[k * 8 + q], da), x, y);
+            w[q] = pack_bf16(x, y);
+          }
+        }
+        if (check_keys || !inside) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = some ? w[e] : 0u;
+        }
+        tmem_st8(dbuf + k * 8, w);
+        if (inside) {
+          ds[(2 * k) * 64] = make_uint4(w[0], w[1], w[2], w[3]);
+          ds[(2 * k + 1) * 64] = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&bar_ds);
     }
     if (ok) ok = warp_wait(&bar_done, 0, ctx);
     tc_fence_after();
@@ -777,7 +821,7 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, KeysCfg<DP>::CTAS)
     const float fv = DROP ? p.drop_scale : 1.f;
     if (ok) {  // K's and V's tiles are free: every product has completed
 #pragma unroll 1
-      for (int d = wg * 32; d < DP; d += C::EW * 32) {
+      for (int d = wg * 32; d < DP; d += 128) {
         float x[32];
         tmem_ld32(lanes + C::TM_DK + d, x);
         if (tk) stage_row32(xsmem, r, d, x, p.scale);
@@ -788,7 +832,7 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, KeysCfg<DP>::CTAS)
       }
     }
     fence_proxy_async_smem();
-    named_sync(1, C::EW * 128);
+    named_sync(1, C::EWT);
     if (threadIdx.x == 0 && ok) {
       if (tk) store_tile<DP>(&maps.dk, xsmem, p.D, j0, kh, b);
       if (tv) store_tile<DP>(&maps.dv, xsmem + C::OFF_V, p.D, j0, kh, b);
