@@ -4,7 +4,11 @@ The library is built in-tree by ``foreswe_gpu_optimization_b200.build.build()``.
 CPU or eager fallback for the hot path.
 """
 import ctypes
+import functools
 import os
+import struct
+
+import torch
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libgeoattn.so")
@@ -68,6 +72,14 @@ class XattnBwdArgs(ctypes.Structure):
                 ("dq", ctypes.c_void_p), ("dq_stride", c_ll4), ("dk", ctypes.c_void_p), ("dk_stride", c_ll4),
                 ("dv", ctypes.c_void_p), ("dv_stride", c_ll4), ("dtable", ctypes.c_void_p),
                 ("workspace", ctypes.c_void_p)]
+
+
+# The same argument blocks as one struct.pack each: filling a ctypes structure field by field costs more than the
+# launches of a small call. Pointers (0 for none), strides and sizes in the order of the structures above.
+XATTN_INPUTS = "9i5q5q5qqqqqqqqif"   # shape, q, k, v, ids, ids_ld, table, kv_lens, key_mask, key_mask_ld, rng, thr, scale
+XATTN_FWD = struct.Struct("@" + XATTN_INPUTS + "5qqq")               # o, stats, workspace
+XATTN_BWD = struct.Struct("@" + XATTN_INPUTS + "5q5qq5q5q5qqq")      # o, dO, stats, dq, dk, dv, dtable, workspace
+assert XATTN_FWD.size == ctypes.sizeof(XattnFwdArgs) and XATTN_BWD.size == ctypes.sizeof(XattnBwdArgs)
 
 
 class GeoAttnError(RuntimeError):
@@ -136,6 +148,31 @@ def lib():
 def check(rc):
     if rc != GEOATTN_OK:
         raise GeoAttnError(rc, "libgeoattn: " + lib().geoattn_error_string(rc).decode())
+
+
+@functools.lru_cache(maxsize=None)
+def packed(name):
+    """Entry point `name` taking (packed argument block, stream)."""
+    fn = lib()[name]  # a function object of its own, with its own argument types
+    fn.restype, fn.argtypes = ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]
+    return fn
+
+
+@functools.lru_cache(maxsize=4096)
+def xattn_workspace(name, *shape):
+    return getattr(lib(), name)(ctypes.byref(XattnShape(*shape)))
+
+
+def launch(device, fn, *args):
+    """fn(*args, stream) with `device` current (the library launches on the current device), its status checked."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc)
 
 
 def tensor_arg(t):

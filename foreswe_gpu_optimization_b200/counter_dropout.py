@@ -7,8 +7,6 @@ masks at every replay (the reference's graph step: tests/test_gpu_graphs.py:34-4
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
@@ -29,15 +27,6 @@ def _dtype_code(t, what):
     raise TypeError("%s must be bf16 or fp32, got %s" % (what, t.dtype))
 
 
-def _launch(device, call):
-    """Run `call(stream)` with `device` current (the library launches on the current device) and check its status."""
-    if torch.cuda.current_device() == device.index:
-        _lib.check(call(torch.cuda.current_stream().cuda_stream))
-    else:
-        with torch.cuda.device(device):
-            _lib.check(call(torch.cuda.current_stream().cuda_stream))
-
-
 class CounterRNG:
     """(seed, offset) of the counter-based generator, int64[2] on one device; each `take` hands out the next offset."""
 
@@ -49,8 +38,7 @@ class CounterRNG:
 
     def take(self) -> torch.Tensor:
         out = torch.empty_like(self.state)
-        _launch(self.state.device,
-                lambda s: _lib.lib().geoattn_rng_take(self.state.data_ptr(), out.data_ptr(), s))
+        _lib.launch(self.state.device, _lib.lib().geoattn_rng_take, self.state.data_ptr(), out.data_ptr())
         return out
 
 
@@ -70,9 +58,8 @@ def _snapshot(rng, device):
 def _run(x, residual, rng, thr):
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if x.numel():
-        _launch(x.device, lambda s: _lib.lib().geoattn_dropout(
-            _dtype_code(x, "x"), x.numel(), x.data_ptr(), None if residual is None else residual.data_ptr(),
-            y.data_ptr(), rng.data_ptr(), thr, s))
+        _lib.launch(x.device, _lib.lib().geoattn_dropout, _dtype_code(x, "x"), x.numel(), x.data_ptr(),
+                    None if residual is None else residual.data_ptr(), y.data_ptr(), rng.data_ptr(), thr)
     return y
 
 
@@ -110,4 +97,4 @@ def dropout(x, p, rng, residual=None):
     key = _snapshot(rng, x.device)
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
         return _Dropout.apply(x, residual, key, thr)
-    return _run(x.detach().contiguous(), None if residual is None else residual.detach().contiguous(), key, thr)
+    return _run(x.contiguous(), None if residual is None else residual.contiguous(), key, thr)

@@ -9,13 +9,12 @@ backward instead of stored. No [Nq, Nk] tensor per head ever reaches memory in t
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
 
 from . import _lib
-from .counter_dropout import _dtype_code, _launch, _snapshot, _threshold
+from .counter_dropout import _dtype_code, _snapshot, _threshold
 from .geo_attention_v2 import _tma_ready
 
 MAX_BUCKETS = 64
@@ -23,9 +22,12 @@ MAX_BUCKETS = 64
 
 def _ready(t):
     """Operand layout of the kernels: bf16 as TMA reads it; fp32 with the head dim contiguous."""
-    if t.dtype == torch.bfloat16:
-        return _tma_ready(t)
-    return t if t.stride(3) == 1 else t.contiguous()
+    if t.dtype == torch.float32:
+        return t if t.stride(3) == 1 else t.contiguous()
+    s0, s1, s2, s3 = t.stride()
+    if s3 == 1 and not ((t.data_ptr() >> 1) | s0 | s1 | s2) & 7 and s0 > 0 and s1 > 0 and s2 > 0:
+        return t
+    return _tma_ready(t)
 
 
 def _like(t):
@@ -33,26 +35,25 @@ def _like(t):
     return torch.empty_like(t) if t.stride(3) == 1 else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
-def _strides(t):
-    s = t.stride()  # of a head dim of size 1 any stride says the same
-    return _lib.c_ll4(s[0], s[1], s[2], 1 if t.shape[3] == 1 else s[3])
-
-
-def _tensor(t):
-    return _lib.Tensor(t.data_ptr(), _strides(t))
+def _arg(t):
+    """(pointer, four strides) of an argument block."""
+    s0, s1, s2, s3 = t.stride()  # of a head dim of size 1 any stride says the same
+    return t.data_ptr(), s0, s1, s2, 1 if t.shape[3] == 1 else s3
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
-def _inputs(q, k, v, table, ids, lens, mask, rng, thr, scale):
+def _shape(q, k, table):
     B, H, Nq, D = q.shape
-    sh = _lib.XattnShape(B, H, k.shape[1], Nq, k.shape[2], D, _dtype_code(q, "q"), table.shape[1] if table is not None
-                         else 0, _dtype_code(table, "bias_table") if table is not None else _lib.DTYPE_FP32)
-    return _lib.XattnInputs(sh, _tensor(q), _tensor(k), _tensor(v), _ptr(ids),
-                            0 if ids is None else ids.stride(0), _ptr(table), _ptr(lens), _ptr(mask),
-                            0 if mask is None else mask.stride(0), _ptr(rng), thr, scale)
+    T, tdt = (0, _lib.DTYPE_FP32) if table is None else (table.shape[1], _dtype_code(table, "bias_table"))
+    return B, H, k.shape[1], Nq, k.shape[2], D, _dtype_code(q, "q"), T, tdt
+
+
+def _inputs(shape, q, k, v, table, ids, lens, mask, rng, thr, scale):
+    return (*shape, *_arg(q), *_arg(k), *_arg(v), _ptr(ids), 0 if ids is None else ids.stride(0), _ptr(table),
+            _ptr(lens), _ptr(mask), 0 if mask is None else mask.stride(0), _ptr(rng), thr, scale)
 
 
 def _forward(q, k, v, table, ids, lens, mask, rng, thr, scale, need_stats):
@@ -60,12 +61,11 @@ def _forward(q, k, v, table, ids, lens, mask, rng, thr, scale, need_stats):
     if k.shape[2] == 0 or thr == 65536:  # no key, or no weight is kept
         return o.zero_(), None
     q, k, v = _ready(q), _ready(k), _ready(v)
-    L = _lib.lib()
-    inp = _inputs(q, k, v, table, ids, lens, mask, rng, thr, scale)
-    ws = torch.empty(L.geoattn_xattn_fwd_workspace_bytes(ctypes.byref(inp.shape)), dtype=torch.uint8, device=q.device)
-    stats = torch.empty(*q.shape[:3], 2, dtype=torch.float32, device=q.device) if need_stats else None
-    args = _lib.XattnFwdArgs(inp, o.data_ptr(), _strides(o), _ptr(stats), ws.data_ptr())
-    _launch(q.device, lambda s: L.geoattn_xattn_fwd(ctypes.byref(args), s))
+    shape, dev = _shape(q, k, table), q.device
+    ws = torch.empty(_lib.xattn_workspace("geoattn_xattn_fwd_workspace_bytes", *shape), dtype=torch.uint8, device=dev)
+    stats = torch.empty(*q.shape[:3], 2, dtype=torch.float32, device=dev) if need_stats else None
+    _lib.launch(dev, _lib.packed("geoattn_xattn_fwd"), _lib.XATTN_FWD.pack(
+        *_inputs(shape, q, k, v, table, ids, lens, mask, rng, thr, scale), *_arg(o), _ptr(stats), ws.data_ptr()))
     return o, stats
 
 
@@ -75,13 +75,11 @@ def _backward(q, k, v, table, ids, lens, mask, rng, thr, scale, o, stats, do):
     if k.shape[2] == 0 or thr == 65536:
         return dq.zero_(), dk.zero_(), dv.zero_(), None if dtable is None else dtable.zero_()
     q, k, v, do = _ready(q), _ready(k), _ready(v), _ready(do)
-    L = _lib.lib()
-    inp = _inputs(q, k, v, table, ids, lens, mask, rng, thr, scale)
-    ws = torch.empty(L.geoattn_xattn_bwd_workspace_bytes(ctypes.byref(inp.shape)), dtype=torch.uint8, device=q.device)
-    args = _lib.XattnBwdArgs(inp, _tensor(o), _tensor(do), stats.data_ptr(), dq.data_ptr(),
-                             _strides(dq), dk.data_ptr(), _strides(dk), dv.data_ptr(),
-                             _strides(dv), _ptr(dtable), ws.data_ptr())
-    _launch(q.device, lambda s: L.geoattn_xattn_bwd(ctypes.byref(args), s))
+    shape, dev = _shape(q, k, table), q.device
+    ws = torch.empty(_lib.xattn_workspace("geoattn_xattn_bwd_workspace_bytes", *shape), dtype=torch.uint8, device=dev)
+    _lib.launch(dev, _lib.packed("geoattn_xattn_bwd"), _lib.XATTN_BWD.pack(
+        *_inputs(shape, q, k, v, table, ids, lens, mask, rng, thr, scale), *_arg(o), *_arg(do), stats.data_ptr(),
+        *_arg(dq), *_arg(dk), *_arg(dv), _ptr(dtable), ws.data_ptr()))
     return dq, dk, dv, dtable
 
 
@@ -148,11 +146,12 @@ def cross_attention(q, k, v, *, buckets=None, bias_table=None, kv_lens=None, key
         raise ValueError("scale must be positive and finite, got %r" % (scale,))
     if not q.is_cuda:
         raise RuntimeError("cross attention runs on CUDA tensors only (no CPU path)")
+    dev = q.device
     for name, t in (("k", k), ("v", v), ("buckets", buckets), ("bias_table", bias_table), ("kv_lens", kv_lens),
                     ("key_mask", key_mask)):
-        if t is not None and t.device != q.device:
-            raise ValueError("%s lives on %s, q on %s" % (name, t.device, q.device))
-    key = _snapshot(rng, q.device) if thr else None
+        if t is not None and t.device != dev:
+            raise ValueError("%s lives on %s, q on %s" % (name, t.device, dev))
+    key = _snapshot(rng, dev) if thr else None
     if q.numel() == 0:  # no batch, head, query or head dim: nothing to launch
         return q * 1.0
     if bias_table is not None:
@@ -162,7 +161,7 @@ def cross_attention(q, k, v, *, buckets=None, bias_table=None, kv_lens=None, key
         if buckets.stride(1) != 1 or buckets.stride(0) < Nk:
             buckets = buckets.contiguous()
     if kv_lens is not None:
-        kv_lens = kv_lens.to(torch.int32).contiguous()
+        kv_lens = (kv_lens if kv_lens.dtype == torch.int32 else kv_lens.to(torch.int32)).contiguous()
     if key_mask is not None and (key_mask.stride(1) != 1 or key_mask.stride(0) < Nk):
         key_mask = key_mask.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
