@@ -178,8 +178,8 @@ int xlaunch(K kernel, long long grid, int threads, int smem, cudaStream_t st, co
 
 template <int DP>
 int simt_fwd(const XParams& p, cudaStream_t st) {
-  return xlaunch(xattn_simt_fwd_kernel<DP>, (long long)((p.Nq + 127) / 128) * p.B * p.H * p.splits, kSimtThreads,
-                 SimtFwd<DP>::SMEM, st, p);
+  return xlaunch(xattn_simt_fwd_kernel<DP>, (long long)((p.Nq + 127) / 128) * p.B * p.H * p.splits,
+                 SimtFwd<DP>::NT, SimtFwd<DP>::SMEM, st, p);
 }
 int forward_simt(const XParams& p, const XDims& d, cudaStream_t st) {
   return d.DP == 64 ? simt_fwd<64>(p, st) : d.DP == 128 ? simt_fwd<128>(p, st) : simt_fwd<192>(p, st);

@@ -2,60 +2,76 @@
 // these kernels keep every product and sum in fp32, so the results carry fp32 accuracy.
 //
 // Tiles sit in shared memory head-dim-major ([d][row], rows padded by 4 floats), so that a thread's 4 or 8 rows (or
-// keys) are one or two 16-byte loads per d; each of the 256 threads (16 x 16) owns a register block of the product.
-// Bound by the FMA pipe: per d a warp issues 32 (forward) or 32 (S and dP together) FMAs against 4-5 shared-memory
-// wavefronts.
+// keys) are one or two 16-byte loads per d; each of the 256 threads (16 x 16) owns a register block of the product and
+// works on it two values at a time (fma.rn.f32x2). Weights go through shared memory between the two products, in
+// 16-byte chunks whose place is XORed with the writing lane so that neither side meets a bank conflict.
+// Bound by the FMA pipe.
 #pragma once
+#include <type_traits>
+
 #include "xattn_common.cuh"
 
 namespace geoattn {
 
 constexpr int kSimtThreads = 256;
 
-// dst[d][r] = row r of `src` (zero where r >= n, d >= D or !live[r]); 4 consecutive d per load where `vec`.
-template <int ROWS, int DP, int ST>
-__device__ __forceinline__ void simt_load_t(float* dst, const float* src, long long ld, int n, int D, bool vec,
-                                            const float* live) {
-  for (int x = threadIdx.x; x < ROWS * (DP / 4); x += kSimtThreads) {
-    const int r = x % ROWS, d = (x / ROWS) * 4;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (r < n && d < D && (!live || live[r] == 0.f)) {
-      const float* s = src + (long long)r * ld + d;
-      if (vec) {
-        const float4 f = *reinterpret_cast<const float4*>(s);
-        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (d + i < D) v[i] = s[i];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) dst[(d + i) * ST + r] = v[i];
+// One thread's share of a tile of ROWS rows x DP columns, 4 consecutive d at a time, on its way from global to shared
+// memory: `at` gives its x-th (row, d), `get` fetches them (zero where d >= D or ok(row) is false), so that a tile can
+// be fetched while another is worked on.
+template <int ROWS, int DP, int NT = kSimtThreads>
+struct SimtTile {
+  static constexpr int N = ROWS * DP / 4 / NT;
+  float4 v[N];
+  // head-dim-major tiles: a warp takes 16 rows x 8 d, whole 32-byte sectors in and 32 different banks out
+  static __device__ __forceinline__ void at_t(int x, int& r, int& d) {
+    static_assert(ROWS % 16 == 0, "");
+    const int y = x / 32;
+    r = y % (ROWS / 16) * 16 + x % 16, d = y / (ROWS / 16) * 8 + x % 32 / 16 * 4;
   }
-}
+  // row-major tiles
+  static __device__ __forceinline__ void at_n(int x, int& r, int& d) { r = x / (DP / 4), d = x % (DP / 4) * 4; }
 
-// dst[r][d], row stride DP, as above.
-template <int ROWS, int DP>
-__device__ __forceinline__ void simt_load_n(float* dst, const float* src, long long ld, int n, int D, bool vec,
-                                            const float* live) {
-  for (int x = threadIdx.x; x < ROWS * (DP / 4); x += kSimtThreads) {
-    const int r = x / (DP / 4), d = (x % (DP / 4)) * 4;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (r < n && d < D && (!live || live[r] == 0.f)) {
-      const float* s = src + (long long)r * ld + d;
-      if (vec) {
-        const float4 f = *reinterpret_cast<const float4*>(s);
-        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-      } else {
+  template <bool T, class OK>
+  __device__ __forceinline__ void get(const float* src, long long ld, int D, bool vec, OK ok) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (d + i < D) v[i] = s[i];
+    for (int k = 0; k < N; ++k) {
+      int r, d;
+      if (T) at_t(threadIdx.x + k * NT, r, d);
+      else at_n(threadIdx.x + k * NT, r, d);
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (d < D && ok(r)) {
+        const float* s = src + (long long)r * ld + d;
+        if (vec) {
+          v[k] = *reinterpret_cast<const float4*>(s);
+        } else {
+          v[k].x = s[0];
+          if (d + 1 < D) v[k].y = s[1];
+          if (d + 2 < D) v[k].z = s[2];
+          if (d + 3 < D) v[k].w = s[3];
+        }
       }
     }
-    *reinterpret_cast<float4*>(dst + r * DP + d) = make_float4(v[0], v[1], v[2], v[3]);
   }
-}
+  template <int ST>
+  __device__ __forceinline__ void put_t(float* dst) const {
+    static_assert(4 * ST % 32 == 16, "");
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      int r, d;
+      at_t(threadIdx.x + k * NT, r, d);
+      dst[d * ST + r] = v[k].x, dst[(d + 1) * ST + r] = v[k].y;
+      dst[(d + 2) * ST + r] = v[k].z, dst[(d + 3) * ST + r] = v[k].w;
+    }
+  }
+  __device__ __forceinline__ void put_n(float* dst) const {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      int r, d;
+      at_n(threadIdx.x + k * NT, r, d);
+      *reinterpret_cast<float4*>(dst + r * DP + d) = v[k];
+    }
+  }
+};
 
 __device__ __forceinline__ bool simt_vec(const XTensor& t, int D) {
   return D % 4 == 0 && (reinterpret_cast<uintptr_t>(t.p) & 15) == 0 && t.s[0] % 4 == 0 &&
@@ -68,25 +84,30 @@ __device__ __forceinline__ bool simt_vec(const XTensor& t, int D) {
 // ---------------------------------------------------------------------------------------------------------------
 template <int DP>
 struct SimtFwd {
+  // 16 x XT threads of 8 rows and CT columns. (8 x 8 blocks load less from shared memory per FMA, but leave 4 warps per
+  // CTA, which cannot hide the softmax between the products: 579 against 538 us at 32 x 8 x 512 x 64.)
+  static constexpr int XT = 16, NT = 16 * XT, CT = 64 / XT, CO = DP / XT;
   static constexpr int BM = 128, BN = 64, SQ = BM + 4, SK = BN + 4;
-  static constexpr int FLOATS = DP * SQ + DP * SK + BN * SQ + 256 + BN;
+  static constexpr int FLOATS = DP * SQ + DP * SK + BN * BM + 256 + BN;
   static constexpr int SMEM = FLOATS * 4;
 };
 
 template <int DP>
-__global__ void __launch_bounds__(kSimtThreads) xattn_simt_fwd_kernel(const XParams p) {
+__global__ void __launch_bounds__(SimtFwd<DP>::NT, DP == 64 ? 2 : 1) xattn_simt_fwd_kernel(const XParams p) {
   using C = SimtFwd<DP>;
+  constexpr int XT = C::XT, CT = C::CT, CO = C::CO;
   extern __shared__ float4 simt_smem[];
   float* qt = reinterpret_cast<float*>(simt_smem);
   float* kv = qt + DP * C::SQ;
   float* pt = kv + DP * C::SK;
-  float* tab = pt + C::BN * C::SQ;
+  float* tab = pt + C::BN * C::BM;
   float* live = tab + 256;
   const int nqt = (p.Nq + C::BM - 1) / C::BM;
   const int qt_i = blockIdx.x % nqt, rest = blockIdx.x / nqt;
   const int h = rest % p.H, b = (rest / p.H) % p.B, split = rest / p.H / p.B;
   const int kh = h / p.G, i0 = qt_i * C::BM, bh = b * p.H + h;
-  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  const int ty = threadIdx.x / XT, tx = threadIdx.x % XT;
+  const auto col = [&](int c) { return c / 4 * (XT * 4) + tx * 4 + c % 4; };  // this thread's columns
   const int n = key_count(p, b);
   const int ntiles = (n + C::BN - 1) / C::BN;
   const int t0 = (int)((long long)ntiles * split / p.splits), t1 = (int)((long long)ntiles * (split + 1) / p.splits);
@@ -96,90 +117,121 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_fwd_kernel(const XPar
   const bool vq = simt_vec(p.q, p.D), vk = simt_vec(p.k, p.D), vv = simt_vec(p.v, p.D);
   const AttnDrop drop = attn_drop(p.rng, p.drop_thr, p.drop_scale);
 
-  if (p.ids) tab[threadIdx.x] = table_log2(p, h, threadIdx.x);
-  simt_load_t<C::BM, DP, C::SQ>(qt, Q + (long long)i0 * p.q.s[2], p.q.s[2], p.Nq - i0, p.D, vq, nullptr);
+  if (p.ids)
+    for (int t = threadIdx.x; t < 256; t += C::NT) tab[t] = table_log2(p, h, t);
+  {
+    SimtTile<C::BM, DP, C::NT> q;
+    q.template get<true>(Q + (long long)i0 * p.q.s[2], p.q.s[2], p.D, vq, [&](int r) { return i0 + r < p.Nq; });
+    q.template put_t<C::SQ>(qt);
+  }
+  SimtTile<C::BN, DP, C::NT> next;  // the next K, then V tile, fetched a product ahead
+  auto fetch = [&](const XTensor& x, const float* src, bool vec, auto t, int j0) {
+    next.template get<decltype(t)::value>(src + (long long)j0 * x.s[2], x.s[2], p.D, vec,
+                                          [&](int r) { return key_live(p, b, j0 + r, n); });
+  };
+  if (t0 < t1) fetch(p.k, K, vk, std::true_type{}, t0 * C::BN);
 
-  float m[8], l[8], acc[8][DP / 16];
+  float m[8], l[8];
+  uint64_t acc[4][CO];  // pairs of rows
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
     m[r] = -INFINITY;
     l[r] = 0.f;
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) acc[r][c] = 0.f;
+    for (int c = 0; c < CO; ++c) acc[r / 2][c] = 0;
   }
   for (int t = t0; t < t1; ++t) {
     const int j0 = t * C::BN;
-    __syncthreads();  // the last tile's products have read kv and pt; the first time: tab
+    __syncthreads();  // the last tile's products have read kv, pt and live
     if (threadIdx.x < C::BN) live[threadIdx.x] = key_live(p, b, j0 + threadIdx.x, n) ? 0.f : -INFINITY;
+    next.template put_t<C::SK>(kv);
     __syncthreads();
-    simt_load_t<C::BN, DP, C::SK>(kv, K + (long long)j0 * p.k.s[2], p.k.s[2], n - j0, p.D, vk, live);
-    __syncthreads();
-    float s[8][4] = {};
+    fetch(p.v, V, vv, std::false_type{}, j0);
+    uint64_t s2[4][CT] = {};
 #pragma unroll 4
     for (int d = 0; d < DP; ++d) {
-      const float4 a0 = *reinterpret_cast<const float4*>(qt + d * C::SQ + ty * 8);
-      const float4 a1 = *reinterpret_cast<const float4*>(qt + d * C::SQ + ty * 8 + 4);
-      const float4 k4 = *reinterpret_cast<const float4*>(kv + d * C::SK + tx * 4);
-      const float a[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w}, kk[4] = {k4.x, k4.y, k4.z, k4.w};
+      const ulonglong2 a0 = *reinterpret_cast<const ulonglong2*>(qt + d * C::SQ + ty * 8);
+      const ulonglong2 a1 = *reinterpret_cast<const ulonglong2*>(qt + d * C::SQ + ty * 8 + 4);
+      const uint64_t a[4] = {a0.x, a0.y, a1.x, a1.y};
 #pragma unroll
-      for (int r = 0; r < 8; ++r)
+      for (int c = 0; c < CT; c += 4) {
+        const float4 k4 = *reinterpret_cast<const float4*>(kv + d * C::SK + col(c));
+        const uint64_t kk[4] = {f2(k4.x, k4.x), f2(k4.y, k4.y), f2(k4.z, k4.z), f2(k4.w, k4.w)};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) s[r][c] = fmaf(a[r], kk[c], s[r][c]);
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s2[r][c + e] = fma2(a[r], kk[e], s2[r][c + e]);
+      }
     }
     __syncthreads();  // every thread has read K
-    simt_load_n<C::BN, DP>(kv, V + (long long)j0 * p.v.s[2], p.v.s[2], n - j0, p.D, vv, live);
+    next.put_n(kv);
+    if (t + 1 < t1) fetch(p.k, K, vk, std::true_type{}, j0 + C::BN);
+    float s[8][CT];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int c = 0; c < CT; ++c) unf2(s2[r][c], s[2 * r][c], s[2 * r + 1][c]);
+    float corr[8];
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
       const int i = i0 + ty * 8 + r;
       float mx = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int j = j0 + tx * 4 + c;
+      for (int c = 0; c < CT; ++c) {
+        const int j = j0 + col(c);
         float x = s[r][c] * p.scale_log2;
         if (p.ids && i < p.Nq && j < p.Nk) x += tab[p.ids[i * p.ids_ld + j]];
-        s[r][c] = live[tx * 4 + c] == 0.f ? x : -INFINITY;
+        s[r][c] = live[col(c)] == 0.f ? x : -INFINITY;
         mx = fmaxf(mx, s[r][c]);
       }
 #pragma unroll
-      for (int w = 1; w < 16; w *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+      for (int w = 1; w < XT; w *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
       const float mn = fmaxf(m[r], mx), base = mn == -INFINITY ? 0.f : mn;
-      const float corr = xex2(m[r] - base);
+      corr[r] = xex2(m[r] - base);
       m[r] = mn;
       float sum = 0.f;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < CT; ++c) {
         s[r][c] = xex2(s[r][c] - base);
         sum += s[r][c];
       }
 #pragma unroll
-      for (int w = 1; w < 16; w *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-      l[r] = l[r] * corr + sum;
+      for (int w = 1; w < XT; w *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+      l[r] = l[r] * corr[r] + sum;
       if (drop.thr) {
-        const uint32_t kb = drop.keep8(i, (j0 + tx * 4) >> 3, bh) >> ((tx & 1) * 4);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) s[r][c] = (kb >> c) & 1 ? s[r][c] : 0.f;
+        for (int c = 0; c < CT; c += 4) {
+          const uint32_t kb = drop.keep8(i, (j0 + col(c)) >> 3, bh) >> ((tx & 1) * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[r][c + e] = (kb >> e) & 1 ? s[r][c + e] : 0.f;
+        }
       }
+    }
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) acc[r][c] *= corr;
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) pt[(tx * 4 + c) * C::SQ + ty * 8 + r] = s[r][c];
+      for (int c = 0; c < CO; ++c) acc[r][c] = mul2(acc[r][c], f2(corr[2 * r], corr[2 * r + 1]));
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      float* dst = pt + col(c) * C::BM;
+      *reinterpret_cast<float4*>(dst + ((ty * 2) ^ (tx & 7)) * 4) = make_float4(s[0][c], s[1][c], s[2][c], s[3][c]);
+      *reinterpret_cast<float4*>(dst + ((ty * 2 + 1) ^ (tx & 7)) * 4) = make_float4(s[4][c], s[5][c], s[6][c], s[7][c]);
     }
     __syncthreads();
-#pragma unroll 2
+#pragma unroll 4
     for (int j = 0; j < C::BN; ++j) {
-      const float4 a0 = *reinterpret_cast<const float4*>(pt + j * C::SQ + ty * 8);
-      const float4 a1 = *reinterpret_cast<const float4*>(pt + j * C::SQ + ty * 8 + 4);
-      const float a[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+      const int w = (j >> 2) & 7;
+      const ulonglong2 a0 = *reinterpret_cast<const ulonglong2*>(pt + j * C::BM + ((ty * 2) ^ w) * 4);
+      const ulonglong2 a1 = *reinterpret_cast<const ulonglong2*>(pt + j * C::BM + ((ty * 2 + 1) ^ w) * 4);
+      const uint64_t a[4] = {a0.x, a0.y, a1.x, a1.y};
 #pragma unroll
-      for (int c = 0; c < DP / 64; ++c) {
-        const float4 v4 = *reinterpret_cast<const float4*>(kv + j * DP + c * 64 + tx * 4);
+      for (int c = 0; c < CO; c += 4) {
+        const float4 v4 = *reinterpret_cast<const float4*>(kv + j * DP + col(c));
+        const uint64_t v[4] = {f2(v4.x, v4.x), f2(v4.y, v4.y), f2(v4.z, v4.z), f2(v4.w, v4.w)};
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          acc[r][c * 4 + 0] = fmaf(a[r], v4.x, acc[r][c * 4 + 0]);
-          acc[r][c * 4 + 1] = fmaf(a[r], v4.y, acc[r][c * 4 + 1]);
-          acc[r][c * 4 + 2] = fmaf(a[r], v4.z, acc[r][c * 4 + 2]);
-          acc[r][c * 4 + 3] = fmaf(a[r], v4.w, acc[r][c * 4 + 3]);
-        }
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[r][c + e] = fma2(a[r], v[e], acc[r][c + e]);
       }
     }
   }
@@ -187,13 +239,20 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_fwd_kernel(const XPar
   for (int r = 0; r < 8; ++r) {
     const int i = i0 + ty * 8 + r;
     if (i >= p.Nq) continue;
+    float out[CO];
+#pragma unroll
+    for (int c = 0; c < CO; ++c) {
+      float a, d;
+      unf2(acc[r / 2][c], a, d);
+      out[c] = r & 1 ? d : a;
+    }
     const long long row = (long long)bh * p.Nq + i;
     if (p.splits > 1) {
       const long long at = (long long)split * p.B * p.H * p.Nq + row;
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) {
-        const int d = (c / 4) * 64 + tx * 4 + c % 4;
-        if (d < p.D) p.part_o[at * p.D + d] = acc[r][c];
+      for (int c = 0; c < CO; ++c) {
+        const int d = col(c);
+        if (d < p.D) p.part_o[at * p.D + d] = out[c];
       }
       if (tx == 0) {
         p.part_ml[at * 2] = m[r];
@@ -203,9 +262,9 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_fwd_kernel(const XPar
       const float inv = l[r] == 0.f ? 0.f : (drop.thr ? drop.scale : 1.f) / l[r];
       float* O = reinterpret_cast<float*>(p.o.p) + b * p.o.s[0] + h * p.o.s[1] + i * p.o.s[2];
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) {
-        const int d = (c / 4) * 64 + tx * 4 + c % 4;
-        if (d < p.D) O[d] = acc[r][c] * inv;
+      for (int c = 0; c < CO; ++c) {
+        const int d = col(c);
+        if (d < p.D) O[d] = out[c] * inv;
       }
       if (tx == 0 && p.stats) p.stats[row] = row_stats(m[r], l[r]);
     }
@@ -262,12 +321,12 @@ __global__ void __launch_bounds__(256) xattn_delta_kernel(const XParams p) {
 template <int DP>
 struct SimtBwd {
   static constexpr int TK = DP <= 128 ? 64 : 32, KT = TK / 16, BQ = 64, SK = TK + 4, SQ = BQ + 4;
-  static constexpr int FLOATS = 2 * DP * SK + 2 * DP * SQ + 2 * TK * SQ + 256 + TK + 3 * BQ;
+  static constexpr int FLOATS = 2 * DP * SK + 2 * DP * SQ + 2 * TK * BQ + 256 + TK + 3 * BQ;
   static constexpr int SMEM = FLOATS * 4;
 };
 
 template <int DP>
-__global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_keys_kernel(const XParams p) {
+__global__ void __launch_bounds__(kSimtThreads, DP == 64 ? 2 : 1) xattn_simt_bwd_keys_kernel(const XParams p) {
   using C = SimtBwd<DP>;
   constexpr int KT = C::KT, NC = DP / 16;
   extern __shared__ float4 simt_smem[];
@@ -276,8 +335,8 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_keys_kernel(const
   float* qt = vt + DP * C::SK;
   float* gt = qt + DP * C::SQ;
   float* pt = gt + DP * C::SQ;
-  float* st = pt + C::TK * C::SQ;
-  float* tab = st + C::TK * C::SQ;
+  float* st = pt + C::TK * C::BQ;
+  float* tab = st + C::TK * C::BQ;
   float* live = tab + 256;
   float* mx = live + C::TK;
   float* inv = mx + C::BQ;
@@ -288,20 +347,27 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_keys_kernel(const
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   const int n = key_count(p, b);
   const AttnDrop drop = attn_drop(p.rng, p.drop_thr, p.drop_scale);
-  float ak[KT][NC], av[KT][NC];
+  uint64_t ak[KT][NC], av[KT][NC];  // sums over even and odd queries
 #pragma unroll
   for (int x = 0; x < KT; ++x)
 #pragma unroll
-    for (int c = 0; c < NC; ++c) ak[x][c] = av[x][c] = 0.f;
+    for (int c = 0; c < NC; ++c) ak[x][c] = av[x][c] = 0;
 
   if (j0 < n) {
     if (threadIdx.x < C::TK) live[threadIdx.x] = key_live(p, b, j0 + threadIdx.x, n) ? 0.f : -INFINITY;
     __syncthreads();
     const float* K = reinterpret_cast<const float*>(p.k.p) + b * p.k.s[0] + kh * p.k.s[1] + (long long)j0 * p.k.s[2];
     const float* V = reinterpret_cast<const float*>(p.v.p) + b * p.v.s[0] + kh * p.v.s[1] + (long long)j0 * p.v.s[2];
-    simt_load_t<C::TK, DP, C::SK>(kt, K, p.k.s[2], n - j0, p.D, simt_vec(p.k, p.D), live);
-    simt_load_t<C::TK, DP, C::SK>(vt, V, p.v.s[2], n - j0, p.D, simt_vec(p.v, p.D), live);
+    {
+      SimtTile<C::TK, DP> x;
+      const auto ok = [&](int r) { return live[r] == 0.f; };
+      x.template get<true>(K, p.k.s[2], p.D, simt_vec(p.k, p.D), ok);
+      x.template put_t<C::SK>(kt);
+      x.template get<true>(V, p.v.s[2], p.D, simt_vec(p.v, p.D), ok);
+      x.template put_t<C::SK>(vt);
+    }
     const int nqt = (p.Nq + C::BQ - 1) / C::BQ;
+    const bool vq = simt_vec(p.q, p.D), vg = simt_vec(p.dout, p.D);
     for (int it = 0; it < nqt * p.G; ++it) {
       const int h = kh * p.G + it / nqt, i0 = (it % nqt) * C::BQ, bh = b * p.H + h;
       const float* Q = reinterpret_cast<const float*>(p.q.p) + b * p.q.s[0] + h * p.q.s[1] + (long long)i0 * p.q.s[2];
@@ -315,30 +381,48 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_keys_kernel(const
         inv[threadIdx.x] = st.y;
         del[threadIdx.x] = i < p.Nq ? p.delta[(long long)bh * p.Nq + i] : 0.f;
       }
-      simt_load_t<C::BQ, DP, C::SQ>(qt, Q, p.q.s[2], p.Nq - i0, p.D, simt_vec(p.q, p.D), nullptr);
-      simt_load_t<C::BQ, DP, C::SQ>(gt, G, p.dout.s[2], p.Nq - i0, p.D, simt_vec(p.dout, p.D), nullptr);
+      {
+        SimtTile<C::BQ, DP> x, y;
+        const auto ok = [&](int r) { return i0 + r < p.Nq; };
+        x.template get<true>(Q, p.q.s[2], p.D, vq, ok);
+        y.template get<true>(G, p.dout.s[2], p.D, vg, ok);
+        x.template put_t<C::SQ>(qt);
+        y.template put_t<C::SQ>(gt);
+      }
       __syncthreads();
-      float s[4][KT] = {}, dp[4][KT] = {};
+      uint64_t s2[2][KT] = {}, dp2[2][KT] = {};  // pairs of queries
 #pragma unroll 4
       for (int d = 0; d < DP; ++d) {
-        const float4 q4 = *reinterpret_cast<const float4*>(qt + d * C::SQ + ty * 4);
-        const float4 g4 = *reinterpret_cast<const float4*>(gt + d * C::SQ + ty * 4);
-        const float a[4] = {q4.x, q4.y, q4.z, q4.w}, g[4] = {g4.x, g4.y, g4.z, g4.w};
+        const ulonglong2 q2 = *reinterpret_cast<const ulonglong2*>(qt + d * C::SQ + ty * 4);
+        const ulonglong2 g2 = *reinterpret_cast<const ulonglong2*>(gt + d * C::SQ + ty * 4);
         float kk[KT], vv[KT];
-#pragma unroll
-        for (int c = 0; c < KT; c += 2) {
-          const float2 k2 = *reinterpret_cast<const float2*>(kt + d * C::SK + tx * KT + c);
-          const float2 v2 = *reinterpret_cast<const float2*>(vt + d * C::SK + tx * KT + c);
-          kk[c] = k2.x, kk[c + 1] = k2.y, vv[c] = v2.x, vv[c + 1] = v2.y;
+        if constexpr (KT == 4) {
+          const float4 k4 = *reinterpret_cast<const float4*>(kt + d * C::SK + tx * 4);
+          const float4 v4 = *reinterpret_cast<const float4*>(vt + d * C::SK + tx * 4);
+          kk[0] = k4.x, kk[1] = k4.y, kk[2] = k4.z, kk[3] = k4.w;
+          vv[0] = v4.x, vv[1] = v4.y, vv[2] = v4.z, vv[3] = v4.w;
+        } else {
+          const float2 k2 = *reinterpret_cast<const float2*>(kt + d * C::SK + tx * 2);
+          const float2 v2 = *reinterpret_cast<const float2*>(vt + d * C::SK + tx * 2);
+          kk[0] = k2.x, kk[1] = k2.y, vv[0] = v2.x, vv[1] = v2.y;
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int c = 0; c < KT; ++c) {
-            s[r][c] = fmaf(a[r], kk[c], s[r][c]);
-            dp[r][c] = fmaf(g[r], vv[c], dp[r][c]);
-          }
+        for (int c = 0; c < KT; ++c) {
+          const uint64_t k2 = f2(kk[c], kk[c]), v2 = f2(vv[c], vv[c]);
+          s2[0][c] = fma2(q2.x, k2, s2[0][c]);
+          s2[1][c] = fma2(q2.y, k2, s2[1][c]);
+          dp2[0][c] = fma2(g2.x, v2, dp2[0][c]);
+          dp2[1][c] = fma2(g2.y, v2, dp2[1][c]);
+        }
       }
+      float s[4][KT], dp[4][KT];
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int c = 0; c < KT; ++c) {
+          unf2(s2[r][c], s[2 * r][c], s[2 * r + 1][c]);
+          unf2(dp2[r][c], dp[2 * r][c], dp[2 * r + 1][c]);
+        }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = i0 + ty * 4 + r;
@@ -360,33 +444,38 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_keys_kernel(const
           dp[r][c] = live[tx * KT + c] == 0.f ? pr * (g - dl) : 0.f;
         }
       }
-      float* ds = reinterpret_cast<float*>(p.ds) + (long long)(ul * p.G + it / nqt) * p.nkp * p.nqp +
-                  ((long long)(j0 / 64) * (p.nqp / 8) + (i0 + ty * 4) / 8) * 512 + (ty & 1) * 4;
 #pragma unroll
       for (int c = 0; c < KT; ++c) {
-        const float4 a4 = make_float4(s[0][c], s[1][c], s[2][c], s[3][c]);
-        const float4 d4 = make_float4(dp[0][c], dp[1][c], dp[2][c], dp[3][c]);
-        *reinterpret_cast<float4*>(pt + (tx * KT + c) * C::SQ + ty * 4) = a4;
-        *reinterpret_cast<float4*>(st + (tx * KT + c) * C::SQ + ty * 4) = d4;
-        *reinterpret_cast<float4*>(ds + (j0 % 64 + tx * KT + c) * 8) = d4;
+        const int at = (tx * KT + c) * C::BQ + (ty ^ (tx & 7)) * 4;
+        *reinterpret_cast<float4*>(pt + at) = make_float4(s[0][c], s[1][c], s[2][c], s[3][c]);
+        *reinterpret_cast<float4*>(st + at) = make_float4(dp[0][c], dp[1][c], dp[2][c], dp[3][c]);
       }
       __syncthreads();
+      float* ds = reinterpret_cast<float*>(p.ds) + (long long)(ul * p.G + it / nqt) * p.nkp * p.nqp +
+                  ((long long)(j0 / 64) * (p.nqp / 8) + i0 / 8) * 512 + j0 % 64 * 8;
 #pragma unroll 2
-      for (int r = 0; r < C::BQ; r += 4) {
-        float4 pp[KT], ss[KT];
+      for (int x = threadIdx.x; x < C::TK * 16; x += kSimtThreads) {  // granules of 8 queries, keys side by side
+        const int g = x / (2 * C::TK), key = x / 2 % C::TK, half = x % 2;
+        *reinterpret_cast<float4*>(ds + g * 512 + key * 8 + half * 4) =
+            *reinterpret_cast<const float4*>(st + key * C::BQ + ((2 * g + half) ^ (key / KT & 7)) * 4);
+      }
+#pragma unroll 2
+      for (int r = 0; r < C::BQ / 4; ++r) {
+        ulonglong2 pp[KT], ss[KT];
 #pragma unroll
         for (int x = 0; x < KT; ++x) {
-          pp[x] = *reinterpret_cast<const float4*>(pt + (ty * KT + x) * C::SQ + r);
-          ss[x] = *reinterpret_cast<const float4*>(st + (ty * KT + x) * C::SQ + r);
+          const int at = (ty * KT + x) * C::BQ + (r ^ (ty & 7)) * 4;
+          pp[x] = *reinterpret_cast<const ulonglong2*>(pt + at);
+          ss[x] = *reinterpret_cast<const ulonglong2*>(st + at);
         }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          const float4 g4 = *reinterpret_cast<const float4*>(gt + (tx + 16 * c) * C::SQ + r);
-          const float4 q4 = *reinterpret_cast<const float4*>(qt + (tx + 16 * c) * C::SQ + r);
+          const ulonglong2 g2 = *reinterpret_cast<const ulonglong2*>(gt + (tx + 16 * c) * C::SQ + r * 4);
+          const ulonglong2 q2 = *reinterpret_cast<const ulonglong2*>(qt + (tx + 16 * c) * C::SQ + r * 4);
 #pragma unroll
           for (int x = 0; x < KT; ++x) {
-            av[x][c] = fmaf(pp[x].x, g4.x, fmaf(pp[x].y, g4.y, fmaf(pp[x].z, g4.z, fmaf(pp[x].w, g4.w, av[x][c]))));
-            ak[x][c] = fmaf(ss[x].x, q4.x, fmaf(ss[x].y, q4.y, fmaf(ss[x].z, q4.z, fmaf(ss[x].w, q4.w, ak[x][c]))));
+            av[x][c] = fma2(pp[x].x, g2.x, fma2(pp[x].y, g2.y, av[x][c]));
+            ak[x][c] = fma2(ss[x].x, q2.x, fma2(ss[x].y, q2.y, ak[x][c]));
           }
         }
       }
@@ -402,8 +491,11 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_keys_kernel(const
     for (int c = 0; c < NC; ++c) {
       const int d = tx + 16 * c;
       if (d < p.D) {
-        dK[d] = ak[x][c] * p.scale;
-        dV[d] = av[x][c];
+        float e, o;
+        unf2(ak[x][c], e, o);
+        dK[d] = (e + o) * p.scale;
+        unf2(av[x][c], e, o);
+        dV[d] = e + o;
       }
     }
   }
@@ -415,7 +507,7 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_keys_kernel(const
 template <int DP>
 struct SimtDq {
   static constexpr int BQ = 64, BK = 32;
-  static constexpr int SMEM = (BK * BQ + BK * DP + BK) * 4;
+  static constexpr int SMEM = (BK * BQ + BK * DP) * 4;
 };
 
 template <int DP>
@@ -424,22 +516,21 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_dq_kernel(const X
   extern __shared__ float4 simt_smem[];
   float* ds = reinterpret_cast<float*>(simt_smem);
   float* kn = ds + C::BK * C::BQ;
-  float* live = kn + C::BK * DP;
   const int nqt = (p.Nq + C::BQ - 1) / C::BQ;
   const int i0 = (blockIdx.x % nqt) * C::BQ, ul = blockIdx.x / nqt;  // ul: local (unit, head of the group)
   const int unit = p.u0 + ul / p.G, b = unit / p.Hkv, kh = unit % p.Hkv, h = kh * p.G + ul % p.G;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   const int n = key_count(p, b);
+  const bool vk = simt_vec(p.k, p.D);
   const float* K = reinterpret_cast<const float*>(p.k.p) + b * p.k.s[0] + kh * p.k.s[1];
   const float* S = reinterpret_cast<const float*>(p.ds) + (long long)ul * p.nkp * p.nqp;
-  float acc[4][DP / 16];
+  uint64_t acc[2][DP / 16];  // pairs of queries
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+  for (int r = 0; r < 2; ++r)
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) acc[r][c] = 0.f;
+    for (int c = 0; c < DP / 16; ++c) acc[r][c] = 0;
   for (int j0 = 0; j0 < n; j0 += C::BK) {
     __syncthreads();
-    if (threadIdx.x < C::BK) live[threadIdx.x] = key_live(p, b, j0 + threadIdx.x, n) ? 0.f : -INFINITY;
     for (int x = threadIdx.x; x < C::BK * C::BQ / 4; x += kSimtThreads) {
       const int r = x / (C::BQ / 4), c = (x % (C::BQ / 4)) * 4;
       *reinterpret_cast<float4*>(ds + r * C::BQ + c) =
@@ -447,22 +538,23 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_dq_kernel(const X
                            S + ((long long)((j0 + r) / 64) * (p.nqp / 8) + (i0 + c) / 8) * 512 + (j0 + r) % 64 * 8 + c % 8)
                      : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    __syncthreads();
-    simt_load_n<C::BK, DP>(kn, K + (long long)j0 * p.k.s[2], p.k.s[2], n - j0, p.D, simt_vec(p.k, p.D), live);
+    {
+      SimtTile<C::BK, DP> x;
+      x.template get<false>(K + (long long)j0 * p.k.s[2], p.k.s[2], p.D, vk, [&](int r) { return key_live(p, b, j0 + r, n); });
+      x.put_n(kn);
+    }
     __syncthreads();
 #pragma unroll 4
     for (int j = 0; j < C::BK; ++j) {
-      const float4 a4 = *reinterpret_cast<const float4*>(ds + j * C::BQ + ty * 4);
-      const float a[4] = {a4.x, a4.y, a4.z, a4.w};
+      const ulonglong2 a2 = *reinterpret_cast<const ulonglong2*>(ds + j * C::BQ + ty * 4);
 #pragma unroll
       for (int c = 0; c < DP / 64; ++c) {
         const float4 k4 = *reinterpret_cast<const float4*>(kn + j * DP + c * 64 + tx * 4);
+        const uint64_t k[4] = {f2(k4.x, k4.x), f2(k4.y, k4.y), f2(k4.z, k4.z), f2(k4.w, k4.w)};
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          acc[r][c * 4 + 0] = fmaf(a[r], k4.x, acc[r][c * 4 + 0]);
-          acc[r][c * 4 + 1] = fmaf(a[r], k4.y, acc[r][c * 4 + 1]);
-          acc[r][c * 4 + 2] = fmaf(a[r], k4.z, acc[r][c * 4 + 2]);
-          acc[r][c * 4 + 3] = fmaf(a[r], k4.w, acc[r][c * 4 + 3]);
+        for (int e = 0; e < 4; ++e) {
+          acc[0][c * 4 + e] = fma2(a2.x, k[e], acc[0][c * 4 + e]);
+          acc[1][c * 4 + e] = fma2(a2.y, k[e], acc[1][c * 4 + e]);
         }
       }
     }
@@ -475,7 +567,9 @@ __global__ void __launch_bounds__(kSimtThreads) xattn_simt_bwd_dq_kernel(const X
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
       const int d = (c / 4) * 64 + tx * 4 + c % 4;
-      if (d < p.D) dQ[d] = acc[r][c] * p.scale;
+      float e, o;
+      unf2(acc[r / 2][c], e, o);
+      if (d < p.D) dQ[d] = (r & 1 ? o : e) * p.scale;
     }
   }
 }
