@@ -49,10 +49,10 @@ __device__ __forceinline__ bool named_any(int id, int threads, bool yes) {
   return r != 0;
 }
 
-// The bias of the two pairs whose byte offsets `w` holds, from the table at `off` in shared memory.
+// The bias of the pair with byte offset `id`, from the table at `off` in shared memory.
+__device__ __forceinline__ float table_at(int off, uint32_t id) { return *reinterpret_cast<const float*>(xsmem + off + id); }
 __device__ __forceinline__ uint64_t table_pair(int off, uint32_t w) {
-  return f2(*reinterpret_cast<const float*>(xsmem + off + (w & 0xFFFF)),
-            *reinterpret_cast<const float*>(xsmem + off + (w >> 16)));
+  return f2(table_at(off, w & 0xFFFF), table_at(off, w >> 16));
 }
 
 // NKB regions of `rows` x 128 bytes.
@@ -273,7 +273,6 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
     const uint4* idrow = reinterpret_cast<const uint4*>(p.idsQ) +
                          ((long long)((i < p.nqp ? i : i - 64) / 64) * (p.nkp / 8) + c0 * 8 + wg * 4) * 64 + i % 64;
     float* xrow = reinterpret_cast<float*>(xsmem + C::OFF_ROW);
-    const uint64_t sc2 = f2(p.scale_log2, p.scale_log2);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     // this thread's 32 ids and this lane's key of the next chunk, fetched a chunk ahead
@@ -293,37 +292,26 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
       const uint32_t sbuf = lanes + C::TM_S + (c % NSB) * 64 + wg * 32;
       if (ok) ok = warp_wait(&bar_s[c % NSB], (c / NSB) & 1, ctx);
       tc_fence_after();
-      uint64_t x[16];
+      float x[32];
       float mx = -INFINITY;
       if (ok && any_row) {
-        uint32_t s[32];
-        tmem_ld32_issue(sbuf, s);
-        tmem_wait32(s);
+        tmem_ld32(sbuf, x);
+        if (BIAS) {
+          const uint32_t* w = reinterpret_cast<const uint32_t*>(id);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float a = __uint_as_float(s[2 * e]), d = __uint_as_float(s[2 * e + 1]);
-          x[e] = f2(a, d);
-          if (BIAS) x[e] = fma2(x[e], sc2, table_pair(C::OFF_TAB, reinterpret_cast<const uint32_t*>(id)[e]));
+          for (int e = 0; e < 32; ++e) x[e] = fmaf(x[e], p.scale_log2, table_at(C::OFF_TAB, e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xFFFF));
         }
         if (live != ~0u) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float a, d;
-            unf2(x[e], a, d);
-            x[e] = f2((live >> (2 * e)) & 1 ? a : -INFINITY, (live >> (2 * e + 1)) & 1 ? d : -INFINITY);
-          }
+          for (int e = 0; e < 32; ++e) x[e] = (live >> e) & 1 ? x[e] : -INFINITY;
         }
         float y[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float a, d, g, f;
-          unf2(x[e], a, d);
-          unf2(x[e + 4], g, f);
-          y[e] = max3(fmaxf(a, d), g, f);
-          unf2(x[e + 8], a, d);
-          y[e] = max3(y[e], a, d);
-          unf2(x[e + 12], a, d);
-          y[e] = max3(y[e], a, d);
+          y[e] = max3(x[e], x[e + 4], x[e + 8]);
+          y[e] = max3(y[e], x[e + 12], x[e + 16]);
+          y[e] = max3(y[e], x[e + 20], x[e + 24]);
+          y[e] = fmaxf(y[e], x[e + 28]);
         }
         mx = fmaxf(max3(y[0], y[1], y[2]), y[3]);
         if (!BIAS) mx *= p.scale_log2;  // x is still the raw product (scale > 0: the order and -inf stay)
@@ -355,19 +343,17 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
       }
       if (ok && any_row) {
         const float base = m == -INFINITY ? 0.f : m;
-        const uint64_t nb2 = f2(-base, -base);
-        uint64_t sum[2] = {0, 0};  // two pairs of zeros
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
         uint32_t w[16];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint64_t t = BIAS ? add2(x[4 * g + e], nb2) : fma2(x[4 * g + e], sc2, nb2);
-            float a, d;
-            unf2(t, a, d);
-            a = xex2(a), d = xex2(d);
-            sum[e & 1] = add2(sum[e & 1], f2(a, d));
-            w[g * 4 + e] = pack_bf16(a, d);
+          for (int e = 0; e < 8; e += 2) {
+            float a = x[8 * g + e], d = x[8 * g + e + 1];
+            a = xex2(BIAS ? a - base : fmaf(a, p.scale_log2, -base));
+            d = xex2(BIAS ? d - base : fmaf(d, p.scale_log2, -base));
+            sum[e & 2] += a, sum[(e & 2) + 1] += d;
+            w[g * 4 + e / 2] = pack_bf16(a, d);
           }
           if (DROP) {
             const uint4 u = drop.words(i, (j0 >> 3) + g, bh);
@@ -378,9 +364,7 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
           }
         }
         tmem_st16(sbuf, w);
-        float a, d;
-        unf2(add2(sum[0], sum[1]), a, d);
-        l += a + d;
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         tmem_wait_st();
       }
       if (live != ~0u) {  // what absent keys hold must not reach the product: 0 * NaN
