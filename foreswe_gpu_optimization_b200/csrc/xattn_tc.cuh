@@ -149,8 +149,8 @@ __device__ __forceinline__ bool vec_rows(const XTensor& t) {
 //   2 warpgroups   P(c) = 2^(t - m): thread r of warpgroup w has row r and keys 32 w .. 32 w + 31 of the chunk; P goes
 //                  in bf16 over the scores it came from
 // m is one per row and moves only when a chunk would pass it by more than kLazy (P stays below 2^kLazy; l and O are
-// fp32): one barrier per chunk tells both warpgroups whether any row has to move, and only then do they exchange their
-// maxima and rescale O, after O's product c - 1 (the only one that can be in flight: S(c) was issued after c - 2).
+// fp32): one barrier per chunk tells the two warps of 32 rows whether any of them has to move, and only then do they
+// exchange their maxima and rescale O, after O's product c - 1 (the only one that can be in flight: S(c) was issued after c - 2).
 // Few queries of heads that share a key head (G * Nq <= 128) are packed into one tile's rows.
 // DP = 192 has room for one score buffer and one chunk of K and V; S(c + 1) then follows O's product c.
 // ---------------------------------------------------------------------------------------------------------------
@@ -317,9 +317,9 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
         if (!BIAS) mx *= p.scale_log2;  // x is still the raw product (scale > 0: the order and -inf stay)
       }
       if (c + 1 < nc) fetch(c + 1);
-      if (named_any(1, C::EWT, row && (mx > m + kLazy || (m == -INFINITY && mx > m)))) {
+      if (named_any(1 + (warp & 3), 64, row && (mx > m + kLazy || (m == -INFINITY && mx > m)))) {
         xrow[wg * 128 + r] = mx;
-        named_sync(2, C::EWT);
+        named_sync(1 + (warp & 3), 64);
         const float top = fmaxf(mx, xrow[(wg ^ 1) * 128 + r]);
         const bool grow = top > m + kLazy || (m == -INFINITY && top > m);
         const float f = grow ? xex2(m - top) : 1.f;
@@ -379,9 +379,9 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
     }
     if (ok && nc > 0) ok = warp_wait(&bar_pv[(nc - 1) & 1], ((nc - 1) >> 1) & 1, ctx);
     tc_fence_after();
-    named_sync(2, C::EWT);  // the last exchange has been read
+    named_sync(1 + (warp & 3), 64);  // the last exchange has been read
     xrow[wg * 128 + r] = l;
-    named_sync(2, C::EWT);
+    named_sync(1 + (warp & 3), 64);
     l += xrow[(wg ^ 1) * 128 + r];
     const long long stat = (long long)bh * p.Nq + i;
     const long long part = (long long)split * p.B * p.H * p.Nq + stat;
@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
     }
     if (tma) {
       fence_proxy_async_smem();
-      named_sync(2, C::EWT);
+      named_sync(5, C::EWT);
       if (threadIdx.x == 0 && ok) {
         if (pack) store_tile<DP>(&maps.o, xsmem, p.D, 0, kh * p.G, b);
         else store_tile<DP>(&maps.o, xsmem, p.D, qt * 128, hx, b);
