@@ -271,47 +271,81 @@ __global__ void __launch_bounds__(SimtFwd<DP>::NT, DP == 64 ? 2 : 1) xattn_simt_
   }
 }
 
-// Join the key splits of each row: one warp per row.
+// Join the key splits of each row: one warp per row. The splits' weights are worked out by the lanes side by side (32 at
+// a time) and handed round; a lane sums 4 consecutive columns.
 template <class E>
 __global__ void __launch_bounds__(256) xattn_combine_kernel(const XParams p) {
   const long long rows = (long long)p.B * p.H * p.Nq;
   const long long row = (long long)blockIdx.x * 8 + threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
   if (row >= rows) return;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row;
   float m = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[(s * rows + row) * 2]);
+  for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, ml[s * rows].x);
+#pragma unroll
+  for (int w = 16; w; w /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
   const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float* ml = p.part_ml + (s * rows + row) * 2;
-    l += ml[1] * xex2(ml[0] - base);
-  }
-  const float inv = l == 0.f ? 0.f : (p.drop_thr ? p.drop_scale : 1.f) / l;
   const int i = (int)(row % p.Nq), bh = (int)(row / p.Nq), h = bh % p.H, b = bh / p.H;
   E* O = reinterpret_cast<E*>(p.o.p) + b * p.o.s[0] + h * p.o.s[1] + i * p.o.s[2];
-  for (int d = lane; d < p.D; d += 32) {
-    float x = 0.f;
-    for (int s = 0; s < p.splits; ++s)
-      x += p.part_o[(s * rows + row) * p.D + d] * xex2(p.part_ml[(s * rows + row) * 2] - base);
-    O[d] = from_f<E>(x * inv);
+  const bool vec = p.D % 4 == 0;
+  float l = 0.f;
+  for (int d0 = 0; d0 < p.D; d0 += 128) {
+    const int d = d0 + lane * 4;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < p.splits; s0 += 32) {
+      const float2 mine = s0 + lane < p.splits ? ml[(s0 + lane) * rows] : make_float2(-INFINITY, 0.f);
+      const float weight = xex2(mine.x - base);
+      if (d0 == 0) l += mine.y * weight;
+      const int n = p.splits - s0 < 32 ? p.splits - s0 : 32;
+#pragma unroll 4
+      for (int s = 0; s < n; ++s) {
+        const float w = __shfl_sync(0xffffffffu, weight, s);
+        const float* src = p.part_o + ((s0 + s) * rows + row) * p.D + d;
+        if (vec && d < p.D) {
+          const float4 v = *reinterpret_cast<const float4*>(src);
+          x[0] = fmaf(v.x, w, x[0]), x[1] = fmaf(v.y, w, x[1]), x[2] = fmaf(v.z, w, x[2]), x[3] = fmaf(v.w, w, x[3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (d + e < p.D) x[e] = fmaf(src[e], w, x[e]);
+        }
+      }
+    }
+    if (d0 == 0) {
+#pragma unroll
+      for (int w = 16; w; w /= 2) l += __shfl_xor_sync(0xffffffffu, l, w);
+    }
+    const float inv = l == 0.f ? 0.f : (p.drop_thr ? p.drop_scale : 1.f) / l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (d + e < p.D) O[d + e] = from_f<E>(x[e] * inv);
   }
   if (lane == 0 && p.stats) p.stats[row] = row_stats(m, l);
 }
 
-// delta_i = dO_i . O_i, one warp per row.
+// delta_i = dO_i . O_i: 8 lanes per row, 4 rows per warp.
 __global__ void __launch_bounds__(256) xattn_delta_kernel(const XParams p) {
   const long long rows = (long long)p.B * p.H * p.Nq;
-  const long long row = (long long)blockIdx.x * 8 + threadIdx.x / 32;
-  const int lane = threadIdx.x % 32;
-  if (row >= rows) return;
-  const int i = (int)(row % p.Nq), bh = (int)(row / p.Nq), h = bh % p.H, b = bh / p.H;
-  const float* O = reinterpret_cast<const float*>(p.o.p) + b * p.o.s[0] + h * p.o.s[1] + i * p.o.s[2];
-  const float* G = reinterpret_cast<const float*>(p.dout.p) + b * p.dout.s[0] + h * p.dout.s[1] + i * p.dout.s[2];
+  const long long row = (long long)blockIdx.x * 32 + threadIdx.x / 8;
+  const int lane = threadIdx.x % 8;
   float x = 0.f;
-  for (int d = lane; d < p.D; d += 32) x = fmaf(O[d], G[d], x);
+  if (row < rows) {
+    const int i = (int)(row % p.Nq), bh = (int)(row / p.Nq), h = bh % p.H, b = bh / p.H;
+    const float* O = reinterpret_cast<const float*>(p.o.p) + b * p.o.s[0] + h * p.o.s[1] + i * p.o.s[2];
+    const float* G = reinterpret_cast<const float*>(p.dout.p) + b * p.dout.s[0] + h * p.dout.s[1] + i * p.dout.s[2];
+    if (simt_vec(p.o, p.D) && simt_vec(p.dout, p.D)) {
+#pragma unroll 2
+      for (int d = lane * 4; d < p.D; d += 32) {
+        const float4 u = *reinterpret_cast<const float4*>(O + d), v = *reinterpret_cast<const float4*>(G + d);
+        x = fmaf(u.x, v.x, fmaf(u.y, v.y, fmaf(u.z, v.z, fmaf(u.w, v.w, x))));
+      }
+    } else {
+      for (int d = lane; d < p.D; d += 8) x = fmaf(O[d], G[d], x);
+    }
+  }
 #pragma unroll
-  for (int w = 16; w; w /= 2) x += __shfl_xor_sync(0xffffffffu, x, w);
-  if (lane == 0) p.delta[row] = x;
+  for (int w = 4; w; w /= 2) x += __shfl_xor_sync(0xffffffffu, x, w);
+  if (lane == 0 && row < rows) p.delta[row] = x;
 }
 
 // ---------------------------------------------------------------------------------------------------------------

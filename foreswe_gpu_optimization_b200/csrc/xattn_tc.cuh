@@ -442,60 +442,58 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
 // ---------------------------------------------------------------------------------------------------------------
 template <int LPR>  // lanes per row: 8 columns each
 __global__ void __launch_bounds__(256) xattn_records_kernel(const XParams p, int heads_first) {
-  constexpr int RPW = 32 / LPR, UNROLL = 4;  // rows per warp and step, steps in flight
-  const int lane = threadIdx.x % 32, sub = lane / LPR, c = (lane % LPR) * 8;
-  const uint32_t total = (uint32_t)p.H * p.nqp;  // rows of a batch entry (< 2^31)
-  const uint32_t x0 = (blockIdx.x * 8 + threadIdx.x / 32) * (RPW * UNROLL);
-  const int b = blockIdx.y;
+  constexpr int ROWS = 256 / LPR;  // rows of a step
+  __shared__ float delta[256];
+  // 256 rows: 16 rows of 16 heads, head by head in memory, or 256 rows of one head
+  const int HB = heads_first ? 16 : 1, IB = 256 / HB;
+  const int b = blockIdx.z, h0 = blockIdx.y * HB, i0 = blockIdx.x * IB;
+  const int sub = threadIdx.x / LPR, c = threadIdx.x % LPR * 8;
   const bool vec = vec_rows(p.o) && vec_rows(p.dout);
-  uint4 a[UNROLL], g[UNROLL];
-  int ri[UNROLL], rbh[UNROLL];
+  const __nv_bfloat16* O = reinterpret_cast<const __nv_bfloat16*>(p.o.p) + b * p.o.s[0] + c;
+  const __nv_bfloat16* G = reinterpret_cast<const __nv_bfloat16*>(p.dout.p) + b * p.dout.s[0] + c;
 #pragma unroll
-  for (int u = 0; u < UNROLL; ++u) {
-    const uint32_t x = x0 + u * RPW + sub;
-    a[u] = g[u] = make_uint4(0, 0, 0, 0);
-    ri[u] = -1;
-    if (x >= total) continue;
-    // rows in the order of memory: heads side by side in a row, or rows of one head
-    const uint32_t lo = heads_first ? p.H : p.nqp, hi = x / lo, in = x - hi * lo;
-    const int h = heads_first ? in : hi, i = heads_first ? hi : in;
-    ri[u] = i;
-    rbh[u] = b * p.H + h;
-    if (i >= p.Nq || c >= p.D) continue;
-    const __nv_bfloat16* O =
-        reinterpret_cast<const __nv_bfloat16*>(p.o.p) + b * p.o.s[0] + h * p.o.s[1] + (long long)i * p.o.s[2] + c;
-    const __nv_bfloat16* G = reinterpret_cast<const __nv_bfloat16*>(p.dout.p) + b * p.dout.s[0] + h * p.dout.s[1] +
-                             (long long)i * p.dout.s[2] + c;
-    if (vec && c + 8 <= p.D) {
-      a[u] = *reinterpret_cast<const uint4*>(O);
-      g[u] = *reinterpret_cast<const uint4*>(G);
-    } else {
-      __nv_bfloat16 *av = reinterpret_cast<__nv_bfloat16*>(&a[u]), *gv = reinterpret_cast<__nv_bfloat16*>(&g[u]);
+  for (int s0 = 0; s0 < LPR; s0 += 4) {
+    uint4 a[4], g[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c + e < p.D) av[e] = O[e], gv[e] = G[e];
-    }
-  }
+    for (int u = 0; u < 4; ++u) {
+      const int x = (s0 + u) * ROWS + sub, h = h0 + x % HB, i = i0 + x / HB;
+      a[u] = g[u] = make_uint4(0, 0, 0, 0);
+      if (h >= p.H || i >= p.Nq || c >= p.D) continue;
+      const __nv_bfloat16 *o = O + h * p.o.s[1] + i * p.o.s[2], *d = G + h * p.dout.s[1] + i * p.dout.s[2];
+      if (vec && c + 8 <= p.D) {
+        a[u] = *reinterpret_cast<const uint4*>(o);
+        g[u] = *reinterpret_cast<const uint4*>(d);
+      } else {
+        __nv_bfloat16 *av = reinterpret_cast<__nv_bfloat16*>(&a[u]), *gv = reinterpret_cast<__nv_bfloat16*>(&g[u]);
 #pragma unroll
-  for (int u = 0; u < UNROLL; ++u) {
-    const __nv_bfloat162 *av = reinterpret_cast<const __nv_bfloat162*>(&a[u]),
-                         *gv = reinterpret_cast<const __nv_bfloat162*>(&g[u]);
-    float d = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 s = __bfloat1622float2(av[e]), t = __bfloat1622float2(gv[e]);
-      d = fmaf(s.x, t.x, fmaf(s.y, t.y, d));
+        for (int e = 0; e < 8; ++e)
+          if (c + e < p.D) av[e] = o[e], gv[e] = d[e];
+      }
     }
 #pragma unroll
-    for (int w = LPR / 2; w; w /= 2) d += __shfl_xor_sync(0xffffffffu, d, w);
-    if (lane % LPR || ri[u] < 0) continue;
-    const int i = ri[u];
-    const float2 st = i < p.Nq ? p.stats[(long long)rbh[u] * p.Nq + i] : make_float2(0.f, 0.f);
-    float* rec = p.rec + ((long long)rbh[u] * (p.nqp / 64) + i / 64) * 192 + i % 64;
-    rec[0] = p.ids ? -st.x : st.y == 0.f ? -INFINITY : log2f(st.y) - st.x;
-    rec[64] = st.y;
-    rec[128] = -d;
+    for (int u = 0; u < 4; ++u) {
+      const __nv_bfloat162 *av = reinterpret_cast<const __nv_bfloat162*>(&a[u]),
+                           *gv = reinterpret_cast<const __nv_bfloat162*>(&g[u]);
+      float d = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 s = __bfloat1622float2(av[e]), t = __bfloat1622float2(gv[e]);
+        d = fmaf(s.x, t.x, fmaf(s.y, t.y, d));
+      }
+#pragma unroll
+      for (int w = LPR / 2; w; w /= 2) d += __shfl_xor_sync(0xffffffffu, d, w);
+      if (threadIdx.x % LPR == 0) delta[(s0 + u) * ROWS + sub] = d;
+    }
   }
+  __syncthreads();
+  const int h = h0 + threadIdx.x / IB, i = i0 + threadIdx.x % IB;
+  if (h >= p.H || i >= p.nqp) return;
+  const long long bh = (long long)b * p.H + h;
+  const float2 st = i < p.Nq ? p.stats[bh * p.Nq + i] : make_float2(0.f, 0.f);
+  float* rec = p.rec + (bh * (p.nqp / 64) + i / 64) * 192 + i % 64;
+  rec[0] = p.ids ? -st.x : st.y == 0.f ? -INFINITY : log2f(st.y) - st.x;
+  rec[64] = st.y;
+  rec[128] = -delta[threadIdx.x % IB * HB + threadIdx.x / IB];
 }
 
 // ---------------------------------------------------------------------------------------------------------------
