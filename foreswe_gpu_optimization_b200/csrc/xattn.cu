@@ -31,15 +31,25 @@ struct XDims {
 bool packs_rows(const XDims& d) { return d.bf16 && d.G > 1 && d.T == 0 && (long long)d.G * d.Nq <= 128; }
 
 int forward_splits(const XDims& d) {
-  // Enough key ranges to give every SM a tile when the rows alone do not. Joining them costs a launch of about 4 us, as
-  // much as 4 chunks of 64 keys: below 12 chunks one range is faster (1 x 16 heads, 1 query, 512 keys: 13 against 17 us),
-  // and a range keeps at least 4.
+  // Enough key ranges to give every SM a tile when the rows alone do not.
   const long long tiles = packs_rows(d) ? (long long)d.B * d.Hkv : (long long)((d.Nq + 127) / 128) * d.B * d.H;
   const int ktiles = (d.Nk + 63) / 64;
-  if (tiles >= kSMs || ktiles < 12) return 1;
-  const long long want = (4 * kSMs + tiles - 1) / tiles;
-  const long long most = ktiles / 4;
-  return (int)(want < most ? want : most);
+  if (tiles >= kSMs) return 1;
+  long long want, most;
+  if (d.bf16) {
+    // Joining the ranges costs a launch of about 4 us, as much as 4 chunks of 64 keys: below 12 chunks one range is
+    // faster (1 x 16 heads, 1 query, 512 keys: 13 against 17 us), and a range keeps at least 4. Lengths may differ, so
+    // twice as many ranges as the GPU holds at once.
+    want = (4 * kSMs + tiles - 1) / tiles;
+    most = ktiles < 12 ? 1 : ktiles / 4;
+  } else {
+    // A chunk takes about 12 us on the FMA pipe: one wave of two CTAs per SM, at least two chunks each (8 x 8 heads, 130
+    // queries, 517 keys: 106 against 129 us).
+    want = 2 * kSMs / tiles;
+    most = ktiles / 2;
+  }
+  const long long n = want < most ? want : most;
+  return n < 1 ? 1 : (int)n;
 }
 
 int check_xshape(const GeoXattnShape* s, XDims& d) {
@@ -277,10 +287,12 @@ int records(const XParams& p, const XDims& d, cudaStream_t st) {
 template <int DP>
 int tc_bwd(const xa::XMaps& maps, const XParams& p, int units, cudaStream_t st) {
   using C = xa::KeysCfg<DP>;
-  const long long grid = (long long)((p.Nk + 127) / 128) * units;
+  const long long tiles = (long long)((p.Nk + 127) / 128) * units, grid = tiles < kSMs ? tiles : kSMs;
+  XParams pk = p;
+  pk.tiles = (int)tiles;
   auto keys = p.ids ? (p.drop_thr ? xa::xattn_bwd_keys_kernel<DP, true, true> : xa::xattn_bwd_keys_kernel<DP, true, false>)
                     : (p.drop_thr ? xa::xattn_bwd_keys_kernel<DP, false, true> : xa::xattn_bwd_keys_kernel<DP, false, false>);
-  if (int rc = tc_launch(keys, grid, C::THREADS, C::SMEM, st, maps, p)) return rc;
+  if (int rc = tc_launch(keys, grid, C::THREADS, C::SMEM, st, maps, pk)) return rc;
   return tc_launch(xa::xattn_bwd_dq_kernel<DP>, (long long)((p.Nq + 127) / 128) * units * p.G, xa::DqCfg<DP>::THREADS,
                    xa::DqCfg<DP>::SMEM, st, maps, p);
 }

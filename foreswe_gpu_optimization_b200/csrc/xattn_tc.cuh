@@ -497,8 +497,8 @@ __global__ void __launch_bounds__(256) xattn_records_kernel(const XParams p, int
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Backward, key pass. One CTA per (128 keys, key head, batch); loops over chunks of BQ queries of the heads that share
-// the key head. Scores are formed transposed (keys in the lanes), so that P^T and dS^T are written over them in tensor
+// Backward, key pass. Tiles of (128 keys, key head, batch); loops over chunks of BQ queries of the heads that share the
+// key head. Scores are formed transposed (keys in the lanes), so that P^T and dS^T are written over them in tensor
 // memory as the A operands of
 //   dV += P^T dO,  dK += dS^T Q
 // and a thread owns one key's BQ / 4 queries; dS^T also goes to the scratch for dQ and the table's gradient.
@@ -508,6 +508,10 @@ __global__ void __launch_bounds__(256) xattn_records_kernel(const XParams p, int
 // Bound by the operand feed of the products (S and dP 64 clocks per 16 of the head dim and 128 queries, dV and dK as
 // many per 16 queries at DP = 128): chunks of 128 queries, which halve K's and V's share of it, with one score buffer
 // (S 128, dP 128, dK 128, dV 128 columns) beat chunks of 64 with two. DP = 192 has columns for 64 queries only.
+// One persistent CTA per SM (tensor memory is full): K and V of the next tile are loaded as soon as this one's last
+// scores are formed, and the next tile's first scores run while dK and dV leave. They are staged in the slot of the
+// tile's last chunk, which is refilled only then. (One CTA per tile spent 40 % of its time filling and draining at 512
+// queries.)
 // Dropout: a Philox call covers one query and 8 keys. Each lane makes the calls of 2 or 4 queries for its octet of keys
 // and the 8 x 8 bit blocks are transposed among 8 lanes (3 shuffles), so no call is made twice.
 // ---------------------------------------------------------------------------------------------------------------
@@ -551,28 +555,26 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, 1)
     xattn_bwd_keys_kernel(const __grid_constant__ XMaps maps, const XParams p) {
   using C = KeysCfg<DP>;
   constexpr int NST = C::NST, BQ = C::BQ, QT = C::QT;
-  __shared__ uint64_t bar_k, bar_full[NST], bar_empty[NST], bar_s, bar_dp, bar_p, bar_ds, bar_done;
+  __shared__ uint64_t bar_k, bar_kfree, bar_full[NST], bar_empty[NST], bar_s, bar_dp, bar_p, bar_ds, bar_done, bar_acc,
+      bar_out;
   __shared__ uint32_t tmem_sh;
   __shared__ int abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int nkt = (p.Nk + 127) / 128, kt = blockIdx.x % nkt, ul = blockIdx.x / nkt, unit = p.u0 + ul;
-  const int b = unit / p.Hkv, kh = unit % p.Hkv, j0 = kt * 128;
-  const int n = key_count(p, b);
-  const int nqc = (p.nqp + BQ - 1) / BQ, nc = nqc * p.G;
+  const int nkt = (p.Nk + 127) / 128;
+  const int nqc = (p.nqp + BQ - 1) / BQ, nc = nqc * p.G;  // chunks per head and per tile
   WaitCtx ctx{&abort_flag, p.status};
-  __nv_bfloat16* dK = reinterpret_cast<__nv_bfloat16*>(p.dk.p) + b * p.dk.s[0] + kh * p.dk.s[1];
-  __nv_bfloat16* dV = reinterpret_cast<__nv_bfloat16*>(p.dv.p) + b * p.dv.s[0] + kh * p.dv.s[1];
+  struct Tile {
+    int j0, ul, b, kh, n;
+  };
+  auto tile_of = [&](int t) {
+    Tile x;
+    x.j0 = t % nkt * 128, x.ul = t / nkt;
+    const int unit = p.u0 + x.ul;
+    x.b = unit / p.Hkv, x.kh = unit % p.Hkv;
+    x.n = key_count(p, x.b);
+    return x;
+  };
 
-  if (j0 >= n) {  // no key of this tile exists: zero gradients, and the scratch is not read here
-    for (int x = threadIdx.x; x < 128 * p.D; x += C::THREADS) {
-      const int j = j0 + x / p.D, d = x % p.D;
-      if (j < p.Nk) {
-        dK[(long long)j * p.dk.s[2] + d] = __float2bfloat16_rn(0.f);
-        dV[(long long)j * p.dv.s[2] + d] = __float2bfloat16_rn(0.f);
-      }
-    }
-    return;
-  }
   if (threadIdx.x == 0) {
     abort_flag = 0;
     mbar_init(&bar_k, 1);
@@ -584,7 +586,10 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, 1)
     mbar_init(&bar_dp, 1);
     mbar_init(&bar_p, C::EWT);
     mbar_init(&bar_ds, C::EWT);
+    mbar_init(&bar_kfree, 1);
     mbar_init(&bar_done, 1);
+    mbar_init(&bar_acc, C::EWT);
+    mbar_init(&bar_out, 1);
     fence_barrier_init();
   }
   if (warp == C::MMA_WARP) {
@@ -598,205 +603,256 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, 1)
 
   if (warp == C::TMA_WARP) {
     if (lane == 0) {
-      mbar_arrive_expect_tx(&bar_k, 2 * C::K_BYTES);
-      for (int x = 0; x < 128; x += 64) {  // the maps' boxes hold 64 rows
-        load_rows<DP>(xsmem + x * 128, &maps.k, &bar_k, 128 * 128, j0 + x, kh, b);
-        load_rows<DP>(xsmem + C::OFF_V + x * 128, &maps.v, &bar_k, 128 * 128, j0 + x, kh, b);
-      }
       const int recs = p.nqp / 64;  // blocks of 64 records per head
-      for (int c = 0; c < nc; ++c) {
-        const int st = c % NST, h = kh * p.G + c / nqc, q0 = c % nqc * BQ;
-        // a last chunk of 128 queries may hold 64 padded rows only: no records for the others (`inside` below)
-        const int rec = (p.nqp - q0 < BQ ? 64 : BQ) * 12;
-        if (!mbar_wait(&bar_empty[st], ((c / NST) & 1) ^ 1, ctx)) break;
-        uint8_t* dst = xsmem + C::OFF_ST + st * C::STAGE;
-        mbar_arrive_expect_tx(&bar_full[st], C::STAGE + rec);
-        for (int x = 0; x < BQ; x += 64) {
-          load_rows<DP>(dst + x * 128, &maps.q, &bar_full[st], BQ * 128, q0 + x, h, b);
-          load_rows<DP>(dst + C::Q_BYTES + x * 128, &maps.dout, &bar_full[st], BQ * 128, q0 + x, h, b);
+      int t = 0, g = 0;             // tiles and chunks so far
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x) {
+        const Tile x = tile_of(tile);
+        if (x.j0 >= x.n) continue;  // no key of this tile exists
+        if (!(ok = mbar_wait(&bar_kfree, (t & 1) ^ 1, ctx))) break;
+        mbar_arrive_expect_tx(&bar_k, 2 * C::K_BYTES);
+        for (int y = 0; y < 128; y += 64) {  // the maps' boxes hold 64 rows
+          load_rows<DP>(xsmem + y * 128, &maps.k, &bar_k, 128 * 128, x.j0 + y, x.kh, x.b);
+          load_rows<DP>(xsmem + C::OFF_V + y * 128, &maps.v, &bar_k, 128 * 128, x.j0 + y, x.kh, x.b);
         }
-        bulk_load(xsmem + C::OFF_REC + st * C::REC_BYTES, p.rec + ((long long)(b * p.H + h) * recs + q0 / 64) * 192, rec,
-                  &bar_full[st]);
+        for (int c = 0; c < nc && ok; ++c, ++g) {
+          const int st = g % NST, h = x.kh * p.G + c / nqc, q0 = c % nqc * BQ;
+          // a last chunk of 128 queries may hold 64 padded rows only: no records for the others (`inside` below)
+          const int rec = (p.nqp - q0 < BQ ? 64 : BQ) * 12;
+          if (!(ok = mbar_wait(&bar_empty[st], ((g / NST) & 1) ^ 1, ctx))) break;
+          // The last tile's dK and dV leave through its last chunk's slot, which chunk NST - 1 of this tile takes over.
+          // Not later than this tile's last chunk, so that bar_out cannot run two phases ahead of the wait.
+          if (t > 0 && c == (NST < nc ? NST : nc) - 1 && !(ok = mbar_wait(&bar_out, (t - 1) & 1, ctx))) break;
+          uint8_t* dst = xsmem + C::OFF_ST + st * C::STAGE;
+          mbar_arrive_expect_tx(&bar_full[st], C::STAGE + rec);
+          for (int y = 0; y < BQ; y += 64) {
+            load_rows<DP>(dst + y * 128, &maps.q, &bar_full[st], BQ * 128, q0 + y, h, x.b);
+            load_rows<DP>(dst + C::Q_BYTES + y * 128, &maps.dout, &bar_full[st], BQ * 128, q0 + y, h, x.b);
+          }
+          bulk_load(xsmem + C::OFF_REC + st * C::REC_BYTES, p.rec + ((long long)(x.b * p.H + h) * recs + q0 / 64) * 192,
+                    rec, &bar_full[st]);
+        }
+        ++t;
       }
     }
   } else if (warp == C::MMA_WARP) {
     if (lane == 0) {
-      bool ok = mbar_wait(&bar_k, 0, ctx) && mbar_wait(&bar_full[0], 0, ctx);
-      const uint32_t q0 = sbase + C::OFF_ST;
-      if (ok) {
+      int t = 0, g = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x) {
+        const Tile x = tile_of(tile);
+        if (x.j0 >= x.n) continue;
+        const uint32_t slots = sbase + C::OFF_ST;
+        if (!(ok = mbar_wait(&bar_k, t & 1, ctx) && mbar_wait(&bar_full[g % NST], (g / NST) & 1, ctx))) break;
         tc_fence_after();
-        mma_scores<DP, BQ>(tmem + C::TM_S, sbase, q0);
+        mma_scores<DP, BQ>(tmem + C::TM_S, sbase, slots + g % NST * C::STAGE);
         mma_commit(&bar_s);
-        mma_scores<DP, BQ>(tmem + C::TM_DP, sbase + C::OFF_V, q0 + C::Q_BYTES);
+        mma_scores<DP, BQ>(tmem + C::TM_DP, sbase + C::OFF_V, slots + g % NST * C::STAGE + C::Q_BYTES);
         mma_commit(&bar_dp);
-      }
-      for (int c = 0; c < nc && ok; ++c) {
-        const int st = c % NST, sn = (c + 1) % NST;
-        const uint32_t q = q0 + st * C::STAGE, qn = q0 + sn * C::STAGE;
-        if (!(ok = mbar_wait(&bar_p, c & 1, ctx))) break;
-        tc_fence_after();
-        mma_pieces<DP, BQ, QT>(tmem + C::TM_DV, tmem + C::TM_S, q + C::Q_BYTES, c > 0);
-        if (c + 1 < nc) {
-          if (!(ok = mbar_wait(&bar_full[sn], ((c + 1) / NST) & 1, ctx))) break;
+        if (nc == 1) mma_commit(&bar_kfree);
+        for (int c = 0; c < nc; ++c, ++g) {
+          const int sn = (g + 1) % NST;
+          const uint32_t q = slots + g % NST * C::STAGE, qn = slots + sn * C::STAGE;
+          if (!(ok = mbar_wait(&bar_p, g & 1, ctx))) break;
+          // the last tile's dK and dV have been read
+          if (c == 0 && t > 0 && !(ok = mbar_wait(&bar_acc, (t - 1) & 1, ctx))) break;
           tc_fence_after();
-          mma_scores<DP, BQ>(tmem + C::TM_S, sbase, qn);
-          mma_commit(&bar_s);
+          mma_pieces<DP, BQ, QT>(tmem + C::TM_DV, tmem + C::TM_S, q + C::Q_BYTES, c > 0);
+          if (c + 1 < nc) {
+            if (!(ok = mbar_wait(&bar_full[sn], ((g + 1) / NST) & 1, ctx))) break;
+            tc_fence_after();
+            mma_scores<DP, BQ>(tmem + C::TM_S, sbase, qn);
+            mma_commit(&bar_s);
+          }
+          if (!(ok = mbar_wait(&bar_ds, g & 1, ctx))) break;
+          tc_fence_after();
+          mma_pieces<DP, BQ, QT>(tmem + C::TM_DK, tmem + C::TM_DP, q, c > 0);
+          mma_commit(&bar_empty[g % NST]);
+          if (c + 1 < nc) {
+            mma_scores<DP, BQ>(tmem + C::TM_DP, sbase + C::OFF_V, qn + C::Q_BYTES);
+            mma_commit(&bar_dp);
+            if (c + 2 == nc) mma_commit(&bar_kfree);
+          }
         }
-        if (!(ok = mbar_wait(&bar_ds, c & 1, ctx))) break;
-        tc_fence_after();
-        mma_pieces<DP, BQ, QT>(tmem + C::TM_DK, tmem + C::TM_DP, q, c > 0);
-        mma_commit(&bar_empty[st]);
-        if (c + 1 < nc) {
-          mma_scores<DP, BQ>(tmem + C::TM_DP, sbase + C::OFF_V, qn + C::Q_BYTES);
-          mma_commit(&bar_dp);
-        }
+        if (ok) mma_commit(&bar_done);
+        ++t;
       }
-      if (ok) mma_commit(&bar_done);
     }
   } else {
-    const int wg = warp / 4, r = (warp & 3) * 32 + lane, j = j0 + r;
+    const int wg = warp / 4, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t sbuf = lanes + C::TM_S + wg * QT, dbuf = lanes + C::TM_DP + wg * QT;
-    const bool check_keys = p.kmask != nullptr || j0 + 128 > n, live = key_live(p, b, j, n);
     const AttnDrop drop = attn_drop(p.rng, DROP ? p.drop_thr : 0, p.drop_scale);
     const uint32_t thr2 = drop.pair();
     const uint64_t sc2 = f2(p.scale_log2, p.scale_log2), ds2 = f2(drop.scale, drop.scale);
-    // ids and dS lie in granules of 8 queries: this key's first granule of a chunk, and 8 BQ granules per chunk
-    const long long tile = ((long long)(j / 64) * (p.nqp / 8) + wg * (QT / 8)) * 64 + j % 64;
-    const uint4* idp = reinterpret_cast<const uint4*>(p.idsT) + tile;
-    uint4* const ds0 = reinterpret_cast<uint4*>(p.ds) + (long long)ul * p.G * (p.nkp / 8) * p.nqp + tile;
     constexpr uint32_t no = kNoPairOffset * 0x10001u;
     const uint4 none = make_uint4(no, no, no, no);
-    uint4 id[QT / 8];
-    auto fetch = [&](int qc) {  // a chunk ahead
-#pragma unroll
-      for (int x = 0; x < QT / 8; ++x)
-        id[x] = qc * BQ + wg * QT < p.nqp ? __ldg(idp + qc * (8 * BQ) + x * 64) : none;
-    };
-    if (BIAS) fetch(0);
-    bool ok = true;
-    int qc = 0, g = 0;
-    for (int c = 0; c < nc; ++c) {
-      const int st = c % NST, i0 = qc * BQ + wg * QT, bh = b * p.H + kh * p.G + g;
-      const bool inside = i0 < p.nqp;  // else a last chunk's padding: P = dS = 0, and nothing to store
-      uint4* ds = ds0 + (long long)g * (p.nkp / 8) * p.nqp + qc * (8 * BQ);
-      if (BIAS && qc == 0) {  // the next head's bias
-        named_sync(1, C::EWT);
-        if (threadIdx.x <= kMaxBuckets)
-          reinterpret_cast<float*>(xsmem + C::OFF_TAB)[threadIdx.x] = table_log2(p, kh * p.G + g, threadIdx.x);
-        named_sync(1, C::EWT);
-      }
-      if (++qc == nqc) qc = 0, ++g;
-      uint32_t keep = 0;
-      if (DROP) keep = keep_column<QT / 8>(drop, thr2, i0, j0 + (warp & 3) * 32, bh);
-      const bool some = (!check_keys || live) && inside;
-      const float* rec = reinterpret_cast<const float*>(xsmem + C::OFF_REC + st * C::REC_BYTES) + wg * QT / 64 * 192 +
-                         wg * QT % 64;
-      // bar_s follows bar_full, so the records are there too; the wait on bar_full makes their copy visible here
-      if (ok) ok = warp_wait(&bar_full[st], (c / NST) & 1, ctx) && warp_wait(&bar_s, c & 1, ctx);
-      if (!ok) continue;  // given up: only the barriers above are still met
-      tc_fence_after();
-      uint64_t pr[QT / 2];
-#pragma unroll
-      for (int k = 0; k < QT / 16; ++k) {
-        uint32_t s[16], w[8];
-        tmem_ld16_issue(sbuf + k * 16, s);
-        tmem_wait16(s);
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {  // two pairs of queries
-          const ulonglong2 r0 = *reinterpret_cast<const ulonglong2*>(rec + k * 16 + 2 * e);
-          ulonglong2 r1 = make_ulonglong2(0, 0);
-          if (BIAS) r1 = *reinterpret_cast<const ulonglong2*>(rec + 64 + k * 16 + 2 * e);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int q = e + u;
-            uint64_t t = f2(__uint_as_float(s[2 * q]), __uint_as_float(s[2 * q + 1]));
-            if (BIAS)
-              t = add2(fma2(t, sc2, table_pair(C::OFF_TAB, reinterpret_cast<const uint32_t*>(id)[k * 8 + q])), u ? r0.y : r0.x);
-            else
-              t = fma2(t, sc2, u ? r0.y : r0.x);
-            float x, y;
-            unf2(t, x, y);
-            t = f2(xex2(x), xex2(y));
-            if (BIAS) t = mul2(t, u ? r1.y : r1.x);
-            pr[k * 8 + q] = t;
-            unf2(t, x, y);
-            w[q] = pack_bf16(x, y);
-            if (DROP) w[q] &= spread_pair(keep << (k * 8 + q));
-          }
-        }
-        if (check_keys || !inside) {  // an absent key's row is 0 whatever K and V hold there
-#pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = some ? w[e] : 0u;
-        }
-        tmem_st8(sbuf + k * 8, w);
-      }
-      if (BIAS && c + 1 < nc) fetch(qc);
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&bar_p);
-      if (!(ok = warp_wait(&bar_dp, c & 1, ctx))) continue;
-      tc_fence_after();
-#pragma unroll
-      for (int k = 0; k < QT / 16; ++k) {
-        uint32_t dp[16], w[8];
-        tmem_ld16_issue(dbuf + k * 16, dp);
-        tmem_wait16(dp);
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const ulonglong2 r2 = *reinterpret_cast<const ulonglong2*>(rec + 128 + k * 16 + 2 * e);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int q = e + u;
-            uint64_t da;
-            if (DROP) {
-              const uint32_t kb = keep << (k * 8 + q);
-              da = f2(__uint_as_float(dp[2 * q] & spread_one<0>(kb)), __uint_as_float(dp[2 * q + 1] & spread_one<1>(kb)));
-              da = fma2(da, ds2, u ? r2.y : r2.x);
-            } else {
-              da = add2(f2(__uint_as_float(dp[2 * q]), __uint_as_float(dp[2 * q + 1])), u ? r2.y : r2.x);
-            }
-            float x, y;
-            unf2(mul2(pr[k * 8 + q], da), x, y);
-            w[q] = pack_bf16(x, y);
-          }
-        }
-        if (check_keys || !inside) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = some ? w[e] : 0u;
-        }
-        tmem_st8(dbuf + k * 8, w);
-        if (inside) {
-          ds[(2 * k) * 64] = make_uint4(w[0], w[1], w[2], w[3]);
-          ds[(2 * k + 1) * 64] = make_uint4(w[4], w[5], w[6], w[7]);
-        }
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&bar_ds);
-    }
-    if (ok) ok = warp_wait(&bar_done, 0, ctx);
-    tc_fence_after();
     const bool vk = vec_rows(p.dk), vv = vec_rows(p.dv), tk = p.out_tma & 2, tv = p.out_tma & 4;
-    const float fv = DROP ? p.drop_scale : 1.f;
-    if (ok) {  // K's and V's tiles are free: every product has completed
-#pragma unroll 1
-      for (int d = wg * 32; d < DP; d += 128) {
-        float x[32];
-        tmem_ld32(lanes + C::TM_DK + d, x);
-        if (tk) stage_row32(xsmem, r, d, x, p.scale);
-        else if (j < p.Nk && d < p.D) store_row(dK + (long long)j * p.dk.s[2] + d, x, p.scale, p.D - d, vk);
-        tmem_ld32(lanes + C::TM_DV + d, x);
-        if (tv) stage_row32(xsmem + C::OFF_V, r, d, x, fv);
-        else if (j < p.Nk && d < p.D) store_row(dV + (long long)j * p.dv.s[2] + d, x, fv, p.D - d, vv);
+    bool ok = true;
+    int t = 0, gc = 0;  // tiles and chunks so far
+    for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
+      const Tile x = tile_of(tile);
+      const int b = x.b, kh = x.kh, j0 = x.j0, j = j0 + r;
+      __nv_bfloat16* dK = reinterpret_cast<__nv_bfloat16*>(p.dk.p) + b * p.dk.s[0] + kh * p.dk.s[1];
+      __nv_bfloat16* dV = reinterpret_cast<__nv_bfloat16*>(p.dv.p) + b * p.dv.s[0] + kh * p.dv.s[1];
+      if (j0 >= x.n) {  // no key of this tile exists: zero gradients, and the scratch is not read here
+        for (int y = threadIdx.x; y < 128 * p.D; y += C::EWT) {
+          const int jj = j0 + y / p.D, d = y % p.D;
+          if (jj < p.Nk) {
+            dK[(long long)jj * p.dk.s[2] + d] = __float2bfloat16_rn(0.f);
+            dV[(long long)jj * p.dv.s[2] + d] = __float2bfloat16_rn(0.f);
+          }
+        }
+        continue;
       }
-    }
-    fence_proxy_async_smem();
-    named_sync(1, C::EWT);
-    if (threadIdx.x == 0 && ok) {
-      if (tk) store_tile<DP>(&maps.dk, xsmem, p.D, j0, kh, b);
-      if (tv) store_tile<DP>(&maps.dv, xsmem + C::OFF_V, p.D, j0, kh, b);
-      bulk_wait_read0();
+      const bool check_keys = p.kmask != nullptr || j0 + 128 > x.n, live = key_live(p, b, j, x.n);
+      // ids and dS lie in granules of 8 queries: this key's first granule of a chunk, and 8 BQ granules per chunk
+      const long long at = ((long long)(j / 64) * (p.nqp / 8) + wg * (QT / 8)) * 64 + j % 64;
+      const uint4* idp = reinterpret_cast<const uint4*>(p.idsT) + at;
+      uint4* const ds0 = reinterpret_cast<uint4*>(p.ds) + (long long)x.ul * p.G * (p.nkp / 8) * p.nqp + at;
+      uint4 id[QT / 8];
+      auto fetch = [&](int qc) {  // a chunk ahead
+#pragma unroll
+        for (int x = 0; x < QT / 8; ++x)
+          id[x] = qc * BQ + wg * QT < p.nqp ? __ldg(idp + qc * (8 * BQ) + x * 64) : none;
+      };
+      if (BIAS) fetch(0);
+      int qc = 0, g = 0;
+      for (int c = 0; c < nc; ++c, ++gc) {
+        const int st = gc % NST, i0 = qc * BQ + wg * QT, bh = b * p.H + kh * p.G + g;
+        const bool inside = i0 < p.nqp;  // else a last chunk's padding: P = dS = 0, and nothing to store
+        uint4* ds = ds0 + (long long)g * (p.nkp / 8) * p.nqp + qc * (8 * BQ);
+        if (BIAS && qc == 0) {  // the next head's bias
+          named_sync(1, C::EWT);
+          if (threadIdx.x <= kMaxBuckets)
+            reinterpret_cast<float*>(xsmem + C::OFF_TAB)[threadIdx.x] = table_log2(p, kh * p.G + g, threadIdx.x);
+          named_sync(1, C::EWT);
+        }
+        if (++qc == nqc) qc = 0, ++g;
+        uint32_t keep = 0;
+        if (DROP) keep = keep_column<QT / 8>(drop, thr2, i0, j0 + (warp & 3) * 32, bh);
+        const bool some = (!check_keys || live) && inside;
+        const float* rec = reinterpret_cast<const float*>(xsmem + C::OFF_REC + st * C::REC_BYTES) + wg * QT / 64 * 192 +
+                           wg * QT % 64;
+        // bar_s follows bar_full, so the records are there too; the wait on bar_full makes their copy visible here
+        if (ok) ok = warp_wait(&bar_full[st], (gc / NST) & 1, ctx) && warp_wait(&bar_s, gc & 1, ctx);
+        if (!ok) continue;  // given up: only the barriers above are still met
+        tc_fence_after();
+        uint64_t pr[QT / 2];
+#pragma unroll
+        for (int k = 0; k < QT / 16; ++k) {
+          uint32_t s[16], w[8];
+          tmem_ld16_issue(sbuf + k * 16, s);
+          tmem_wait16(s);
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {  // two pairs of queries
+            const ulonglong2 r0 = *reinterpret_cast<const ulonglong2*>(rec + k * 16 + 2 * e);
+            ulonglong2 r1 = make_ulonglong2(0, 0);
+            if (BIAS) r1 = *reinterpret_cast<const ulonglong2*>(rec + 64 + k * 16 + 2 * e);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int q = e + u;
+              uint64_t t = f2(__uint_as_float(s[2 * q]), __uint_as_float(s[2 * q + 1]));
+              if (BIAS)
+                t = add2(fma2(t, sc2, table_pair(C::OFF_TAB, reinterpret_cast<const uint32_t*>(id)[k * 8 + q])), u ? r0.y : r0.x);
+              else
+                t = fma2(t, sc2, u ? r0.y : r0.x);
+              float x, y;
+              unf2(t, x, y);
+              t = f2(xex2(x), xex2(y));
+              if (BIAS) t = mul2(t, u ? r1.y : r1.x);
+              pr[k * 8 + q] = t;
+              unf2(t, x, y);
+              w[q] = pack_bf16(x, y);
+              if (DROP) w[q] &= spread_pair(keep << (k * 8 + q));
+            }
+          }
+          if (check_keys || !inside) {  // an absent key's row is 0 whatever K and V hold there
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = some ? w[e] : 0u;
+          }
+          tmem_st8(sbuf + k * 8, w);
+        }
+        if (BIAS && c + 1 < nc) fetch(qc);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bar_p);
+        if (!(ok = warp_wait(&bar_dp, gc & 1, ctx))) continue;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < QT / 16; ++k) {
+          uint32_t dp[16], w[8];
+          tmem_ld16_issue(dbuf + k * 16, dp);
+          tmem_wait16(dp);
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const ulonglong2 r2 = *reinterpret_cast<const ulonglong2*>(rec + 128 + k * 16 + 2 * e);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int q = e + u;
+              uint64_t da;
+              if (DROP) {
+                const uint32_t kb = keep << (k * 8 + q);
+                da = f2(__uint_as_float(dp[2 * q] & spread_one<0>(kb)), __uint_as_float(dp[2 * q + 1] & spread_one<1>(kb)));
+                da = fma2(da, ds2, u ? r2.y : r2.x);
+              } else {
+                da = add2(f2(__uint_as_float(dp[2 * q]), __uint_as_float(dp[2 * q + 1])), u ? r2.y : r2.x);
+              }
+              float x, y;
+              unf2(mul2(pr[k * 8 + q], da), x, y);
+              w[q] = pack_bf16(x, y);
+            }
+          }
+          if (check_keys || !inside) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = some ? w[e] : 0u;
+          }
+          tmem_st8(dbuf + k * 8, w);
+          if (inside) {
+            ds[(2 * k) * 64] = make_uint4(w[0], w[1], w[2], w[3]);
+            ds[(2 * k + 1) * 64] = make_uint4(w[4], w[5], w[6], w[7]);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bar_ds);
+      }
+      if (ok) ok = warp_wait(&bar_done, t & 1, ctx);
+      tc_fence_after();
+      // dK and dV leave through the last chunk's slot; DP = 192 has room for one of them at a time
+      uint8_t* stage = xsmem + C::OFF_ST + (gc - 1) % NST * C::STAGE;
+      constexpr bool BOTH = C::STAGE >= 2 * C::K_BYTES;
+      const float fv = DROP ? p.drop_scale : 1.f;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        const bool tma = which ? tv : tk;
+        __nv_bfloat16* out = which ? dV + (long long)j * p.dv.s[2] : dK + (long long)j * p.dk.s[2];
+        uint8_t* dst = stage + (BOTH ? which * C::K_BYTES : 0);
+        if (ok) {
+#pragma unroll 1
+          for (int d = wg * 32; d < DP; d += 128) {
+            float v[32];
+            tmem_ld32(lanes + (which ? C::TM_DV : C::TM_DK) + d, v);
+            if (tma) stage_row32(dst, r, d, v, which ? fv : p.scale);
+            else if (j < p.Nk && d < p.D) store_row(out + d, v, which ? fv : p.scale, p.D - d, which ? vv : vk);
+          }
+        }
+        if (which == 1) {
+          tc_fence_before();
+          mbar_arrive(&bar_acc);  // the accumulators may be overwritten
+        }
+        if (BOTH && which == 0) continue;
+        fence_proxy_async_smem();
+        named_sync(1, C::EWT);
+        if (threadIdx.x == 0 && ok) {
+          if (tk && (BOTH || which == 0)) store_tile<DP>(&maps.dk, stage, p.D, j0, kh, b);
+          if (tv && which == 1) store_tile<DP>(&maps.dv, dst, p.D, j0, kh, b);
+          bulk_wait_read0();
+        }
+        if (!BOTH && which == 0) named_sync(1, C::EWT);  // dK has left the stage
+      }
+      if (threadIdx.x == 0) mbar_arrive(&bar_out);
+      ++t;
     }
   }
   tc_fence_before();
