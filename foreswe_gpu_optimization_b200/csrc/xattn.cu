@@ -373,7 +373,6 @@ int geoattn_xattn_bwd(const GeoXattnBwdArgs* a, void* stream) {
   std::memset(&maps, 0, sizeof(maps));
   int rc = d.bf16 ? backward_maps(maps, p, d) : GEOATTN_OK;
   if (rc) return rc;
-  if (cudaMemsetAsync(ws.status, 0, sizeof(int), st) != cudaSuccess) return GEOATTN_ERR_LAUNCH;
   rc = d.bf16 ? records(p, d, st)
               : xlaunch(xattn_delta_kernel, ((long long)d.B * d.H * d.Nq + 31) / 32, 256, 0, st, p);
   if (rc) return rc;

@@ -444,6 +444,7 @@ template <int LPR>  // lanes per row: 8 columns each
 __global__ void __launch_bounds__(256) xattn_records_kernel(const XParams p, int heads_first) {
   constexpr int ROWS = 256 / LPR;  // rows of a step
   __shared__ float delta[256];
+  if (threadIdx.x == 0 && blockIdx.x + blockIdx.y + blockIdx.z == 0) *p.status = kDevOk;
   // 256 rows: 16 rows of 16 heads, head by head in memory, or 256 rows of one head
   const int HB = heads_first ? 16 : 1, IB = 256 / HB;
   const int b = blockIdx.z, h0 = blockIdx.y * HB, i0 = blockIdx.x * IB;

@@ -15,23 +15,37 @@ import torch
 
 from . import _lib
 from .counter_dropout import _dtype_code, _snapshot, _threshold
-from .geo_attention_v2 import _tma_ready
 
 MAX_BUCKETS = 64
+
+
+def _aligned(t):
+    """bf16 operands and outputs go through TMA: head dim contiguous, base and other strides multiples of 16 bytes."""
+    s0, s1, s2, s3 = t.stride()
+    return s3 == 1 and not ((t.data_ptr() >> 1) | s0 | s1 | s2) & 7 and s0 > 0 and s1 > 0 and s2 > 0
+
+
+def _padded(t):
+    """Uninitialised [B, H, N, D] whose rows start on 16 bytes, heads and rows in t's order."""
+    B, H, N, D = t.shape
+    d8 = (D + 7) // 8 * 8
+    if t.stride(1) < t.stride(2):  # heads side by side, as projections write them
+        return torch.empty(B, N, H, d8, dtype=t.dtype, device=t.device).transpose(1, 2)[..., :D]
+    return torch.empty(B, H, N, d8, dtype=t.dtype, device=t.device)[..., :D]
 
 
 def _ready(t):
     """Operand layout of the kernels: bf16 as TMA reads it; fp32 with the head dim contiguous."""
     if t.dtype == torch.float32:
         return t if t.stride(3) == 1 else t.contiguous()
-    s0, s1, s2, s3 = t.stride()
-    if s3 == 1 and not ((t.data_ptr() >> 1) | s0 | s1 | s2) & 7 and s0 > 0 and s1 > 0 and s2 > 0:
-        return t
-    return _tma_ready(t)
+    return t if _aligned(t) else _padded(t).copy_(t)
 
 
 def _like(t):
-    """An output with t's layout where that keeps the head dim contiguous (split_heads views do), else contiguous."""
+    """An output with t's layout where that keeps the head dim contiguous (split_heads views do), else contiguous; in
+    bf16 with padded rows where the layout has none that start on 16 bytes (a head dim that is no multiple of 8)."""
+    if t.dtype == torch.bfloat16 and t.shape[3] % 8:
+        return _padded(t)
     return torch.empty_like(t) if t.stride(3) == 1 else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
@@ -56,11 +70,18 @@ def _inputs(shape, q, k, v, table, ids, lens, mask, rng, thr, scale):
             _ptr(lens), _ptr(mask), 0 if mask is None else mask.stride(0), _ptr(rng), thr, scale)
 
 
+def _dense(o, q):
+    """o without padded rows, in q's layout."""
+    if o.dtype == torch.float32 or q.shape[3] % 8 == 0:
+        return o
+    return (torch.empty_like(q) if q.stride(3) == 1 else torch.empty(q.shape, dtype=q.dtype, device=q.device)).copy_(o)
+
+
 def _forward(q, k, v, table, ids, lens, mask, rng, thr, scale, need_stats):
+    """(o, row statistics) for operands in the kernels' layout (_ready)."""
     o = _like(q)
     if k.shape[2] == 0 or thr == 65536:  # no key, or no weight is kept
         return o.zero_(), None
-    q, k, v = _ready(q), _ready(k), _ready(v)
     shape, dev = _shape(q, k, table), q.device
     ws = torch.empty(_lib.xattn_workspace("geoattn_xattn_fwd_workspace_bytes", *shape), dtype=torch.uint8, device=dev)
     stats = torch.empty(*q.shape[:3], 2, dtype=torch.float32, device=dev) if need_stats else None
@@ -74,7 +95,7 @@ def _backward(q, k, v, table, ids, lens, mask, rng, thr, scale, o, stats, do):
     dtable = torch.empty_like(table, memory_format=torch.contiguous_format) if table is not None else None
     if k.shape[2] == 0 or thr == 65536:
         return dq.zero_(), dk.zero_(), dv.zero_(), None if dtable is None else dtable.zero_()
-    q, k, v, do = _ready(q), _ready(k), _ready(v), _ready(do)
+    do = _ready(do)
     shape, dev = _shape(q, k, table), q.device
     ws = torch.empty(_lib.xattn_workspace("geoattn_xattn_bwd_workspace_bytes", *shape), dtype=torch.uint8, device=dev)
     _lib.launch(dev, _lib.packed("geoattn_xattn_bwd"), _lib.XATTN_BWD.pack(
@@ -88,16 +109,17 @@ class CrossAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, table, ids, lens, mask, rng, thr, scale):
-        o, stats = _forward(q, k, v, table, ids, lens, mask, rng, thr, scale, True)
-        ctx.save_for_backward(q, k, v, table, ids, lens, mask, rng, o, stats)
+        args = (_ready(q), _ready(k), _ready(v), table, ids, lens, mask, rng)
+        o, stats = _forward(*args, thr, scale, True)
+        ctx.save_for_backward(*args, o, stats)  # o as the kernels wrote it
         ctx.thr, ctx.scale = thr, scale
-        return o
+        return _dense(o, q)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
-        q, k, v, table, ids, lens, mask, rng, o, stats = ctx.saved_tensors
-        grads = _backward(q, k, v, table, ids, lens, mask, rng, ctx.thr, ctx.scale, o, stats, do)
+        *args, o, stats = ctx.saved_tensors
+        grads = _backward(*args, ctx.thr, ctx.scale, o, stats, do)
         return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), *([None] * 6))
 
 
@@ -167,4 +189,5 @@ def cross_attention(q, k, v, *, buckets=None, bias_table=None, kv_lens=None, key
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
                                     (bias_table is not None and bias_table.requires_grad)):
         return CrossAttention.apply(q, k, v, bias_table, buckets, kv_lens, key_mask, key, thr, scale)
-    return _forward(q, k, v, bias_table, buckets, kv_lens, key_mask, key, thr, scale, False)[0]
+    o = _forward(_ready(q), _ready(k), _ready(v), bias_table, buckets, kv_lens, key_mask, key, thr, scale, False)[0]
+    return _dense(o, q)
