@@ -284,22 +284,31 @@ int records(const XParams& p, const XDims& d, cudaStream_t st) {
   return status_of(cudaGetLastError());
 }
 
-template <int DP>
-int tc_bwd(const xa::XMaps& maps, const XParams& p, int units, cudaStream_t st) {
-  using C = xa::KeysCfg<DP>;
+template <int DP, int BQ>
+int tc_bwd_keys(const xa::XMaps& maps, const XParams& p, int units, cudaStream_t st) {
+  using C = xa::KeysCfg<DP, BQ>;
   const long long tiles = (long long)((p.Nk + 127) / 128) * units, grid = tiles < kSMs ? tiles : kSMs;
   XParams pk = p;
   pk.tiles = (int)tiles;
-  auto keys = p.ids ? (p.drop_thr ? xa::xattn_bwd_keys_kernel<DP, true, true> : xa::xattn_bwd_keys_kernel<DP, true, false>)
-                    : (p.drop_thr ? xa::xattn_bwd_keys_kernel<DP, false, true> : xa::xattn_bwd_keys_kernel<DP, false, false>);
-  if (int rc = tc_launch(keys, grid, C::THREADS, C::SMEM, st, maps, pk)) return rc;
+  auto keys = p.ids ? (p.drop_thr ? xa::xattn_bwd_keys_kernel<DP, BQ, true, true> : xa::xattn_bwd_keys_kernel<DP, BQ, true, false>)
+                    : (p.drop_thr ? xa::xattn_bwd_keys_kernel<DP, BQ, false, true> : xa::xattn_bwd_keys_kernel<DP, BQ, false, false>);
+  return tc_launch(keys, grid, C::THREADS, C::SMEM, st, maps, pk);
+}
+
+template <int DP>
+int tc_bwd_dq(const xa::XMaps& maps, const XParams& p, int units, cudaStream_t st) {
   return tc_launch(xa::xattn_bwd_dq_kernel<DP>, (long long)((p.Nq + 127) / 128) * units * p.G, xa::DqCfg<DP>::THREADS,
                    xa::DqCfg<DP>::SMEM, st, maps, p);
 }
 
 int backward_tc(const xa::XMaps& maps, const XParams& p, const XDims& d, int units, cudaStream_t st) {
-  return d.DP == 64 ? tc_bwd<64>(maps, p, units, st)
-                    : d.DP == 128 ? tc_bwd<128>(maps, p, units, st) : tc_bwd<192>(maps, p, units, st);
+  const bool few = d.nqp <= 64;  // half of a chunk of 128 queries would be padding
+  int rc = d.DP == 64    ? few ? tc_bwd_keys<64, 64>(maps, p, units, st) : tc_bwd_keys<64, 128>(maps, p, units, st)
+           : d.DP == 128 ? few ? tc_bwd_keys<128, 64>(maps, p, units, st) : tc_bwd_keys<128, 128>(maps, p, units, st)
+                         : tc_bwd_keys<192, 64>(maps, p, units, st);
+  if (rc) return rc;
+  return d.DP == 64 ? tc_bwd_dq<64>(maps, p, units, st)
+                    : d.DP == 128 ? tc_bwd_dq<128>(maps, p, units, st) : tc_bwd_dq<192>(maps, p, units, st);
 }
 
 template <class S>

@@ -508,23 +508,26 @@ __global__ void __launch_bounds__(256) xattn_records_kernel(const XParams p, int
 //   4 warpgroups   P of chunk c while dK(c - 1) and dP^T(c) run, then dS of chunk c while dV(c) and S^T(c + 1) run
 // Bound by the operand feed of the products (S and dP 64 clocks per 16 of the head dim and 128 queries, dV and dK as
 // many per 16 queries at DP = 128): chunks of 128 queries, which halve K's and V's share of it, with one score buffer
-// (S 128, dP 128, dK 128, dV 128 columns) beat chunks of 64 with two. DP = 192 has columns for 64 queries only.
+// (S 128, dP 128, dK 128, dV 128 columns) beat chunks of 64 with two. DP = 192 has columns for 64 queries.
 // One persistent CTA per SM (tensor memory is full): K and V of the next tile are loaded as soon as this one's last
-// scores are formed, and the next tile's first scores run while dK and dV leave. They are staged in the slot of the
-// tile's last chunk, which is refilled only then. (One CTA per tile spent 40 % of its time filling and draining at 512
-// queries.)
+// scores are formed, and the next tile's first scores run while dK and dV leave, from a stage of their own where shared
+// memory has one, else from the slot of the tile's last chunk, which is refilled only then. (One CTA per tile spent 40 %
+// of its time filling and draining at 512 queries.) Up to 64 queries per head run chunks of 64.
 // Dropout: a Philox call covers one query and 8 keys. Each lane makes the calls of 2 or 4 queries for its octet of keys
 // and the 8 x 8 bit blocks are transposed among 8 lanes (3 shuffles), so no call is made twice.
 // ---------------------------------------------------------------------------------------------------------------
-template <int DP>
+template <int DP, int BQ_>
 struct KeysCfg {
-  static constexpr int BQ = DP == 192 ? 64 : 128, QT = BQ / 4;  // queries per chunk and per thread
-  static constexpr int NST = DP == 64 ? 4 : 2;                  // chunks of Q, dO and records in flight
+  static constexpr int BQ = BQ_, QT = BQ / 4;  // queries per chunk and per thread
+  static constexpr int NST = DP == 64 ? 4 : 2;  // chunks of Q, dO and records in flight
   static constexpr int K_BYTES = DP / 64 * 128 * 128, Q_BYTES = DP / 64 * BQ * 128, REC_BYTES = BQ * 12;
   static constexpr int STAGE = 2 * Q_BYTES;
-  static constexpr int OFF_V = K_BYTES, OFF_ST = 2 * K_BYTES, OFF_REC = OFF_ST + NST * STAGE,
-                       OFF_TAB = OFF_REC + NST * REC_BYTES, SMEM = OFF_TAB + 512;
+  static constexpr bool OWN = DP == 64 || (DP == 128 && BQ == 64);  // dK and dV have a stage of their own
+  static constexpr int OFF_V = K_BYTES, OFF_ST = 2 * K_BYTES, OFF_OUT = OFF_ST + NST * STAGE,
+                       OFF_REC = OFF_OUT + (OWN ? 2 * K_BYTES : 0), OFF_TAB = OFF_REC + NST * REC_BYTES,
+                       SMEM = OFF_TAB + 512;
   static constexpr int TM_DK = 0, TM_DV = DP, TM_S = 2 * DP, TM_DP = TM_S + BQ, TM_COLS = 512;
+  static_assert(TM_DP + BQ <= 512 && SMEM + 1024 <= 227 * 1024, "");
   static constexpr int EWT = 512, THREADS = EWT + 64, TMA_WARP = 16, MMA_WARP = 17;
 };
 
@@ -551,10 +554,10 @@ __device__ __forceinline__ uint32_t keep_column(const AttnDrop& drop, uint32_t t
   return lane & 4 ? (x & 0x33333333u) | ((y << 2) & 0xCCCCCCCCu) : (x & 0xCCCCCCCCu) | ((y >> 2) & 0x33333333u);
 }
 
-template <int DP, bool BIAS, bool DROP>
-__global__ void __launch_bounds__(KeysCfg<DP>::THREADS, 1)
+template <int DP, int BQ_, bool BIAS, bool DROP>
+__global__ void __launch_bounds__(KeysCfg<DP, BQ_>::THREADS, 1)
     xattn_bwd_keys_kernel(const __grid_constant__ XMaps maps, const XParams p) {
-  using C = KeysCfg<DP>;
+  using C = KeysCfg<DP, BQ_>;
   constexpr int NST = C::NST, BQ = C::BQ, QT = C::QT;
   __shared__ uint64_t bar_k, bar_kfree, bar_full[NST], bar_empty[NST], bar_s, bar_dp, bar_p, bar_ds, bar_done, bar_acc,
       bar_out;
@@ -623,7 +626,7 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, 1)
           if (!(ok = mbar_wait(&bar_empty[st], ((g / NST) & 1) ^ 1, ctx))) break;
           // The last tile's dK and dV leave through its last chunk's slot, which chunk NST - 1 of this tile takes over.
           // Not later than this tile's last chunk, so that bar_out cannot run two phases ahead of the wait.
-          if (t > 0 && c == (NST < nc ? NST : nc) - 1 && !(ok = mbar_wait(&bar_out, (t - 1) & 1, ctx))) break;
+          if (!C::OWN && t > 0 && c == (NST < nc ? NST : nc) - 1 && !(ok = mbar_wait(&bar_out, (t - 1) & 1, ctx))) break;
           uint8_t* dst = xsmem + C::OFF_ST + st * C::STAGE;
           mbar_arrive_expect_tx(&bar_full[st], C::STAGE + rec);
           for (int y = 0; y < BQ; y += 64) {
@@ -688,6 +691,7 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, 1)
     const uint64_t sc2 = f2(p.scale_log2, p.scale_log2), ds2 = f2(drop.scale, drop.scale);
     constexpr uint32_t no = kNoPairOffset * 0x10001u;
     const uint4 none = make_uint4(no, no, no, no);
+    const uint32_t zeros[8] = {};
     const bool vk = vec_rows(p.dk), vv = vec_rows(p.dv), tk = p.out_tma & 2, tv = p.out_tma & 4;
     bool ok = true;
     int t = 0, gc = 0;  // tiles and chunks so far
@@ -715,13 +719,13 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, 1)
       auto fetch = [&](int qc) {  // a chunk ahead
 #pragma unroll
         for (int x = 0; x < QT / 8; ++x)
-          id[x] = qc * BQ + wg * QT < p.nqp ? __ldg(idp + qc * (8 * BQ) + x * 64) : none;
+          id[x] = qc * BQ + wg * QT < p.Nq ? __ldg(idp + qc * (8 * BQ) + x * 64) : none;
       };
       if (BIAS) fetch(0);
       int qc = 0, g = 0;
       for (int c = 0; c < nc; ++c, ++gc) {
         const int st = gc % NST, i0 = qc * BQ + wg * QT, bh = b * p.H + kh * p.G + g;
-        const bool inside = i0 < p.nqp;  // else a last chunk's padding: P = dS = 0, and nothing to store
+        const bool inside = i0 < p.Nq;  // else padding: P = dS = 0
         uint4* ds = ds0 + (long long)g * (p.nkp / 8) * p.nqp + qc * (8 * BQ);
         if (BIAS && qc == 0) {  // the next head's bias
           named_sync(1, C::EWT);
@@ -731,8 +735,7 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, 1)
         }
         if (++qc == nqc) qc = 0, ++g;
         uint32_t keep = 0;
-        if (DROP) keep = keep_column<QT / 8>(drop, thr2, i0, j0 + (warp & 3) * 32, bh);
-        const bool some = (!check_keys || live) && inside;
+        if (DROP && inside) keep = keep_column<QT / 8>(drop, thr2, i0, j0 + (warp & 3) * 32, bh);
         const float* rec = reinterpret_cast<const float*>(xsmem + C::OFF_REC + st * C::REC_BYTES) + wg * QT / 64 * 192 +
                            wg * QT % 64;
         // bar_s follows bar_full, so the records are there too; the wait on bar_full makes their copy visible here
@@ -742,6 +745,10 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, 1)
         uint64_t pr[QT / 2];
 #pragma unroll
         for (int k = 0; k < QT / 16; ++k) {
+          if (!inside) {
+            tmem_st8(sbuf + k * 8, zeros);
+            continue;
+          }
           uint32_t s[16], w[8];
           tmem_ld16_issue(sbuf + k * 16, s);
           tmem_wait16(s);
@@ -768,9 +775,9 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, 1)
               if (DROP) w[q] &= spread_pair(keep << (k * 8 + q));
             }
           }
-          if (check_keys || !inside) {  // an absent key's row is 0 whatever K and V hold there
+          if (check_keys) {  // an absent key's row is 0 whatever K and V hold there
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = some ? w[e] : 0u;
+            for (int e = 0; e < 8; ++e) w[e] = live ? w[e] : 0u;
           }
           tmem_st8(sbuf + k * 8, w);
         }
@@ -782,6 +789,10 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, 1)
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < QT / 16; ++k) {
+          if (!inside) {
+            tmem_st8(dbuf + k * 8, zeros);
+            continue;
+          }
           uint32_t dp[16], w[8];
           tmem_ld16_issue(dbuf + k * 16, dp);
           tmem_wait16(dp);
@@ -804,15 +815,14 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, 1)
               w[q] = pack_bf16(x, y);
             }
           }
-          if (check_keys || !inside) {
+          if (check_keys) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = some ? w[e] : 0u;
+            for (int e = 0; e < 8; ++e) w[e] = live ? w[e] : 0u;
           }
           tmem_st8(dbuf + k * 8, w);
-          if (inside) {
-            ds[(2 * k) * 64] = make_uint4(w[0], w[1], w[2], w[3]);
-            ds[(2 * k + 1) * 64] = make_uint4(w[4], w[5], w[6], w[7]);
-          }
+          // granules without a query are neither written nor read
+          if (i0 + k * 16 < p.Nq) ds[(2 * k) * 64] = make_uint4(w[0], w[1], w[2], w[3]);
+          if (i0 + k * 16 + 8 < p.Nq) ds[(2 * k + 1) * 64] = make_uint4(w[4], w[5], w[6], w[7]);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -820,9 +830,10 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, 1)
       }
       if (ok) ok = warp_wait(&bar_done, t & 1, ctx);
       tc_fence_after();
-      // dK and dV leave through the last chunk's slot; DP = 192 has room for one of them at a time
-      uint8_t* stage = xsmem + C::OFF_ST + (gc - 1) % NST * C::STAGE;
-      constexpr bool BOTH = C::STAGE >= 2 * C::K_BYTES;
+      // dK and dV leave through a stage of their own (thread 0 saw it read before it went on to this tile) or the last
+      // chunk's slot; DP = 192 has room for one of them at a time
+      uint8_t* stage = xsmem + (C::OWN ? C::OFF_OUT : C::OFF_ST + (gc - 1) % NST * C::STAGE);
+      constexpr bool BOTH = C::OWN || C::STAGE >= 2 * C::K_BYTES;
       const float fv = DROP ? p.drop_scale : 1.f;
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
@@ -852,7 +863,7 @@ __global__ void __launch_bounds__(KeysCfg<DP>::THREADS, 1)
         }
         if (!BOTH && which == 0) named_sync(1, C::EWT);  // dK has left the stage
       }
-      if (threadIdx.x == 0) mbar_arrive(&bar_out);
+      if (!C::OWN && threadIdx.x == 0) mbar_arrive(&bar_out);
       ++t;
     }
   }
@@ -910,8 +921,8 @@ __global__ void __launch_bounds__(192, 2) xattn_bwd_dq_kernel(const __grid_const
 
   if (warp == C::TMA_WARP) {
     if (lane == 0) {
-      // 16 granules of 8 queries, 8 in a last tile of 64 rows (what its other rows yield is not stored)
-      const int bytes = (p.nqp - qt * 128 < 128 ? 8 : 16) * 1024;
+      // the granules that hold queries (what the tile's other rows yield is not stored)
+      const int rows = p.Nq - qt * 128, bytes = (rows < 128 ? (rows + 7) / 8 : 16) * 1024;
       const uint4* ds = reinterpret_cast<const uint4*>(p.ds) + (long long)ul * (p.nkp / 8) * p.nqp + (long long)qt * 16 * 64;
       for (int c = 0; c < nc; ++c) {
         const int st = c % NST;
