@@ -382,6 +382,88 @@ def test_other_streams():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp32"])
+def test_key_lengths_are_clamped(dtype):
+    """Lengths below 0 and above Nk count as 0 and Nk, in either integer type and from a broadcast tensor."""
+    import foreswe_gpu_optimization_b200 as g
+    x, _ = make(3, 2, 2, 20, 70, 32, dtype, seed=21)
+    q, k, v = (x[n].cuda() for n in "qkv")
+    want = g.cross_attention(q, k, v, kv_lens=torch.tensor([0, 70, 33], device="cuda"))
+    for t in (torch.int32, torch.int64):
+        got = g.cross_attention(q, k, v, kv_lens=torch.tensor([-5, 1000, 33], dtype=t, device="cuda"))
+        assert torch.equal(got, want)
+    assert (want[0] == 0).all()
+    one = g.cross_attention(q, k, v, kv_lens=torch.tensor([33], device="cuda").expand(3))
+    assert torch.equal(one[2], want[2])
+    row = torch.rand(1, 70, device="cuda") > 0.5
+    assert torch.equal(g.cross_attention(q, k, v, key_mask=row.expand(3, 70)),
+                       g.cross_attention(q, k, v, key_mask=row.repeat(3, 1)))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp32"])
+def test_scratch_in_several_launches(dtype):
+    """A batch whose dS scratch passes 4 GB runs its backward in several launches: each batch entry's gradients are
+    bitwise those of a call of its own, and the table's gradient (whose partial sums are grouped differently) is the
+    sum of theirs to the rounding of its terms."""
+    import foreswe_gpu_optimization_b200 as g
+    B, H, Nq, Nk, D, T = (2, 36, 4096, 8192, 16, 6) if dtype == BF else (2, 20, 4096, 8192, 16, 6)
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen, device="cuda").to(dtype)  # noqa: E731
+    q, k, v, do = r(B, H, Nq, D), r(B, H, Nk, D), r(B, H, Nk, D), r(B, H, Nq, D)
+    table = torch.randn(H, T, generator=gen, device="cuda")
+    ids = torch.randint(0, T, (Nq, Nk), generator=gen, device="cuda").to(torch.uint8)
+
+    def grads(sl):
+        x = [t[sl].detach().requires_grad_(True) for t in (q, k, v)]
+        t = table.detach().requires_grad_(True)
+        o = g.cross_attention(*x, buckets=ids, bias_table=t)
+        return torch.autograd.grad(o, [*x, t], do[sl])
+
+    both = grads(slice(0, 2))
+    ones = [grads(slice(b, b + 1)) for b in range(B)]
+    for i in range(3):
+        for b in range(B):
+            assert torch.equal(both[i][b:b + 1], ones[b][i]), (i, b)
+    # 2^12 partial sums at most, each of fp32 terms: 2^-24 * 2^12 of the sums' size bounds the regrouping
+    size = sum(o[3].abs() for o in ones)
+    assert ((both[3] - sum(o[3] for o in ones)).abs() <= 2.0 ** -12 * (size + size.max())).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp32"])
+def test_offsets_past_32_bits(dtype):
+    """Batch entries more than 2^31 elements apart in one cache."""
+    import foreswe_gpu_optimization_b200 as g
+    H, Nk, D = 2, 200, 64
+    far = 2 ** 31 + 64
+    cache = torch.zeros(far + H * Nk * D, dtype=dtype, device="cuda")
+    x, _ = make(2, H, H, 30, Nk, D, dtype, seed=3)
+    k = cache.as_strided((2, H, Nk, D), (far, Nk * D, D, 1))
+    k.copy_(x["k"])
+    outs = []
+    for kk in (k, x["k"].cuda()):
+        leaves = [x["q"].cuda().requires_grad_(True), kk.detach().requires_grad_(True),
+                  x["v"].cuda().requires_grad_(True)]
+        o = g.cross_attention(leaves[0], leaves[1], leaves[1])
+        outs.append([o.detach(), *torch.autograd.grad(o, leaves[:2], x["do"].cuda())])
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+def test_query_counts_around_the_chunks():
+    """1 to 200 queries: the chunk sizes of the backward and the padding of the last one."""
+    for Nq in (1, 8, 9, 16, 17, 31, 63, 64, 65, 96, 127, 128, 129, 192, 193):
+        for D in (64, 128, 192):
+            x, kw = make(1, 2, 1, Nq, 140, D, BF, seed=Nq, T=5, mask=True)
+            check(x, kw, p=0.1, key=[Nq, D])
+
+
+def test_many_key_tiles_per_cta():
+    """More key tiles than the persistent key pass has CTAs, some of them past their batch entry's length."""
+    for D, Nq in ((64, 40), (64, 130), (128, 20), (128, 300), (192, 33)):
+        x, kw = make(7, 6, 6, Nq, 600, D, BF, seed=D + Nq, T=7, lens=[600, 1, 0, 129, 256, 513, 77])
+        check(x, kw, p=0.2, key=[4, 4])
+
+
 def test_a_thread_of_its_own():
     """Forward and backward as the first CUDA work of a thread."""
     import threading
