@@ -8,8 +8,8 @@ OUT = os.path.join(HERE, "libgeoattn.so")
 OBJ = os.path.join(HERE, "_build")
 SOURCES = ("geoattn.cu", "xattn.cu")
 HEADERS = {"geoattn.cu": ("geoattn_kernels.cuh", "sm100.cuh", "tma_host.h", "host_util.h"),
-           "xattn.cu": ("xattn_common.cuh", "xattn_simt.cuh", "xattn_tc.cuh", "xattn_aux.cuh", "philox.cuh", "sm100.cuh",
-                        "tma_host.h", "host_util.h")}
+           "xattn.cu": ("xattn_common.cuh", "xattn_rows.cuh", "xattn_simt.cuh", "xattn_tc.cuh", "xattn_aux.cuh", "philox.cuh",
+                        "sm100.cuh", "tma_host.h", "host_util.h")}
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC"]
 
 

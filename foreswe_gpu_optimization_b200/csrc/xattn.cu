@@ -2,11 +2,13 @@
 #include <cmath>
 #include <cstdint>
 #include <cstring>
+#include <type_traits>
 
 #include "../../include/geoattn.h"
 #include "host_util.h"
-#include "xattn_aux.cuh"
 #include "tma_host.h"
+#include "xattn_aux.cuh"
+#include "xattn_rows.cuh"
 #include "xattn_simt.cuh"
 #include "xattn_tc.cuh"
 
@@ -22,7 +24,11 @@ constexpr size_t kDsCap = (size_t)4 << 30;
 struct XDims {
   int B, H, Hkv, G, Nq, Nk, D, DP, T, nqp, nkp;
   bool bf16;
+  int fwd_rows, bwd_rows;  // few query rows: the kernels' rows (1, 2, 4 or 8), or 0
   int splits;           // forward key splits
+  int bwd_splits;       // backward key splits (few query rows)
+  long long row_ctas;   // forward CTAs per key split (few query rows)
+  int nqb;              // query padding of the dS^T scratch
   int units_per_launch; // backward
   int launches, chunks;
   size_t ds_unit;       // dS^T bytes of one (batch, key head) unit
@@ -52,6 +58,39 @@ int forward_splits(const XDims& d) {
   return n < 1 ? 1 : (int)n;
 }
 
+// Where the kernels for few query rows (xattn_rows.cuh) take a call: how many rows a CTA holds, or 0. Their time grows
+// with the rows of a key head's group, that of the tiled kernels with its heads. Both sides measured:
+//   fp32 forward, up to 32 queries per head (a tile holds 128): 64 x 16 heads, 4096 keys of 64, 8 queries: 702 against
+//     3850 us; backward, a group of up to 8 rows: 64 x 15 / 5 heads, 2 queries, 11785 keys of 64: 2.2 against 27.6 ms.
+//   bf16 forward, one query per head: with K and V of at most 32 MB and no shared key heads (1 x 16 heads, 512 keys of
+//     192: 14.1 against 16.6 us; but 32 x 16, 4096 of 128: 234 against 166 us), or with a bias and shared key heads, whose
+//     rows the tiles do not pack (128 x 16 / 8 heads, 512 keys of 128: 79 against 100 us; groups of 8: 209 against 376).
+//   bf16 backward, one query per head: a head dim of at most 64 (32 x 16 heads of one key head each, 2048 keys: 236
+//     against 279 us; groups of 8: 507 against 852), a bias and shared key heads (groups of 4, 2048 keys of 128: 799
+//     against 969 us), or fewer heads than SMs, which dQ's tiles cannot fill (1 x 16 heads, 16384 keys of 128: 157
+//     against 232 us). Otherwise the tiles: 32 x 16 heads, 2048 keys of 128: 362 against 425 us.
+int rows_of(long long rows) { return rows > 4 ? kRowMax : rows > 2 ? 4 : (int)rows; }
+int forward_rows_of(const XDims& d) {
+  const long long rows = (long long)d.G * d.Nq;
+  if (d.bf16) {
+    const bool small = d.G == 1 && (long long)d.B * d.Hkv * d.Nk * d.D <= 8 << 20, unpacked = d.T && d.G > 1 && rows <= kRowMax;
+    return d.Nq == 1 && (small || unpacked) ? rows_of(rows) : 0;
+  }
+  return d.Nq <= 32 || rows <= kRowMax ? rows_of(rows) : 0;
+}
+int backward_rows_of(const XDims& d) {
+  const long long rows = (long long)d.G * d.Nq;
+  if (rows > kRowMax) return 0;
+  if (d.bf16 && !(d.Nq == 1 && (d.DP == 64 || (d.T && d.G > 1) || (long long)d.B * d.H < kSMs))) return 0;
+  return rows_of(rows);
+}
+// Key ranges of at least 512 keys, enough for four CTAs per SM.
+int row_splits(const XDims& d, long long ctas) {
+  const long long want = (4 * kSMs + ctas - 1) / ctas, most = d.Nk / 512;
+  const long long n = want < most ? want : most;
+  return n < 1 ? 1 : (int)n;
+}
+
 int check_xshape(const GeoXattnShape* s, XDims& d) {
   if (!s || s->batch <= 0 || s->heads <= 0 || s->kv_heads <= 0 || s->nq <= 0 || s->nk <= 0 || s->head_dim <= 0 ||
       s->heads % s->kv_heads || s->buckets < 0)
@@ -69,17 +108,25 @@ int check_xshape(const GeoXattnShape* s, XDims& d) {
   d.nkp = (d.Nk + 127) / 128 * 128;
   if (d.B > 65535 || d.H > 65535) return GEOATTN_ERR_UNSUPPORTED;  // grid of the row records
   if (d.T && (d.nqp / 64 > 65535 || d.nkp / 64 > 65535)) return GEOATTN_ERR_UNSUPPORTED;  // grid of the ids' tiles
-  d.splits = forward_splits(d);
+  d.fwd_rows = forward_rows_of(d);
+  d.bwd_rows = backward_rows_of(d);
+  d.nqb = d.bwd_rows ? 8 : d.nqp;
+  const long long row_units = (long long)d.B * d.Hkv;
+  d.row_ctas = d.fwd_rows ? ((long long)d.G * d.Nq + d.fwd_rows - 1) / d.fwd_rows * row_units : 0;
+  d.splits = d.fwd_rows ? row_splits(d, d.row_ctas) : forward_splits(d);
+  d.bwd_splits = d.bwd_rows ? row_splits(d, row_units) : 1;
+  if (d.row_ctas * d.splits > (1ll << 30)) return GEOATTN_ERR_UNSUPPORTED;
   const long long qt = (d.Nq + 63) / 64, kt = (d.Nk + 31) / 32;
   if (qt * d.B * d.H * d.splits > (1ll << 30) || kt * d.B * d.Hkv > (1ll << 30)) return GEOATTN_ERR_UNSUPPORTED;
-  d.ds_unit = (size_t)d.G * d.nkp * d.nqp * (d.bf16 ? 2 : 4);
+  d.ds_unit = d.bwd_rows && !d.T ? 0 : (size_t)d.G * d.nkp * d.nqb * (d.bf16 ? 2 : 4);
   const long long units = (long long)d.B * d.Hkv;
-  long long per = (long long)(kDsCap / d.ds_unit);
+  long long per = d.ds_unit ? (long long)(kDsCap / d.ds_unit) : units;
   per = per < 1 ? 1 : per > units ? units : per;
   d.units_per_launch = (int)per;
   d.launches = (int)((units + per - 1) / per);
-  const long long want = (16ll * kSMs + d.H - 1) / d.H, most = (long long)d.nkp * d.nqp / (d.bf16 ? 8 : 4) / 256;
-  d.chunks = (int)(want < most ? want : most);
+  const long long want = (16ll * kSMs + d.H - 1) / d.H, most = (long long)d.nkp * d.nqb / (d.bf16 ? 8 : 4) / 256;
+  
+  d.chunks = (int)(want < most ? want : most < 1 ? 1 : most);
   return GEOATTN_OK;
 }
 
@@ -102,7 +149,7 @@ size_t xfwd_ws(const XDims& d, uint8_t* base, XFwdWs* w) {
     t.part_o = reinterpret_cast<float*>(take(rows * d.D * 4));
     t.part_ml = reinterpret_cast<float*>(take(rows * 2 * 4));
   }
-  if (d.T && d.bf16) t.ids = reinterpret_cast<uint16_t*>(take((size_t)d.nqp * d.nkp * 2));
+  if (d.T && d.bf16 && !d.fwd_rows) t.ids = reinterpret_cast<uint16_t*>(take((size_t)d.nqp * d.nkp * 2));
   if (w) *w = t;
   return off;
 }
@@ -113,6 +160,7 @@ struct XBwdWs {
   void* ds;
   uint16_t* idsT;
   float* part;
+  float* part_dq;
 };
 size_t xbwd_ws(const XDims& d, uint8_t* base, XBwdWs* w) {
   size_t off = 0;
@@ -123,11 +171,13 @@ size_t xbwd_ws(const XDims& d, uint8_t* base, XBwdWs* w) {
   };
   XBwdWs t{};
   t.status = reinterpret_cast<int*>(take(sizeof(int)));
-  if (d.bf16) t.rec = reinterpret_cast<float*>(take((size_t)d.B * d.H * d.nqp * 3 * 4));
+  if (d.bwd_splits > 1) t.part_dq = reinterpret_cast<float*>(take((size_t)d.bwd_splits * d.B * d.H * d.Nq * d.D * 4));
+  if (d.bwd_rows) {
+  } else if (d.bf16) t.rec = reinterpret_cast<float*>(take((size_t)d.B * d.H * d.nqp * 3 * 4));
   else t.delta = reinterpret_cast<float*>(take((size_t)d.B * d.H * d.Nq * 4));
   t.ds = take(d.ds_unit * d.units_per_launch);
   if (d.T) {
-    t.idsT = reinterpret_cast<uint16_t*>(take((size_t)d.nkp * d.nqp * 2));
+    t.idsT = reinterpret_cast<uint16_t*>(take((size_t)d.nkp * d.nqb * 2));
     t.part = reinterpret_cast<float*>(take((size_t)d.launches * d.H * d.chunks * d.T * 4));
   }
   if (w) *w = t;
@@ -209,11 +259,46 @@ int backward_simt(const XParams& p, const XDims& d, int units, cudaStream_t st) 
   return d.DP == 64 ? simt_bwd<64>(p, units, st) : d.DP == 128 ? simt_bwd<128>(p, units, st) : simt_bwd<192>(p, units, st);
 }
 
+template <class F>
+int with_rows(int dp, int rows, F f) {
+  const auto nv = [&](auto v) {
+    return rows == 1   ? f(v, std::integral_constant<int, 1>())
+           : rows == 2 ? f(v, std::integral_constant<int, 2>())
+           : rows == 4 ? f(v, std::integral_constant<int, 4>())
+                       : f(v, std::integral_constant<int, 8>());
+  };
+  return dp == 64    ? nv(std::integral_constant<int, 1>())
+         : dp == 128 ? nv(std::integral_constant<int, 2>())
+                     : nv(std::integral_constant<int, 3>());
+}
+int forward_rows(const XParams& p, const XDims& d, cudaStream_t st) {
+  return with_rows(d.DP, d.fwd_rows, [&](auto nv, auto r) {
+    constexpr int NV = decltype(nv)::value, R = decltype(r)::value;
+    const long long grid = d.row_ctas * d.splits;
+    if (!d.bf16) return xlaunch(xattn_rows_fwd_kernel<float, NV, R>, grid, kRowThreads, 0, st, p);
+    return xlaunch(xattn_rows_fwd_kernel<__nv_bfloat16, NV, R>, grid, kRowThreads, 0, st, p);
+  });
+}
+template <class E>
+int backward_rows(const XParams& p, const XDims& d, int units, cudaStream_t st) {
+  return with_rows(d.DP, d.bwd_rows, [&](auto nv, auto r) {
+    xattn_rows_bwd_kernel<E, decltype(nv)::value, decltype(r)::value>
+        <<<(unsigned)((long long)units * d.bwd_splits), kRowThreads, 0, st>>>(p, units);
+    return status_of(cudaGetLastError());
+  });
+}
+// What the tensor-core kernels ask of their operands, asked of every bf16 call: which kernel runs is not the caller's
+// concern.
+bool tma_ok(const XTensor& t) {
+  if (reinterpret_cast<uintptr_t>(t.p) & 15) return false;
+  for (int i = 0; i < 3; ++i)
+    if (t.s[i] <= 0 || ((t.s[i] * 2) & 15)) return false;
+  return true;
+}
+
 // TMA map over a bf16 tensor [batch, heads, rows, D] (box: 64 columns x `rows` rows x `heads` heads).
 int xmap(CUtensorMap* m, const XTensor& t, int D, int n, int heads, int batch, int box_rows, int box_heads) {
-  if (reinterpret_cast<uintptr_t>(t.p) & 15) return GEOATTN_ERR_ALIGNMENT;
-  for (int i = 0; i < 3; ++i)
-    if (t.s[i] <= 0 || ((t.s[i] * 2) & 15)) return GEOATTN_ERR_ALIGNMENT;
+  if (!tma_ok(t)) return GEOATTN_ERR_ALIGNMENT;
   const uint64_t dims[4] = {(uint64_t)D, (uint64_t)n, (uint64_t)heads, (uint64_t)batch};
   const uint64_t str[3] = {(uint64_t)t.s[2] * 2, (uint64_t)t.s[1] * 2, (uint64_t)t.s[0] * 2};
   const uint32_t box[4] = {64, (uint32_t)box_rows, (uint32_t)box_heads, 1};
@@ -351,7 +436,10 @@ int geoattn_xattn_fwd(const GeoXattnFwdArgs* a, void* stream) {
   XParams p = xparams(a->in, d);
   p.o = xt(a->o, a->o_stride), p.stats = reinterpret_cast<float2*>(a->stats);
   p.splits = d.splits, p.part_o = ws.part_o, p.part_ml = ws.part_ml, p.status = ws.status;
-  int rc = d.bf16 ? forward_tc(p, d, ws.ids, st) : forward_simt(p, d, st);
+  if (d.bf16 && !(tma_ok(p.q) && tma_ok(p.k) && tma_ok(p.v))) return GEOATTN_ERR_ALIGNMENT;
+  int rc = d.fwd_rows ? forward_rows(p, d, st)
+           : d.bf16   ? forward_tc(p, d, ws.ids, st)
+                      : forward_simt(p, d, st);
   if (rc || d.splits == 1) return rc;
   const long long rows = (long long)d.B * d.H * d.Nq;
   return d.bf16 ? xlaunch(xattn_combine_kernel<__nv_bfloat16>, (rows + 7) / 8, 256, 0, st, p)
@@ -378,28 +466,39 @@ int geoattn_xattn_bwd(const GeoXattnBwdArgs* a, void* stream) {
   p.dq = xt(a->dq, a->dq_stride), p.dk = xt(a->dk, a->dk_stride), p.dv = xt(a->dv, a->dv_stride);
   p.stats = reinterpret_cast<float2*>(const_cast<float*>(a->stats)), p.delta = ws.delta, p.rec = ws.rec, p.ds = ws.ds;
   p.idsT = ws.idsT, p.status = ws.status;
+  p.nqp = d.nqb, p.splits = d.bwd_splits, p.part_o = ws.part_dq;
+  if (d.bf16 && !(tma_ok(p.q) && tma_ok(p.k) && tma_ok(p.v) && tma_ok(p.dout))) return GEOATTN_ERR_ALIGNMENT;
   xa::XMaps maps;
   std::memset(&maps, 0, sizeof(maps));
-  int rc = d.bf16 ? backward_maps(maps, p, d) : GEOATTN_OK;
+  int rc = d.bf16 && !d.bwd_rows ? backward_maps(maps, p, d) : GEOATTN_OK;
   if (rc) return rc;
-  rc = d.bf16 ? records(p, d, st)
-              : xlaunch(xattn_delta_kernel, ((long long)d.B * d.H * d.Nq + 31) / 32, 256, 0, st, p);
+  rc = d.bwd_rows ? GEOATTN_OK
+       : d.bf16   ? records(p, d, st)
+                  : xlaunch(xattn_delta_kernel, ((long long)d.B * d.H * d.Nq + 31) / 32, 256, 0, st, p);
   if (rc) return rc;
   if (d.T) {
-    ids_tile_kernel<true><<<dim3(d.nqp / 64, d.nkp / 64), 256, 0, st>>>(p.ids, p.ids_ld, d.Nq, d.Nk, d.nqp, d.T, ws.idsT);
+    ids_tile_kernel<true><<<dim3((d.nqb + 63) / 64, d.nkp / 64), 256, 0, st>>>(p.ids, p.ids_ld, d.Nq, d.Nk, d.nqb, d.T, ws.idsT);
     if ((rc = status_of(cudaGetLastError()))) return rc;
   }
   const int units = d.B * d.Hkv;
   for (int l = 0; l < d.launches; ++l) {
     p.u0 = l * d.units_per_launch;
     const int nu = units - p.u0 < d.units_per_launch ? units - p.u0 : d.units_per_launch;
-    rc = d.bf16 ? backward_tc(maps, p, d, nu, st) : backward_simt(p, d, nu, st);
+    rc = d.bwd_rows ? d.bf16 ? backward_rows<__nv_bfloat16>(p, d, nu, st) : backward_rows<float>(p, d, nu, st)
+         : d.bf16   ? backward_tc(maps, p, d, nu, st)
+                    : backward_simt(p, d, nu, st);
     if (rc) return rc;
     if (d.T) {
       float* part = ws.part + (size_t)l * d.H * d.chunks * d.T;
       rc = d.bf16 ? table_grad<__nv_bfloat16>(p, d, nu, part, st) : table_grad<float>(p, d, nu, part, st);
       if (rc) return rc;
     }
+  }
+  if (d.bwd_splits > 1) {
+    const long long grid = ((long long)d.B * d.H * d.Nq * d.D + 255) / 256;
+    rc = d.bf16 ? xlaunch(xattn_rows_dq_sum_kernel<__nv_bfloat16>, grid, 256, 0, st, p)
+                : xlaunch(xattn_rows_dq_sum_kernel<float>, grid, 256, 0, st, p);
+    if (rc) return rc;
   }
   if (d.T) {
     table_grad_sum_kernel<<<d.H * d.T, 32, 0, st>>>(ws.part, d.launches, d.H, d.chunks, d.T, a->dtable,

@@ -48,6 +48,7 @@ __global__ void __launch_bounds__(256) ids_tile_kernel(const uint8_t* __restrict
   uint4* dst = reinterpret_cast<uint4*>(out) + ((long long)blockIdx.y * (cols_p / 8) + c0 / 8) * 64;
   for (int x = threadIdx.x; x < 64 * 8; x += 256) {
     const int r = x % 64, g = x / 64;
+    if (c0 + g * 8 >= cols_p) break;
     uint32_t w[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -80,7 +81,7 @@ __global__ void __launch_bounds__(256) table_grad_kernel(const XParams p, int un
   for (long long x = c0 + threadIdx.x; x < c1; x += 256) {
     const long long at = x * VEC;
     const int j = (int)(at / (64ll * p.nqp)) * 64 + (int)(at / 8 % 64);
-    const bool held = (int)(at / 512 % (p.nqp / 8)) * 8 < p.Nq;
+    if ((int)(at / 512 % (p.nqp / 8)) * 8 >= p.Nq) continue;  // granules without a query hold nothing
     const S* src = reinterpret_cast<const S*>(p.ds) + (long long)(first * p.G + h % p.G) * slab + at;
     float sum[VEC];
 #pragma unroll
@@ -90,8 +91,8 @@ __global__ void __launch_bounds__(256) table_grad_kernel(const XParams p, int un
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int u = ul + k * p.Hkv;
-        // keys that the key pass left out hold nothing, and so do granules without a query
-        w[k] = held && u < units && j < key_count(p, (p.u0 + u) / p.Hkv) ? __ldcs(reinterpret_cast<const uint4*>(src + k * step))
+        // keys that the key pass left out hold nothing
+        w[k] = u < units && j < key_count(p, (p.u0 + u) / p.Hkv) ? __ldcs(reinterpret_cast<const uint4*>(src + k * step))
                                                                  : make_uint4(0, 0, 0, 0);
       }
       src += 8 * step;

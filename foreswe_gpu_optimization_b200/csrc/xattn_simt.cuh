@@ -9,6 +9,7 @@
 #pragma once
 #include <type_traits>
 
+#include "sm100.cuh"
 #include "xattn_common.cuh"
 
 namespace geoattn {
@@ -115,6 +116,7 @@ __global__ void __launch_bounds__(SimtFwd<DP>::NT, DP == 64 ? 2 : 1) xattn_simt_
   const float* K = reinterpret_cast<const float*>(p.k.p) + b * p.k.s[0] + kh * p.k.s[1];
   const float* V = reinterpret_cast<const float*>(p.v.p) + b * p.v.s[0] + kh * p.v.s[1];
   const bool vq = simt_vec(p.q, p.D), vk = simt_vec(p.k, p.D), vv = simt_vec(p.v, p.D);
+  if (blockIdx.x + threadIdx.x == 0) *p.status = kDevOk;
   const AttnDrop drop = attn_drop(p.rng, p.drop_thr, p.drop_scale);
 
   if (p.ids)
@@ -328,6 +330,7 @@ __global__ void __launch_bounds__(256) xattn_delta_kernel(const XParams p) {
   const long long rows = (long long)p.B * p.H * p.Nq;
   const long long row = (long long)blockIdx.x * 32 + threadIdx.x / 8;
   const int lane = threadIdx.x % 8;
+  if (blockIdx.x + threadIdx.x == 0) *p.status = kDevOk;
   float x = 0.f;
   if (row < rows) {
     const int i = (int)(row % p.Nq), bh = (int)(row / p.Nq), h = bh % p.H, b = bh / p.H;

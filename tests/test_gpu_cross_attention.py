@@ -457,6 +457,77 @@ def test_query_counts_around_the_chunks():
             check(x, kw, p=0.1, key=[Nq, D])
 
 
+FEW = [  # B, H, Hkv, Nq, Nk, D: few query rows per key head, every row count of a CTA, one and several key ranges
+    (3, 2, 2, 1, 1, 64), (2, 2, 2, 1, 63, 40), (1, 2, 2, 1, 1100, 64), (2, 4, 2, 1, 2051, 128), (1, 3, 1, 1, 1030, 192),
+    (2, 6, 2, 1, 130, 100), (1, 5, 1, 1, 1500, 61), (2, 8, 1, 1, 700, 192), (1, 2, 2, 2, 1029, 128), (2, 4, 1, 2, 90, 64),
+    (2, 2, 2, 7, 300, 175), (1, 2, 2, 8, 1025, 64), (2, 3, 3, 9, 70, 64), (1, 6, 2, 28, 1200, 192), (1, 8, 1, 32, 130, 33),
+    (2, 2, 1, 31, 1, 128),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("shape", FEW, ids=lambda s: "x".join(map(str, s)))
+def test_few_rows(shape, dtype):
+    B, H, Hkv, Nq, Nk, D = shape
+    check(*make(*shape, dtype, seed=31))
+    lens = [0 if B > 1 and b == 0 else max(1, Nk - 7 * b) for b in range(B)]
+    x, kw = make(*shape, dtype, seed=32, T=9, lens=lens, mask=Nk > 1, cut=Nk > 1)
+    check(x, kw, p=0.2, key=[99, 7])
+
+
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("Nq, G", [(1, 1), (1, 4), (3, 2)])
+def test_few_rows_garbage_and_guards(Nq, G, dtype):
+    """NaN in absent keys and infinity in absent values; gradients land inside their tensors and nowhere else."""
+    import foreswe_gpu_optimization_b200 as g
+    B, Hkv, Nk, D = 2, 2, 600, 72
+    x, kw = make(B, Hkv * G, Hkv, Nq, Nk, D, dtype, seed=33, lens=[600, 517], mask=True)
+    dead = ~ox.live_keys(B, Nk, kw["lens"], kw["mask"])
+    clean = {n: t.clone() for n, t in x.items()}
+    for n, bad in (("k", float("nan")), ("v", float("inf"))):
+        clean[n] = x[n].masked_fill(dead.view(B, 1, Nk, 1), 0.0)
+        x[n] = x[n].masked_fill(dead.view(B, 1, Nk, 1), bad)
+    got, want = run(x, kw), run(clean, kw)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+    assert got["dk"].masked_select(dead.view(B, 1, Nk, 1)).eq(0).all()
+    # a query that is NaN gives NaN in its own row only
+    y = {n: t.cuda() for n, t in clean.items()}
+    y["q"][0, 0, 0, 3] = float("nan")
+    o = g.cross_attention(y["q"], y["k"], y["v"], kv_lens=kw["lens"].cuda(), key_mask=kw["mask"].cuda())
+    assert o[0, 0, 0].isnan().all() and o.isnan().sum() == D
+
+
+def test_few_rows_repeat_bitwise_and_replay():
+    """The same call twice, and captured and replayed on changed inputs, with key ranges that are joined."""
+    import foreswe_gpu_optimization_b200 as g
+    for dtype in (BF, FP):
+        x, _ = make(1, 2, 2, 1, 5000, 64, dtype, seed=34)
+        y = {n: t.cuda() for n, t in x.items()}
+        for n in "qkv":
+            y[n] = y[n].detach().requires_grad_()
+
+        def step():
+            o = g.cross_attention(y["q"], y["k"], y["v"])
+            return (o.detach(), *torch.autograd.grad(o, [y[n] for n in "qkv"], y["do"]))
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            first = step()
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(a, b) for a, b in zip(first, step()))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        with torch.no_grad():
+            y["k"].mul_(0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
 def test_many_key_tiles_per_cta():
     """More key tiles than the persistent key pass has CTAs, some of them past their batch entry's length."""
     for D, Nq in ((64, 40), (64, 130), (128, 20), (128, 300), (192, 33)):
