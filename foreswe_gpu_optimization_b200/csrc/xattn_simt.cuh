@@ -5,7 +5,10 @@
 // keys) are one or two 16-byte loads per d; each of the 256 threads (16 x 16) owns a register block of the product and
 // works on it two values at a time (fma.rn.f32x2). Weights go through shared memory between the two products, in
 // 16-byte chunks whose place is XORed with the writing lane so that neither side meets a bank conflict.
-// Bound by the FMA pipe.
+// Bound by shared memory's return path (one 32-bit word per lane and clock: as long as the products themselves) and,
+// above D = 64, by the latency that 8 warps per SM cannot hide. 32 x 8 heads x 512 x 512 x 64 with the bias: forward
+// 542 us (32 TFLOP/s of 74), key pass 1163 us (30), dQ 290 us (30); at D = 175 forward and key pass run at 19 and 18. Fetching
+// the next query tile during the products changed nothing there.
 #pragma once
 #include <type_traits>
 
@@ -273,8 +276,8 @@ __global__ void __launch_bounds__(SimtFwd<DP>::NT, DP == 64 ? 2 : 1) xattn_simt_
   }
 }
 
-// Join the key splits of each row: one warp per row. The splits' weights are worked out by the lanes side by side (32 at
-// a time) and handed round; a lane sums 4 consecutive columns.
+// Join the key splits of each row: one warp per row. The splits' weights are worked out by the lanes side by side (32
+// at a time) and handed round; a lane sums 4 consecutive columns. 16 x 32 heads x 4 rows of 128, 5 splits: 6 us.
 template <class E>
 __global__ void __launch_bounds__(256) xattn_combine_kernel(const XParams p) {
   const long long rows = (long long)p.B * p.H * p.Nq;

@@ -2,9 +2,12 @@
 // in tensor memory. Shared-memory tiles are regions of rows x 128 bytes (64 head-dim columns), one region per 64
 // columns of the padded head dim DP (64, 128, 192); TMA fills rows and columns past the tensor with zeros.
 //
-// Every product has M = 128 (the rows of a tile sit in the 128 lanes of tensor memory, one thread per row), and the
-// CTAs are sized so that two share an SM (at most 256 tensor-memory columns and 113 KB each): one CTA's element-wise
-// work overlaps the other's products, loads, prologue and epilogue.
+// Every product has M = 128 (the rows of a tile sit in the 128 lanes of tensor memory, one thread per row). The CTAs of
+// the forward and of dQ are sized so that two share an SM (at most 256 tensor-memory columns and 113 KB each): one CTA's
+// element-wise work overlaps the other's products, loads, prologue and epilogue. The key pass fills tensor memory with
+// one CTA and is persistent instead.
+//
+// Times are of single launches at the burst clock; BxHxNqxNkxD gives the sizes.
 #pragma once
 #include "sm100.cuh"
 #include "xattn_common.cuh"
@@ -150,9 +153,16 @@ __device__ __forceinline__ bool vec_rows(const XTensor& t) {
 //                  in bf16 over the scores it came from
 // m is one per row and moves only when a chunk would pass it by more than kLazy (P stays below 2^kLazy; l and O are
 // fp32): one barrier per chunk tells the two warps of 32 rows whether any of them has to move, and only then do they
-// exchange their maxima and rescale O, after O's product c - 1 (the only one that can be in flight: S(c) was issued after c - 2).
+// exchange their maxima and rescale O, after O's product c - 1 (the only one that can be in flight: S(c) was issued
+// after c - 2).
 // Few queries of heads that share a key head (G * Nq <= 128) are packed into one tile's rows.
 // DP = 192 has room for one score buffer and one chunk of K and V; S(c + 1) then follows O's product c.
+// Measured: 256x16x512x512x128 with the bias 886 us (620 TFLOP/s, 2.8x its products' time), 32x16x700x512x64 with the
+// bias and a mask 192 us, 1x8x4096x8192x128 160 us (859 TFLOP/s; 237 with dropout), 32x16x512x512x192 with bias and
+// dropout 255 us: bound by the products' operand feed (a 64-key score product reads as many shared-memory bytes as it has
+// time for) and the chain from scores to weights. 16x(32/8)x4x16384x128 with lengths 146 us: 5.3 TB/s of K and V.
+// 128-key chunks, one warpgroup per tile, a barrier per half of P, and maxima exchanged a chunk ahead were built and were
+// 5 to 25 % slower at D = 128.
 // ---------------------------------------------------------------------------------------------------------------
 template <int DP>
 struct FwdCfg {
@@ -438,7 +448,8 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
 // Backward, row records: chunks of 64 query rows, rec[b*h][chunk][3][64] floats:
 //   without the bias  -(m + log2 l), unused, -delta       with it  -m, 1 / l, -delta (the bias may dwarf log2 l)
 // so that P = 2^(t + rec0) or 2^(t + rec0) rec1; rows past Nq and rows with nothing left get P = 0. Bound by reading o
-// and dO once: rows are taken in the order they lie in memory, with 8 loads of 16 bytes in flight per lane.
+// and dO once: rows are taken in the order they lie in memory, with 8 loads of 16 bytes in flight per lane (256x16x512
+// rows of 128: 197 us, 5.5 TB/s; 297 us with one or two loads in flight).
 // ---------------------------------------------------------------------------------------------------------------
 template <int LPR>  // lanes per row: 8 columns each
 __global__ void __launch_bounds__(256) xattn_records_kernel(const XParams p, int heads_first) {
@@ -506,6 +517,8 @@ __global__ void __launch_bounds__(256) xattn_records_kernel(const XParams p, int
 //   MMA warp       dV(c), S^T(c + 1), dK(c), dP^T(c + 1), each as soon as what it reads is there and what it overwrites
 //                  has been read by the product before it
 //   4 warpgroups   P of chunk c while dK(c - 1) and dP^T(c) run, then dS of chunk c while dV(c) and S^T(c + 1) run
+// Measured: 256x16x512x512x128 with the bias 1517 us (725 TFLOP/s), 1x8x4096x8192x128 with dropout 346 us (795),
+// 32x16x512x512x192 with bias and dropout 328 us, 32x8x384x512x64 with dropout and lengths 73 us.
 // Bound by the operand feed of the products (S and dP 64 clocks per 16 of the head dim and 128 queries, dV and dK as
 // many per 16 queries at DP = 128): chunks of 128 queries, which halve K's and V's share of it, with one score buffer
 // (S 128, dP 128, dK 128, dV 128 columns) beat chunks of 64 with two. DP = 192 has columns for 64 queries.
@@ -876,7 +889,8 @@ __global__ void __launch_bounds__(KeysCfg<DP, BQ_>::THREADS, 1)
 // dQ = scale dS K from the dS scratch: one CTA per (128 queries, head of the launch's units), over 64-key chunks. The
 // scratch's granules of 8 queries x 64 keys are the tensor core's unswizzled tiles with M contiguous (8 x 8 matrices of
 // 128 bytes, 8 keys apart by 128 and 8 queries apart by 1024), so a chunk's A operand is one contiguous copy of 16 KB.
-// Bound by reading the scratch. Two of the epilogue's warps clear the rows of absent keys first (0 * NaN).
+// Bound by reading the scratch (256x16x512x512x128: 548 us for 2.1 GB of dS, 0.5 of K and 0.5
+// of dQ: 5.9 TB/s). Two of the epilogue's warps clear the rows of absent keys first (0 * NaN).
 // ---------------------------------------------------------------------------------------------------------------
 template <int DP>
 struct DqCfg {
