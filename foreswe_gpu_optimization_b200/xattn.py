@@ -134,6 +134,7 @@ def cross_attention(q, k, v, *, buckets=None, bias_table=None, kv_lens=None, key
         What absent keys hold is not used (NaN included) and their gradients are zero.
     dropout_p, rng: dropout on the attention weights; rng as in `dropout`.
     scale: of the scores, positive, 1/sqrt(D) by default.
+    At most 65535 batch entries and 65535 heads.
     A row with no key left gives zeros. Differentiable (once) in q, k, v and bias_table; the results do not depend on
     the order of any concurrent sums."""
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
@@ -174,8 +175,12 @@ def cross_attention(q, k, v, *, buckets=None, bias_table=None, kv_lens=None, key
         if t is not None and t.device != dev:
             raise ValueError("%s lives on %s, q on %s" % (name, t.device, dev))
     key = _snapshot(rng, dev) if thr else None
-    if q.numel() == 0:  # no batch, head, query or head dim: nothing to launch
-        return q * 1.0
+    if q.numel() == 0:  # no batch, head, query or head dim: nothing to launch, and zero gradients
+        o = q * 1.0
+        for t in (k, v, bias_table):
+            if t is not None and t.requires_grad and torch.is_grad_enabled():
+                o = o + (t.flatten()[:0].sum() * 0.0).to(o.dtype)
+        return o
     if bias_table is not None:
         if bias_table.shape[0] != H:
             bias_table = bias_table.expand(H, -1)
@@ -183,7 +188,9 @@ def cross_attention(q, k, v, *, buckets=None, bias_table=None, kv_lens=None, key
         if buckets.stride(1) != 1 or buckets.stride(0) < Nk:
             buckets = buckets.contiguous()
     if kv_lens is not None:
-        kv_lens = (kv_lens if kv_lens.dtype == torch.int32 else kv_lens.to(torch.int32)).contiguous()
+        if kv_lens.dtype == torch.int64:
+            kv_lens = kv_lens.clamp(0, Nk).to(torch.int32)  # clamped before it narrows
+        kv_lens = kv_lens.contiguous()
     if key_mask is not None and (key_mask.stride(1) != 1 or key_mask.stride(0) < Nk):
         key_mask = key_mask.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or

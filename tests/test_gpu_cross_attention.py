@@ -249,6 +249,25 @@ def test_empty_inputs():
     assert g.dropout(torch.empty(0, 4, device="cuda"), 0.5, g.CounterRNG(1)).shape == (0, 4)
 
 
+def test_empty_queries_give_zero_gradients():
+    import foreswe_gpu_optimization_b200 as g
+    for B, Nq in ((2, 0), (0, 3)):
+        q, k = torch.randn(B, 2, Nq, 8, device="cuda"), torch.randn(B, 2, 4, 8, device="cuda")
+        x = [t.requires_grad_(True) for t in (q, k, k.clone(), torch.randn(2, 5, device="cuda"))]
+        o = g.cross_attention(*x[:3], buckets=torch.zeros(Nq, 4, dtype=torch.uint8, device="cuda"), bias_table=x[3])
+        assert o.shape == q.shape
+        for t, d in zip(x, torch.autograd.grad(o.sum(), x)):
+            assert d.shape == t.shape and (d == 0).all()
+
+
+def test_lengths_beyond_32_bits_are_clamped():
+    import foreswe_gpu_optimization_b200 as g
+    x, _ = make(3, 2, 2, 20, 70, 32, BF, seed=22)
+    q, k, v = (x[n].cuda() for n in "qkv")
+    got = g.cross_attention(q, k, v, kv_lens=torch.tensor([2 ** 32, -2 ** 40, 2 ** 32 + 5], device="cuda"))
+    assert torch.equal(got, g.cross_attention(q, k, v, kv_lens=torch.tensor([70, 0, 70], device="cuda")))
+
+
 @pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp32"])
 def test_long_keys_with_few_rows(dtype):
     """Key ranges of one row are split over the GPU and joined: ragged lengths, one of them shorter than a range."""
