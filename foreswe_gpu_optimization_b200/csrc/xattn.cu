@@ -27,6 +27,7 @@ struct XDims {
   int fwd_rows, bwd_rows;  // few query rows: the kernels' rows (1, 2, 4 or 8), or 0
   int splits;           // forward key splits
   int bwd_splits;       // backward key splits (few query rows)
+  int tail;             // fp32 forward: queries behind the last whole tile that the few-row kernel takes, or 0
   long long row_ctas;   // forward CTAs per key split (few query rows)
   int nqb;              // query padding of the dS^T scratch
   int units_per_launch; // backward
@@ -38,7 +39,7 @@ bool packs_rows(const XDims& d) { return d.bf16 && d.G > 1 && d.T == 0 && (long 
 
 int forward_splits(const XDims& d) {
   // Enough key ranges to give every SM a tile when the rows alone do not.
-  const long long tiles = packs_rows(d) ? (long long)d.B * d.Hkv : (long long)((d.Nq + 127) / 128) * d.B * d.H;
+  const long long tiles = packs_rows(d) ? (long long)d.B * d.Hkv : (long long)((d.Nq - d.tail + 127) / 128) * d.B * d.H;
   const int ktiles = (d.Nk + 63) / 64;
   if (tiles >= kSMs) return 1;
   long long want, most;
@@ -61,7 +62,8 @@ int forward_splits(const XDims& d) {
 // Where the kernels for few query rows (xattn_rows.cuh) take a call: how many rows a CTA holds, or 0. Their time grows
 // with the rows of a key head's group, that of the tiled kernels with its heads. Both sides measured:
 //   fp32 forward, up to 32 queries per head (a tile holds 128): 64 x 16 heads, 4096 keys of 64, 8 queries: 702 against
-//     3850 us; backward, a group of up to 8 rows: 64 x 15 / 5 heads, 2 queries, 11785 keys of 64: 2.2 against 27.6 ms.
+//     3850 us; the queries behind the last whole tile where they are no more (8 x 8 heads, 130 queries, 517 keys of 48:
+//     106 -> 78 us); backward, a group of up to 8 rows: 64 x 15 / 5 heads, 2 queries, 11785 keys of 64: 2.2 against 27.6 ms.
 //   bf16 forward, one query per head: with K and V of at most 32 MB and no shared key heads (1 x 16 heads, 512 keys of
 //     192: 14.1 against 16.6 us; but 32 x 16, 4096 of 128: 234 against 166 us), or with a bias and shared key heads,
 //     whose rows the tiles do not pack (128 x 16 / 8 heads, 512 keys of 128: 79 against 100 us; groups of 8: 209
@@ -72,7 +74,8 @@ int forward_splits(const XDims& d) {
 //     against 232 us). Otherwise the tiles: 32 x 16 heads, 2048 keys of 128: 362 against 425 us.
 int rows_of(long long rows) { return rows > 4 ? kRowMax : rows > 2 ? 4 : (int)rows; }
 int forward_rows_of(const XDims& d) {
-  const long long rows = (long long)d.G * d.Nq;
+  const long long rows = (long long)d.G * (d.tail ? d.tail : d.Nq);
+  if (d.tail) return rows_of(rows);
   if (d.bf16) {
     const bool small = d.G == 1 && (long long)d.B * d.Hkv * d.Nk * d.D <= 8 << 20;
     const bool unpacked = d.T && d.G > 1 && rows <= kRowMax;
@@ -110,12 +113,13 @@ int check_xshape(const GeoXattnShape* s, XDims& d) {
   d.nkp = (d.Nk + 127) / 128 * 128;
   if (d.B > 65535 || d.H > 65535) return GEOATTN_ERR_UNSUPPORTED;  // grid of the row records
   if (d.T && (d.nqp / 64 > 65535 || d.nkp / 64 > 65535)) return GEOATTN_ERR_UNSUPPORTED;  // grid of the ids' tiles
+  d.tail = !d.bf16 && d.Nq > 128 && d.Nq % 128 <= 32 ? d.Nq % 128 : 0;
   d.fwd_rows = forward_rows_of(d);
   d.bwd_rows = backward_rows_of(d);
   d.nqb = d.bwd_rows ? 8 : d.nqp;
   const long long row_units = (long long)d.B * d.Hkv;
-  d.row_ctas = d.fwd_rows ? ((long long)d.G * d.Nq + d.fwd_rows - 1) / d.fwd_rows * row_units : 0;
-  d.splits = d.fwd_rows ? row_splits(d, d.row_ctas) : forward_splits(d);
+  d.row_ctas = d.fwd_rows ? ((long long)d.G * (d.tail ? d.tail : d.Nq) + d.fwd_rows - 1) / d.fwd_rows * row_units : 0;
+  d.splits = d.fwd_rows && !d.tail ? row_splits(d, d.row_ctas) : forward_splits(d);
   d.bwd_splits = d.bwd_rows ? row_splits(d, row_units) : 1;
   if (d.row_ctas * d.splits > (1ll << 30)) return GEOATTN_ERR_UNSUPPORTED;
   const long long qt = (d.Nq + 63) / 64, kt = (d.Nk + 31) / 32;
@@ -230,6 +234,7 @@ XParams xparams(const GeoXattnInputs& a, const XDims& d) {
   p.drop_scale = (float)(65536.0 / (65536 - a.drop_threshold));
   p.scale = a.scale, p.scale_log2 = (float)((double)a.scale * 1.4426950408889634);
   p.nqp = d.nqp, p.nkp = d.nkp, p.splits = 1;
+  p.q0 = 0, p.rq = d.Nq;
   return p;
 }
 
@@ -243,10 +248,11 @@ int xlaunch(K kernel, long long grid, int threads, int smem, cudaStream_t st, co
 
 template <int DP>
 int simt_fwd(const XParams& p, cudaStream_t st) {
-  return xlaunch(xattn_simt_fwd_kernel<DP>, (long long)((p.Nq + 127) / 128) * p.B * p.H * p.splits,
+  return xlaunch(xattn_simt_fwd_kernel<DP>, (long long)p.tiles * p.B * p.H * p.splits,
                  SimtFwd<DP>::NT, SimtFwd<DP>::SMEM, st, p);
 }
-int forward_simt(const XParams& p, const XDims& d, cudaStream_t st) {
+int forward_simt(XParams& p, const XDims& d, cudaStream_t st) {
+  p.tiles = (d.Nq - d.tail + 127) / 128;
   return d.DP == 64 ? simt_fwd<64>(p, st) : d.DP == 128 ? simt_fwd<128>(p, st) : simt_fwd<192>(p, st);
 }
 template <int DP>
@@ -440,9 +446,11 @@ int geoattn_xattn_fwd(const GeoXattnFwdArgs* a, void* stream) {
   p.o = xt(a->o, a->o_stride), p.stats = reinterpret_cast<float2*>(a->stats);
   p.splits = d.splits, p.part_o = ws.part_o, p.part_ml = ws.part_ml, p.status = ws.status;
   if (d.bf16 && !(tma_ok(p.q) && tma_ok(p.k) && tma_ok(p.v))) return GEOATTN_ERR_ALIGNMENT;
+  if (d.tail) p.q0 = d.Nq - d.tail, p.rq = d.tail;
   int rc = d.fwd_rows ? forward_rows(p, d, st)
            : d.bf16   ? forward_tc(p, d, ws.ids, st)
                       : forward_simt(p, d, st);
+  if (!rc && d.tail) rc = forward_simt(p, d, st);
   if (rc || d.splits == 1) return rc;
   const long long rows = (long long)d.B * d.H * d.Nq;
   return d.bf16 ? xlaunch(xattn_combine_kernel<__nv_bfloat16>, (rows + 7) / 8, 256, 0, st, p)

@@ -46,7 +46,8 @@ struct XParams {
   void* ds;                 // dS of the launch's units, [unit * G + head][key / 64][query / 8][key % 64][8] (padded)
   int nqp, nkp;             // Nq, Nk rounded up to 64 and 128
   int u0;                   // first (batch, key head) unit of this launch
-  int tiles;                // key tiles of the launch (key pass, tensor cores)
+  int tiles;                // key tiles of the launch (key pass, tensor cores); query tiles (fp32 forward)
+  int q0, rq;               // few-row kernels: first query and number of queries per head
   int out_tma;              // bit x: output x leaves through TMA stores (o; or dq, dk, dv)
   int pack;                 // forward, tensor cores: a tile holds the G * Nq rows of a key head's group
   int splits;               // > 1: key ranges per row, joined by xattn_combine_kernel

@@ -1,6 +1,6 @@
 // Cross attention for a few query rows per key head (G * Nq <= 8: single tokens, a handful of sites): both types, one
 // pass over K and V forward, and one over K, V, dK and dV backward. In fp32 also for up to 32 queries per head
-// forward, 8 rows per CTA.
+// forward, 8 rows per CTA, and for the queries behind the last whole tile where there are as few.
 //
 // Such calls are bound by reading K and V; a tile of 64 or 128 query rows would be mostly padding. 16 lanes hold one
 // key's row of K and V (4 columns per lane and 64 of the head dim) straight from global memory, no shared memory
@@ -224,8 +224,8 @@ __device__ __forceinline__ void stage_rows(const XParams& p, const XTensor& t, i
     const int r = x / (NV * kRowLanes), d = x % (NV * kRowLanes) * 4;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     const int g = first + r;  // row of the group
-    if (g < p.G * p.Nq)
-      v = load4<E>(row_at<const E>(t, b, kh * p.G + g / p.Nq, g % p.Nq), d, p.D, vec);
+    if (g < p.G * p.rq)
+      v = load4<E>(row_at<const E>(t, b, kh * p.G + g / p.rq, p.q0 + g % p.rq), d, p.D, vec);
     dst[r][d / 4] = v;
   }
 }
@@ -247,13 +247,13 @@ __global__ void __launch_bounds__(kRowThreads) xattn_rows_fwd_kernel(const XPara
   __shared__ float4 slot[kRowWarps / 2][R][NV * kRowLanes];
   __shared__ float tab[kRowMax][kMaxBuckets];
   __shared__ float sm_m[kRowWarps][R], sm_l[kRowWarps][R];
-  const int rows = p.G * p.Nq, parts = (rows + R - 1) / R, first = blockIdx.x % parts * R;
+  const int rows = p.G * p.rq, parts = (rows + R - 1) / R, first = blockIdx.x % parts * R;
   const int units = p.B * p.Hkv, unit = blockIdx.x / parts % units, split = blockIdx.x / parts / units;
   const int b = unit / p.Hkv, kh = unit % p.Hkv;
   const int warp = threadIdx.x / 32, half = threadIdx.x / 16 % 2, lane = threadIdx.x % 16;
   const int idx = lane / C::REP, y0 = idx % KB, r0 = idx / KB;  // this lane's key of the step and row
   const bool row = first + r0 < rows;
-  const int hg = row ? (first + r0) / p.Nq : 0, h = kh * p.G + hg, i = row ? (first + r0) % p.Nq : 0;
+  const int hg = row ? (first + r0) / p.rq : 0, h = kh * p.G + hg, i = p.q0 + (row ? (first + r0) % p.rq : 0);
   if (blockIdx.x + threadIdx.x == 0) *p.status = kDevOk;
   const AttnDrop drop = attn_drop(p.rng, p.drop_thr, p.drop_scale);
   const int n = key_count(p, b);
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kRowThreads) xattn_rows_fwd_kernel(const XPara
   row_range(p, p.splits, split, k0, k1);
   k1 = min(k1, n);
   stage_rows<E, NV, R>(p, p.q, b, kh, first, qs);
-  stage_tables(p, kh, first / p.Nq, tab);
+  stage_tables(p, kh, first / p.rq, tab);
   __syncthreads();
   const E *K = row_at<const E>(p.k, b, kh, 0), *V = row_at<const E>(p.v, b, kh, 0);
   const bool vk = row_vec<E>(p.k), vv = row_vec<E>(p.v);
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(kRowThreads) xattn_rows_fwd_kernel(const XPara
     float x = row_scores<NV, R, KB>(qs, k, lane) * p.scale_log2;
     if (p.ids && live) {
       const int id = p.ids[i * p.ids_ld + j];
-      x += id < p.T ? tab[hg - first / p.Nq][id] : -INFINITY;
+      x += id < p.T ? tab[hg - first / p.rq][id] : -INFINITY;
     }
     if (!live) x = -INFINITY;
     float top = x;
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kRowThreads) xattn_rows_fwd_kernel(const XPara
   for (int r = 0; r < R; ++r) {
     const float lr = __shfl_sync(0xffffffffu, ls, from(r)), mr = __shfl_sync(0xffffffffu, top, from(r));
     if (first + r >= rows || half) continue;
-    const int hr = kh * p.G + (first + r) / p.Nq, ir = (first + r) % p.Nq;
+    const int hr = kh * p.G + (first + r) / p.rq, ir = p.q0 + (first + r) % p.rq;
     const long long at = (long long)(b * p.H + hr) * p.Nq + ir;
     const float inv = p.splits > 1 ? 1.f : lr == 0.f ? 0.f : (p.drop_thr ? p.drop_scale : 1.f) / lr;
 #pragma unroll

@@ -106,8 +106,7 @@ __global__ void __launch_bounds__(SimtFwd<DP>::NT, DP == 64 ? 2 : 1) xattn_simt_
   float* pt = kv + DP * C::SK;
   float* tab = pt + C::BN * C::BM;
   float* live = tab + 256;
-  const int nqt = (p.Nq + C::BM - 1) / C::BM;
-  const int qt_i = blockIdx.x % nqt, rest = blockIdx.x / nqt;
+  const int qt_i = blockIdx.x % p.tiles, rest = blockIdx.x / p.tiles;
   const int h = rest % p.H, b = (rest / p.H) % p.B, split = rest / p.H / p.B;
   const int kh = h / p.G, i0 = qt_i * C::BM, bh = b * p.H + h;
   const int ty = threadIdx.x / XT, tx = threadIdx.x % XT;
