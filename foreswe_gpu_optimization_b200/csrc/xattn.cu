@@ -35,7 +35,11 @@ struct XDims {
   size_t ds_unit;       // dS^T bytes of one (batch, key head) unit
 };
 
-bool packs_rows(const XDims& d) { return d.bf16 && d.G > 1 && d.T == 0 && (long long)d.G * d.Nq <= 128; }
+// The few rows of heads that share a key head in one tile: K and V are read once per key head (128 x 64 / 8 heads, 1 query,
+// 4096 keys of 128 with the bias: 380 against 2114 us).
+bool packs_rows(const XDims& d) {
+  return d.bf16 && d.G > 1 && (long long)d.G * d.Nq <= 128 && (d.T == 0 || d.G <= xa::kPackTables);
+}
 
 int forward_splits(const XDims& d) {
   // Enough key ranges to give every SM a tile when the rows alone do not.
@@ -62,12 +66,12 @@ int forward_splits(const XDims& d) {
 // Where the kernels for few query rows (xattn_rows.cuh) take a call: how many rows a CTA holds, or 0. Their time grows
 // with the rows of a key head's group, that of the tiled kernels with its heads. Both sides measured:
 //   fp32 forward, up to 32 queries per head (a tile holds 128): 64 x 16 heads, 4096 keys of 64, 8 queries: 702 against
-//     3850 us; the queries behind the last whole tile where they are no more (8 x 8 heads, 130 queries, 517 keys of 48:
-//     106 -> 78 us); backward, a group of up to 8 rows: 64 x 15 / 5 heads, 2 queries, 11785 keys of 64: 2.2 against 27.6 ms.
-//   bf16 forward, one query per head: with K and V of at most 32 MB and no shared key heads (1 x 16 heads, 512 keys of
-//     192: 14.1 against 16.6 us; but 32 x 16, 4096 of 128: 234 against 166 us), or with a bias and shared key heads,
-//     whose rows the tiles do not pack (128 x 16 / 8 heads, 512 keys of 128: 79 against 100 us; groups of 8: 209
-//     against 376).
+//     3850 us; the queries behind the last whole tile where they are no more (8 x 8 heads, 130 queries, 517 keys of
+//     48: 106 -> 78 us); backward, a group of up to 8 rows: 64 x 15 / 5 heads, 2 queries, 11785 keys of 64: 2.2 against
+//     27.6 ms.
+//   bf16 forward, one row and K and V of at most 32 MB: 1 x 16 heads, 512 keys of 192: 14.1 against 16.6 us; but 32 x
+//     16, 4096 of 128: 234 against 166 us, and rows of heads that share a key head go into one tile: 128 x 16 / 8 heads,
+//     512 keys of 128: 79 against 62 us.
 //   bf16 backward, one query per head: a head dim of at most 64 (32 x 16 heads of one key head each, 2048 keys: 236
 //     against 279 us; groups of 8: 507 against 852), a bias and shared key heads (groups of 4, 2048 keys of 128: 799
 //     against 969 us), or fewer heads than SMs, which dQ's tiles cannot fill (1 x 16 heads, 16384 keys of 128: 157
@@ -76,11 +80,7 @@ int rows_of(long long rows) { return rows > 4 ? kRowMax : rows > 2 ? 4 : (int)ro
 int forward_rows_of(const XDims& d) {
   const long long rows = (long long)d.G * (d.tail ? d.tail : d.Nq);
   if (d.tail) return rows_of(rows);
-  if (d.bf16) {
-    const bool small = d.G == 1 && (long long)d.B * d.Hkv * d.Nk * d.D <= 8 << 20;
-    const bool unpacked = d.T && d.G > 1 && rows <= kRowMax;
-    return d.Nq == 1 && (small || unpacked) ? rows_of(rows) : 0;
-  }
+  if (d.bf16) return rows == 1 && (long long)d.B * d.Hkv * d.Nk * d.D <= 8 << 20 ? 1 : 0;
   return d.Nq <= 32 || rows <= kRowMax ? rows_of(rows) : 0;
 }
 int backward_rows_of(const XDims& d) {
@@ -285,7 +285,8 @@ int forward_rows(const XParams& p, const XDims& d, cudaStream_t st) {
     constexpr int NV = decltype(nv)::value, R = decltype(r)::value;
     const long long grid = d.row_ctas * d.splits;
     if (!d.bf16) return xlaunch(xattn_rows_fwd_kernel<float, NV, R>, grid, kRowThreads, 0, st, p);
-    return xlaunch(xattn_rows_fwd_kernel<__nv_bfloat16, NV, R>, grid, kRowThreads, 0, st, p);
+    if constexpr (R == 1) return xlaunch(xattn_rows_fwd_kernel<__nv_bfloat16, NV, R>, grid, kRowThreads, 0, st, p);
+    return (int)GEOATTN_ERR_UNSUPPORTED;  // forward_rows_of gives bf16 no other R
   });
 }
 template <class E>
@@ -326,8 +327,9 @@ int tc_launch(K kernel, long long grid, int threads, int smem, cudaStream_t st, 
 template <int DP>
 int tc_fwd(const xa::XMaps& maps, const XParams& p, long long grid, cudaStream_t st) {
   using C = xa::FwdCfg<DP>;
-  auto fwd = p.ids ? (p.drop_thr ? xa::xattn_fwd_kernel<DP, true, true> : xa::xattn_fwd_kernel<DP, true, false>)
-                   : (p.drop_thr ? xa::xattn_fwd_kernel<DP, false, true> : xa::xattn_fwd_kernel<DP, false, false>);
+  auto fwd = !p.ids ? (p.drop_thr ? xa::xattn_fwd_kernel<DP, 0, true> : xa::xattn_fwd_kernel<DP, 0, false>)
+             : p.pack ? (p.drop_thr ? xa::xattn_fwd_kernel<DP, 2, true> : xa::xattn_fwd_kernel<DP, 2, false>)
+                      : (p.drop_thr ? xa::xattn_fwd_kernel<DP, 1, true> : xa::xattn_fwd_kernel<DP, 1, false>);
   return tc_launch(fwd, grid, C::THREADS, C::SMEM, st, maps, p);
 }
 

@@ -155,7 +155,8 @@ __device__ __forceinline__ bool vec_rows(const XTensor& t) {
 // fp32): one barrier per chunk tells the two warps of 32 rows whether any of them has to move, and only then do they
 // exchange their maxima and rescale O, after O's product c - 1 (the only one that can be in flight: S(c) was issued
 // after c - 2).
-// Few queries of heads that share a key head (G * Nq <= 128) are packed into one tile's rows.
+// Few queries of heads that share a key head (G * Nq <= 128) are packed into one tile's rows, each with its head's bias
+// table.
 // DP = 192 has room for one score buffer and one chunk of K and V; S(c + 1) then follows O's product c.
 // Measured: 256x16x512x512x128 with the bias 886 us (620 TFLOP/s, 2.8x its products' time), 32x16x700x512x64 with the
 // bias and a mask 192 us, 1x8x4096x8192x128 160 us (859 TFLOP/s; 237 with dropout), 32x16x512x512x192 with bias and
@@ -170,14 +171,18 @@ struct FwdCfg {
   static constexpr int NKV = DP == 192 ? 1 : DP == 128 ? 2 : 4;  // chunks of K, and of V, in flight
   static constexpr int Q_BYTES = DP / 64 * 128 * 128, KV_BYTES = DP / 64 * 64 * 128;
   static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + NKV * KV_BYTES, OFF_TAB = OFF_V + NKV * KV_BYTES;
-  static constexpr int OFF_ROW = OFF_TAB + 512;                  // [2][128] floats: what the warpgroups exchange
+  static constexpr int OFF_ROW = OFF_TAB + 4224;                 // [2][128] floats: what the warpgroups exchange
   static constexpr int SMEM = OFF_ROW + 1024;
   static constexpr int TM_S = 0, TM_O = NSB * 64, TM_COLS = 256;
   static constexpr int EWT = 256, THREADS = EWT + 64, TMA_WARP = 8, MMA_WARP = 9;
 };
 constexpr float kLazy = 8.f;
+constexpr int kPackTables = 16;                     // heads of a packed tile that has a bias
+constexpr int kTableBytes = (kMaxBuckets + 1) * 4;  // -inf behind the buckets
+static_assert(kPackTables * kTableBytes <= 4224, "");
 
-template <int DP, bool BIAS, bool DROP>
+// BIAS: 0 none, 1 the head's table, 2 a packed tile's tables (a row has its head's)
+template <int DP, int BIAS, bool DROP>
 __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant__ XMaps maps, const XParams p) {
   using C = FwdCfg<DP>;
   constexpr int NKV = C::NKV, NSB = C::NSB;
@@ -218,8 +223,10 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
     tmem_alloc(&tmem_sh, C::TM_COLS);
     tmem_relinquish();
   }
-  if (BIAS && threadIdx.x <= kMaxBuckets)
-    reinterpret_cast<float*>(xsmem + C::OFF_TAB)[threadIdx.x] = table_log2(p, hx, threadIdx.x);
+  if (BIAS)
+    for (int x = threadIdx.x; x < (BIAS == 2 ? p.G : 1) * (kMaxBuckets + 1); x += C::THREADS)
+      reinterpret_cast<float*>(xsmem + C::OFF_TAB)[x] =
+          table_log2(p, BIAS == 2 ? kh * p.G + x / (kMaxBuckets + 1) : hx, x % (kMaxBuckets + 1));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -276,6 +283,7 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
     const int h = pack ? kh * p.G + r / p.Nq : hx;
     const bool row = pack ? r < p.G * p.Nq : i < p.Nq;
     const bool any_row = __any_sync(0xffffffffu, row);
+    const int tab = C::OFF_TAB + (BIAS == 2 && row ? r / p.Nq * kTableBytes : 0);
     const int bh = b * p.H + h;
     const AttnDrop drop = attn_drop(p.rng, DROP ? p.drop_thr : 0, p.drop_scale);
     const uint32_t thr2 = drop.pair();
@@ -309,7 +317,10 @@ __global__ void __launch_bounds__(320, 2) xattn_fwd_kernel(const __grid_constant
         if (BIAS) {
           const uint32_t* w = reinterpret_cast<const uint32_t*>(id);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = fmaf(x[e], p.scale_log2, table_at(C::OFF_TAB, e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xFFFF));
+          for (int e = 0; e < 32; ++e) {
+            const uint32_t o = e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xFFFF;
+            x[e] = fmaf(x[e], p.scale_log2, table_at(BIAS == 2 ? tab : C::OFF_TAB, o));
+          }
         }
         if (live != ~0u) {
 #pragma unroll

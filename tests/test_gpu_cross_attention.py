@@ -476,11 +476,12 @@ def test_query_counts_around_the_chunks():
             check(x, kw, p=0.1, key=[Nq, D])
 
 
-FEW = [  # B, H, Hkv, Nq, Nk, D: few query rows per key head, every row count of a CTA, one and several key ranges
-    (3, 2, 2, 1, 1, 64), (2, 2, 2, 1, 63, 40), (1, 2, 2, 1, 1100, 64), (2, 4, 2, 1, 2051, 128), (1, 3, 1, 1, 1030, 192),
-    (2, 6, 2, 1, 130, 100), (1, 5, 1, 1, 1500, 61), (2, 8, 1, 1, 700, 192), (1, 2, 2, 2, 1029, 128), (2, 4, 1, 2, 90, 64),
-    (2, 2, 2, 7, 300, 175), (1, 2, 2, 8, 1025, 64), (2, 3, 3, 9, 70, 64), (1, 6, 2, 28, 1200, 192), (1, 8, 1, 32, 130, 33),
-    (2, 2, 1, 31, 1, 128),
+FEW = [  # B, H, Hkv, Nq, Nk, D: few query rows per key head: every row count of a CTA, packed tiles, key ranges
+    (3, 2, 2, 1, 1, 64), (2, 2, 2, 1, 63, 40), (1, 2, 2, 1, 1100, 64), (2, 4, 2, 1, 2051, 128),
+    (1, 3, 1, 1, 1030, 192), (2, 6, 2, 1, 130, 100), (1, 5, 1, 1, 1500, 61), (2, 8, 1, 1, 700, 192),
+    (1, 2, 2, 2, 1029, 128), (2, 4, 1, 2, 90, 64), (2, 2, 2, 7, 300, 175), (1, 2, 2, 8, 1025, 64),
+    (2, 3, 3, 9, 70, 64), (1, 6, 2, 28, 1200, 192), (1, 8, 1, 32, 130, 33), (2, 2, 1, 31, 1, 128),
+    (2, 16, 1, 8, 300, 64), (1, 17, 1, 3, 200, 64), (1, 32, 2, 5, 1500, 128), (2, 6, 2, 42, 130, 192),
 ]
 
 
