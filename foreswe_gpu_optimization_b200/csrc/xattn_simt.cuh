@@ -5,10 +5,11 @@
 // keys) are one or two 16-byte loads per d; each of the 256 threads (16 x 16) owns a register block of the product and
 // works on it two values at a time (fma.rn.f32x2). Weights go through shared memory between the two products, in
 // 16-byte chunks whose place is XORed with the writing lane so that neither side meets a bank conflict.
-// Bound by shared memory's return path (one 32-bit word per lane and clock: as long as the products themselves) and,
+// Bound by shared memory's return path (one 32-bit word per lane and clock: longer than the products themselves) and,
 // above D = 64, by the latency that 8 warps per SM cannot hide. 32 x 8 heads x 512 x 512 x 64 with the bias: forward
-// 542 us (32 TFLOP/s of 74), key pass 1163 us (30), dQ 290 us (30); at D = 175 forward and key pass run at 19 and 18. Fetching
-// the next query tile during the products changed nothing there.
+// 542 us (32 TFLOP/s of 74), key pass 1120 us (31), dQ 290 us (30); 8 x 16 / 2 heads, 415 x 1441 of 175 with dropout and
+// the bias: forward 2.1 ms (26), key pass 4.8 ms (22). Fetching the next query tile during the products changed nothing
+// there.
 #pragma once
 #include <type_traits>
 
@@ -356,10 +357,15 @@ __global__ void __launch_bounds__(256) xattn_delta_kernel(const XParams p) {
 // ---------------------------------------------------------------------------------------------------------------
 // Backward, key pass: one CTA per (TK keys, key head, batch); loops over the heads that share the key head and their
 // 64-row query tiles. dK and dV stay in registers (no atomics: fixed order); dS^T goes to the scratch.
+// Half of the threads form the scores and the others dP, in blocks of 8 x 4 (4 x 4 above D = 128), and exchange them
+// through the weights' place in shared memory: fewer words per product than both in every thread's blocks of half the
+// size (173 heads, 327 x 40 of 158: 343 -> 277 us; 32 x 8 heads x 512 x 512 x 64: 1163 -> 1120 us).
 // ---------------------------------------------------------------------------------------------------------------
 template <int DP>
 struct SimtBwd {
   static constexpr int TK = DP <= 128 ? 64 : 32, KT = TK / 16, BQ = 64, SK = TK + 4, SQ = BQ + 4;
+  static constexpr int QR = TK / 8;         // a thread's queries in the first products, by 4 keys
+  static constexpr int XN = 16 * 64 / TK;   // threads across the columns in the second ones, 4 keys each
   static constexpr int FLOATS = 2 * DP * SK + 2 * DP * SQ + 2 * TK * BQ + 256 + TK + 3 * BQ;
   static constexpr int SMEM = FLOATS * 4;
 };
@@ -367,7 +373,7 @@ struct SimtBwd {
 template <int DP>
 __global__ void __launch_bounds__(kSimtThreads, DP == 64 ? 2 : 1) xattn_simt_bwd_keys_kernel(const XParams p) {
   using C = SimtBwd<DP>;
-  constexpr int KT = C::KT, NC = DP / 16;
+  constexpr int KT = C::KT, XN = C::XN, NC = DP / XN, QR = C::QR;
   extern __shared__ float4 simt_smem[];
   float* kt = reinterpret_cast<float*>(simt_smem);
   float* vt = kt + DP * C::SK;
@@ -386,9 +392,13 @@ __global__ void __launch_bounds__(kSimtThreads, DP == 64 ? 2 : 1) xattn_simt_bwd
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   const int n = key_count(p, b);
   const AttnDrop drop = attn_drop(p.rng, p.drop_thr, p.drop_scale);
-  uint64_t ak[KT][NC], av[KT][NC];  // sums over even and odd queries
+  // first products: half of the threads form the scores, the others dP
+  const int part = threadIdx.x / 128, py = threadIdx.x % 128 / (C::TK / 4), px = threadIdx.x % (C::TK / 4);
+  const float *rows = part ? gt : qt, *cols = part ? vt : kt;
+  const int ny = threadIdx.x / XN, nx = threadIdx.x % XN;  // second products: keys 4 ny .., columns nx + XN c
+  uint64_t ak[4][NC], av[4][NC];  // sums over even and odd queries
 #pragma unroll
-  for (int x = 0; x < KT; ++x)
+  for (int x = 0; x < 4; ++x)
 #pragma unroll
     for (int c = 0; c < NC; ++c) ak[x][c] = av[x][c] = 0;
 
@@ -429,39 +439,45 @@ __global__ void __launch_bounds__(kSimtThreads, DP == 64 ? 2 : 1) xattn_simt_bwd
         y.template put_t<C::SQ>(gt);
       }
       __syncthreads();
-      uint64_t s2[2][KT] = {}, dp2[2][KT] = {};  // pairs of queries
+      {
+        uint64_t x2[QR / 2][4] = {};  // pairs of queries
 #pragma unroll 4
-      for (int d = 0; d < DP; ++d) {
-        const ulonglong2 q2 = *reinterpret_cast<const ulonglong2*>(qt + d * C::SQ + ty * 4);
-        const ulonglong2 g2 = *reinterpret_cast<const ulonglong2*>(gt + d * C::SQ + ty * 4);
-        float kk[KT], vv[KT];
-        if constexpr (KT == 4) {
-          const float4 k4 = *reinterpret_cast<const float4*>(kt + d * C::SK + tx * 4);
-          const float4 v4 = *reinterpret_cast<const float4*>(vt + d * C::SK + tx * 4);
-          kk[0] = k4.x, kk[1] = k4.y, kk[2] = k4.z, kk[3] = k4.w;
-          vv[0] = v4.x, vv[1] = v4.y, vv[2] = v4.z, vv[3] = v4.w;
-        } else {
-          const float2 k2 = *reinterpret_cast<const float2*>(kt + d * C::SK + tx * 2);
-          const float2 v2 = *reinterpret_cast<const float2*>(vt + d * C::SK + tx * 2);
-          kk[0] = k2.x, kk[1] = k2.y, vv[0] = v2.x, vv[1] = v2.y;
+        for (int d = 0; d < DP; ++d) {
+          uint64_t a[QR / 2];
+#pragma unroll
+          for (int u = 0; u < QR / 4; ++u) {
+            const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(rows + d * C::SQ + py * QR + u * 4);
+            a[2 * u] = v.x, a[2 * u + 1] = v.y;
+          }
+          const float4 k4 = *reinterpret_cast<const float4*>(cols + d * C::SK + px * 4);
+          const uint64_t kk[4] = {f2(k4.x, k4.x), f2(k4.y, k4.y), f2(k4.z, k4.z), f2(k4.w, k4.w)};
+#pragma unroll
+          for (int u = 0; u < QR / 2; ++u)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x2[u][c] = fma2(a[u], kk[c], x2[u][c]);
         }
 #pragma unroll
-        for (int c = 0; c < KT; ++c) {
-          const uint64_t k2 = f2(kk[c], kk[c]), v2 = f2(vv[c], vv[c]);
-          s2[0][c] = fma2(q2.x, k2, s2[0][c]);
-          s2[1][c] = fma2(q2.y, k2, s2[1][c]);
-          dp2[0][c] = fma2(g2.x, v2, dp2[0][c]);
-          dp2[1][c] = fma2(g2.y, v2, dp2[1][c]);
+        for (int c = 0; c < 4; ++c) {
+          const int key = px * 4 + c;
+          float* dst = (part ? st : pt) + key * C::BQ;
+#pragma unroll
+          for (int u = 0; u < QR / 4; ++u) {
+            float4 v;
+            unf2(x2[2 * u][c], v.x, v.y);
+            unf2(x2[2 * u + 1][c], v.z, v.w);
+            *reinterpret_cast<float4*>(dst + ((py * (QR / 4) + u) ^ (key / KT & 7)) * 4) = v;
+          }
         }
       }
+      __syncthreads();
       float s[4][KT], dp[4][KT];
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int c = 0; c < KT; ++c) {
-          unf2(s2[r][c], s[2 * r][c], s[2 * r + 1][c]);
-          unf2(dp2[r][c], dp[2 * r][c], dp[2 * r + 1][c]);
-        }
+      for (int c = 0; c < KT; ++c) {
+        const int at = (tx * KT + c) * C::BQ + (ty ^ (tx & 7)) * 4;
+        const float4 u = *reinterpret_cast<const float4*>(pt + at), v = *reinterpret_cast<const float4*>(st + at);
+        s[0][c] = u.x, s[1][c] = u.y, s[2][c] = u.z, s[3][c] = u.w;
+        dp[0][c] = v.x, dp[1][c] = v.y, dp[2][c] = v.z, dp[3][c] = v.w;
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = i0 + ty * 4 + r;
@@ -500,19 +516,19 @@ __global__ void __launch_bounds__(kSimtThreads, DP == 64 ? 2 : 1) xattn_simt_bwd
       }
 #pragma unroll 2
       for (int r = 0; r < C::BQ / 4; ++r) {
-        ulonglong2 pp[KT], ss[KT];
+        ulonglong2 pp[4], ss[4];
 #pragma unroll
-        for (int x = 0; x < KT; ++x) {
-          const int at = (ty * KT + x) * C::BQ + (r ^ (ty & 7)) * 4;
+        for (int x = 0; x < 4; ++x) {
+          const int key = ny * 4 + x, at = key * C::BQ + (r ^ (key / KT & 7)) * 4;
           pp[x] = *reinterpret_cast<const ulonglong2*>(pt + at);
           ss[x] = *reinterpret_cast<const ulonglong2*>(st + at);
         }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          const ulonglong2 g2 = *reinterpret_cast<const ulonglong2*>(gt + (tx + 16 * c) * C::SQ + r * 4);
-          const ulonglong2 q2 = *reinterpret_cast<const ulonglong2*>(qt + (tx + 16 * c) * C::SQ + r * 4);
+          const ulonglong2 g2 = *reinterpret_cast<const ulonglong2*>(gt + (nx + XN * c) * C::SQ + r * 4);
+          const ulonglong2 q2 = *reinterpret_cast<const ulonglong2*>(qt + (nx + XN * c) * C::SQ + r * 4);
 #pragma unroll
-          for (int x = 0; x < KT; ++x) {
+          for (int x = 0; x < 4; ++x) {
             av[x][c] = fma2(pp[x].x, g2.x, fma2(pp[x].y, g2.y, av[x][c]));
             ak[x][c] = fma2(ss[x].x, q2.x, fma2(ss[x].y, q2.y, ak[x][c]));
           }
@@ -521,14 +537,14 @@ __global__ void __launch_bounds__(kSimtThreads, DP == 64 ? 2 : 1) xattn_simt_bwd
     }
   }
 #pragma unroll
-  for (int x = 0; x < KT; ++x) {
-    const int j = j0 + ty * KT + x;
+  for (int x = 0; x < 4; ++x) {
+    const int j = j0 + ny * 4 + x;
     if (j >= p.Nk) continue;
     float* dK = reinterpret_cast<float*>(p.dk.p) + b * p.dk.s[0] + kh * p.dk.s[1] + (long long)j * p.dk.s[2];
     float* dV = reinterpret_cast<float*>(p.dv.p) + b * p.dv.s[0] + kh * p.dv.s[1] + (long long)j * p.dv.s[2];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int d = tx + 16 * c;
+      const int d = nx + XN * c;
       if (d < p.D) {
         float e, o;
         unf2(ak[x][c], e, o);
